@@ -162,8 +162,7 @@ def prepare(c, seed):
         sharp = torch.exp(0.7 * torch.randn(1, hq, 1, generator=g, device=dev))   # flat heads and peaked ones
         s["q"] = (torch.randn(rows, hq, HEAD, generator=g, device=dev) * sharp).to(dt).view(rows, hq * HEAD)
         s["dtype"] = dt
-        s["op"] = c["op"]
-        return s
+        return _handle(s, c)
     if c["op"] == "store":
         runs, h, blocks = c["runs"], c["heads"], c["blocks"]
         slots = runs + 3
@@ -180,8 +179,7 @@ def prepare(c, seed):
         loud = torch.exp(0.8 * torch.randn(3 * d, generator=g, device=dev))   # keys have a few loud channels
         rowsin = (torch.randn(rows, 3 * d, generator=g, device=dev) * loud).to(dt)   # a fused product: q | k | v
         s["new_k"], s["new_v"] = rowsin[:, d:2 * d], rowsin[:, 2 * d:]
-        s["op"] = c["op"]
-        return s
+        return _handle(s, c)
     n, k, grp = c["n"], c["k"], c["group"]
     kp = (k + SEGMENT - 1) // SEGMENT * SEGMENT
     q = (torch.randn(n, kp, generator=g, device=dev) * 2.5).round().clamp(-8, 7).to(torch.int32) + 8
@@ -190,7 +188,20 @@ def prepare(c, seed):
     s["x"] = torch.randn(c["rows"], k, generator=g, device=dev).to(dt)
     s["bias"] = (0.1 * torch.randn(n, generator=g, device=dev)).to(dt)
     s["residual"] = torch.randn(c["rows"], n, generator=g, device=dev) if c["accumulate"] else None
-    s["group"], s["k"], s["op"] = grp, k, c["op"]
+    s["group"], s["k_in"] = grp, k
+    return _handle(s, c)
+
+
+def _handle(s, c):
+    """The objects that a program of this framework keeps: its engine, and its cache or weights by their tensors."""
+    s["op"] = c["op"]
+    if own:
+        from whisperdrz_b200.lowbit import PackedLinear, QCache
+        s["engine"] = _engine()
+        if c["op"] == "linear":
+            s["weights"] = PackedLinear(s["w"], s["w_scale"], s["k_in"], s["group"], s["bias"])
+        else:
+            s["cache"] = QCache(s["k"], s["v"], s["k_scale"], s["v_scale"])
     return s
 
 
@@ -290,7 +301,7 @@ def _linear_plain(s):
     shift = 4 * torch.arange(4, device=words.device, dtype=torch.int32).view(4, 1) + torch.tensor([0, 16], device=words.device, dtype=torch.int32)
     q = ((words[..., None, None] >> shift) & 15).reshape(n, kp) - 8
     w = q.float().view(n, -1, s["group"]) * s["w_scale"].float()[..., None]
-    y = s["x"].float() @ w.view(n, kp)[:, :s["k"]].T + s["bias"].float()
+    y = s["x"].float() @ w.view(n, kp)[:, :s["k_in"]].T + s["bias"].float()
     if s["residual"] is not None:
         y = y + s["residual"]
     return y
@@ -312,12 +323,10 @@ def _engine():
 
 
 def _run_own(s):
-    from whisperdrz_b200.lowbit import PackedLinear, QCache
-    e = _engine()
+    e = s["engine"]
     if s["op"] == "linear":
-        w = PackedLinear(s["w"], s["w_scale"], s["k"], s["group"], s["bias"])
-        return e.linear_rows_packed(s["x"], w, residual=s["residual"])
-    cache = QCache(s["k"], s["v"], s["k_scale"], s["v_scale"])
+        return e.linear_rows_packed(s["x"], s["weights"], residual=s["residual"])
+    cache = s["cache"]
     if s["op"] == "attend":
         return e.qcache_attention(s["q"], cache, s["slots"], s["lens"], out_dtype=s["dtype"])
     e.qcache_store(cache, s["new_k"], s["new_v"], s["slots"], s["positions"], row_begin=s["row_begin"], max_run=s["max_run"])
