@@ -304,6 +304,55 @@ int wdz_dtw(wdz_engine* e, const float* matrix_dev, int64_t chunk_stride, int64_
             int limit_stride, int n_chunks, int max_rows, int max_cols, int32_t* text_idx_out_dev,
             int32_t* time_idx_out_dev, int32_t* path_len_out_dev, wdz_stream s);
 
+/* ---- 8-bit key/value cache and 4-bit weights: a decode step's two byte streams in fewer bits ------------
+ * No counterpart in the reference, whose FlashKVCache (model.py:98-147) and nn.Linear hold 16 or 32 bits.
+ * The operators stand beside wdz_cross_kv / the decode step's attention and wdz_linear_rows; they work on
+ * caller-held memory of any head count, need an engine only for its device, status word and error text, and
+ * take no scratch.  All index arrays are device int32; rows are given by a pointer to row 0 and the elements
+ * from one row to the next, rows and caches start on 16 bytes, and heads have 64 values.
+ *
+ * The cache: value(slot, head, token, c) = int8 * scale of the token's block of WDZ_QCACHE_BLOCK tokens.
+ *   k_dev / v_dev              int8 [n_slots][n_heads][n_blocks * 64][64], slot_stride values from slot to slot
+ *   k_scale_dev / v_scale_dev  f32  [n_slots][n_heads][n_blocks], scale_slot_stride scales from slot to slot */
+#define WDZ_QCACHE_BLOCK 64
+typedef struct wdz_qcache {
+  void *k_dev, *v_dev;
+  float *k_scale_dev, *v_scale_dev;
+  int64_t slot_stride, scale_slot_stride;
+  int32_t n_slots, n_heads, n_blocks;
+} wdz_qcache;
+/* Rounds rows into the cache.  Run i is rows [row_begin_dev[i], row_begin_dev[i + 1]) (NULL: row i alone), which
+ * go to tokens positions_dev[i], positions_dev[i] + 1, ... of slot slot_ids_dev[i].  k_dev / v_dev: dtype
+ * [n_rows][n_heads * 64].  For each block that a run reaches, K and V apart, with a = max |x| over the run's
+ * values in the block and head:
+ *   scale' = max(scale, a / 127) where the run enters the block behind its first token, else a / 127
+ *   q = rint(x / scale'), half to even (the quotient is rounded exactly)
+ *   tokens of the block before the run: q' = rint(q * scale / scale') where the scale grew
+ * Tokens behind the run keep their bytes, which are void until written.  An infinity is stored as the largest
+ * value and a NaN as zero, without part in the scale, and the status word says WDZ_ENAN; a < 2^-119 stores
+ * zeros.  Runs of slots outside [0, n_slots) are skipped.  A run outside the rows or the slot, and every run but
+ * the last of several that name one slot, is not stored and the status word says WDZ_EINVAL.  max_run: the longest
+ * run's length, as far as the host knows it (it sizes the launch, no more). */
+int wdz_qcache_store(wdz_engine* e, const wdz_qcache* cache, const void* k_dev, int64_t ldk, const void* v_dev, int64_t ldv,
+                     int dtype, int n_rows, const int32_t* row_begin_dev, const int32_t* slot_ids_dev,
+                     const int32_t* positions_dev, int n_runs, int max_run, wdz_stream s);
+/* Row r's n_q_heads queries (q_dtype [n_rows][n_q_heads * 64]) attend to the first lens_dev[r] tokens of slot
+ * slot_ids_dev[r]: out = softmax(scale * q k^T) v, query head h over key head h / (n_q_heads / n_heads), at most 8
+ * query heads to a key head.  fp32 or better throughout; out_dtype [n_rows][n_q_heads * 64].  Lengths are clamped
+ * to the slot; a row of length 0 gives zeros; a row whose slot is outside [0, n_slots) is left as it was, or
+ * zeroed when clear_skipped != 0. */
+int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_dev, int64_t ldq, int q_dtype, int n_q_heads,
+                         const int32_t* slot_ids_dev, const int32_t* lens_dev, int n_rows, float scale, void* out_dev,
+                         int64_t ldo, int out_dtype, int clear_skipped, wdz_stream s);
+/* wdz_linear_rows with 4-bit weights: y f32 [M][N] = x[M][K] W^T (+ bias, x_dtype [N]) (+ residual f32 [M][N], which
+ * may be y), W[n][k] = (u - 8) * scale[n][k / group], group 32, 64 or 128.  w_dev: K is padded to Kp, a multiple of
+ * 128, with u = 8; row n is Kp / 8 32-bit words; of every 128 weights word 4 t + i (t, i < 4) holds elements
+ * 32 i + 8 t + 0..7, element 2 j in its bits 4 j, element 2 j + 1 in its bits 4 (j + 4).  scale_dev: bf16
+ * [N][Kp / group].  w_dev starts on 16 bytes, scale_dev on 8; x rows may have any alignment. */
+int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_dtype, int M, int K, const void* w_dev,
+                           const void* scale_dev, int group, const void* bias_dev, const float* residual_dev, int N,
+                           float* y_dev, wdz_stream s);
+
 #ifdef __cplusplus
 }
 #endif

@@ -47,6 +47,15 @@ class RuleDesc(C.Structure):
 
 assert C.sizeof(RuleDesc) == 128
 
+
+class QCacheDesc(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("slot_stride", C.c_int64), ("scale_slot_stride", C.c_int64),
+                ("n_slots", C.c_int32), ("n_heads", C.c_int32), ("n_blocks", C.c_int32)]
+
+
+QCACHE_BLOCK = 64
+
 # name -> (restype, argtypes); every symbol include/wdz.h declares
 P, I, I64, SZ = C.c_void_p, C.c_int, C.c_int64, C.c_size_t
 SYMBOLS = {
@@ -85,6 +94,9 @@ SYMBOLS = {
     "wdz_align_configure": (I, [P, P, I]),
     "wdz_align_capacity": (I, [P, I]),
     "wdz_align_matrix": (I, [P, P, P, P, P, I, I, P, P]),
+    "wdz_qcache_store": (I, [P, C.POINTER(QCacheDesc), P, I64, P, I64, I, I, P, P, P, I, I, P]),
+    "wdz_qcache_attention": (I, [P, C.POINTER(QCacheDesc), P, I64, I, I, P, P, I, C.c_float, P, I64, I, I, P]),
+    "wdz_linear_rows_packed": (I, [P, P, I64, I, I, I, P, P, I, P, P, I, P, P]),
     "wdz_dtw": (I, [P, P, I64, I64, P, P, P, P, P, I, I, I, I, P, P, P, P]),
 }
 

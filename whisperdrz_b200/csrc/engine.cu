@@ -24,6 +24,8 @@
 #include "logmel.cuh"
 #include "rules.cuh"
 #include "align.cuh"
+#include "qcache.cuh"
+#include "gemv_packed.cuh"
 #ifdef WDZ_WITH_TC
 #include "gemm_tc.cuh"
 #include "gemm_tc2.cuh"
@@ -1825,6 +1827,131 @@ int wdz_dtw(wdz_engine* e, const float* matrix_dev, int64_t chunk_stride, int64_
   dtw_kernel<<<n_chunks, 512, dtw_smem_bytes(max_rows, max_cols), (cudaStream_t)s>>>(p);
   e->launches += 1;
   WDZ_LAUNCH_CHECK(e, "dtw");
+  return WDZ_OK;
+}
+
+// ---- 8-bit key/value cache and 4-bit linear layer -------------------------------
+namespace {
+
+// The engine's device for the length of a call, whichever device is current on the calling thread.
+struct DeviceScope {
+  int before = -1;
+  explicit DeviceScope(int device) {
+    if (cudaGetDevice(&before) != cudaSuccess) { cudaGetLastError(); before = -1; }
+    if (before == device || cudaSetDevice(device) != cudaSuccess) { cudaGetLastError(); before = -1; }
+  }
+  ~DeviceScope() { if (before >= 0) cudaSetDevice(before); }
+};
+
+bool aligned16(const void* p, int64_t stride_bytes) { return (((uintptr_t)p) & 15) == 0 && (stride_bytes & 15) == 0; }
+
+int qcache_view(wdz_engine* e, const char* who, const wdz_qcache* c, QcView* v) {
+  if (!c || !c->k_dev || !c->v_dev || !c->k_scale_dev || !c->v_scale_dev) return e->fail(WDZ_EINVAL, "%s: null cache", who);
+  if (c->n_slots < 1 || c->n_heads < 1 || c->n_heads > 4096 || c->n_blocks < 1 || c->n_blocks > (INT32_MAX >> 6) - 1)
+    return e->fail(WDZ_EINVAL, "%s: a cache of %d slots, %d heads, %d blocks", who, c->n_slots, c->n_heads, c->n_blocks);
+  const int64_t blocks = (int64_t)c->n_heads * c->n_blocks;
+  if (c->slot_stride < blocks * QC_BLOCK * QC_HD || c->scale_slot_stride < blocks)
+    return e->fail(WDZ_EINVAL, "%s: the slots of the cache overlap", who);
+  if (!aligned16(c->k_dev, c->slot_stride) || !aligned16(c->v_dev, c->slot_stride))
+    return e->fail(WDZ_EINVAL, "%s: the cache's values must start on 16 bytes", who);
+  *v = QcView{(int8_t*)c->k_dev, (int8_t*)c->v_dev, c->k_scale_dev, c->v_scale_dev, c->slot_stride, c->scale_slot_stride,
+              c->n_slots, c->n_heads, c->n_blocks};
+  return WDZ_OK;
+}
+
+}  // namespace
+
+int wdz_qcache_store(wdz_engine* e, const wdz_qcache* cache, const void* k_dev, int64_t ldk, const void* v_dev, int64_t ldv,
+                     int dtype, int n_rows, const int32_t* row_begin_dev, const int32_t* slot_ids_dev,
+                     const int32_t* positions_dev, int n_runs, int max_run, wdz_stream s) {
+  if (!e) return WDZ_EINVAL;
+  int rc;
+  QcStoreParams p{};
+  if ((rc = qcache_view(e, "wdz_qcache_store", cache, &p.c))) return rc;
+  if (dtype != WDZ_F32 && dtype != WDZ_BF16) return e->fail(WDZ_EINVAL, "wdz_qcache_store: unknown type %d", dtype);
+  if (n_rows < 0 || n_rows > INT32_MAX / 2 || n_runs < 0 || max_run < 0 || (!row_begin_dev && n_runs != n_rows))
+    return e->fail(WDZ_EINVAL, "wdz_qcache_store: %d rows in %d runs", n_rows, n_runs);
+  if (n_rows == 0 || n_runs == 0) return WDZ_OK;
+  if (n_runs > 65535) return e->fail(WDZ_ECAPACITY, "wdz_qcache_store: %d runs in one call, at most 65535", n_runs);
+  const int64_t esz = dtype == WDZ_BF16 ? 2 : 4;
+  const int64_t width = (int64_t)p.c.n_heads * QC_HD;
+  if (!k_dev || !v_dev || !slot_ids_dev || !positions_dev) return e->fail(WDZ_EINVAL, "wdz_qcache_store: null argument");
+  if ((ldk < width || ldv < width) && n_rows > 1) return e->fail(WDZ_EINVAL, "wdz_qcache_store: rows overlap");
+  if (!aligned16(k_dev, ldk * esz) || !aligned16(v_dev, ldv * esz))
+    return e->fail(WDZ_EINVAL, "wdz_qcache_store: rows must start on 16 bytes");
+  p.k = k_dev; p.v = v_dev; p.ldk = ldk; p.ldv = ldv;
+  p.n_rows = n_rows; p.n_runs = n_runs;
+  p.row_begin = row_begin_dev; p.slots = slot_ids_dev; p.positions = positions_dev;
+  if ((rc = check_ready(e))) return rc;
+  DeviceScope on(e->device);
+  if (max_run > n_rows) max_run = n_rows;
+  int blocks = row_begin_dev ? (max_run + 2 * QC_BLOCK - 2) / QC_BLOCK : 1;   // a run may start at a block's last token
+  if (blocks < 1) blocks = 1;
+  if (blocks > p.c.n_blocks) blocks = p.c.n_blocks;
+  const dim3 grid(blocks, 2 * p.c.n_heads, n_runs);
+  if (dtype == WDZ_BF16) launch_pdl(e, qcache_store_kernel<bf16>, grid, dim3(64), 0, (cudaStream_t)s, p, e->status);
+  else launch_pdl(e, qcache_store_kernel<float>, grid, dim3(64), 0, (cudaStream_t)s, p, e->status);
+  WDZ_LAUNCH_CHECK(e, "qcache_store");
+  return WDZ_OK;
+}
+
+int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_dev, int64_t ldq, int q_dtype, int n_q_heads,
+                         const int32_t* slot_ids_dev, const int32_t* lens_dev, int n_rows, float scale, void* out_dev,
+                         int64_t ldo, int out_dtype, int clear_skipped, wdz_stream s) {
+  if (!e) return WDZ_EINVAL;
+  int rc;
+  QcAttendParams p{};
+  if ((rc = qcache_view(e, "wdz_qcache_attention", cache, &p.c))) return rc;
+  if ((q_dtype != WDZ_F32 && q_dtype != WDZ_BF16) || (out_dtype != WDZ_F32 && out_dtype != WDZ_BF16))
+    return e->fail(WDZ_EINVAL, "wdz_qcache_attention: unknown type");
+  if (n_q_heads < 1 || n_q_heads % p.c.n_heads || n_q_heads / p.c.n_heads > 8)
+    return e->fail(WDZ_EINVAL, "wdz_qcache_attention: %d query heads over %d key heads (1 to 8 each)", n_q_heads, p.c.n_heads);
+  if (n_rows < 0) return e->fail(WDZ_EINVAL, "wdz_qcache_attention: %d rows", n_rows);
+  if (n_rows == 0) return WDZ_OK;
+  if (!q_dev || !out_dev || !slot_ids_dev || !lens_dev) return e->fail(WDZ_EINVAL, "wdz_qcache_attention: null argument");
+  const int64_t width = (int64_t)n_q_heads * QC_HD;
+  if ((ldq < width || ldo < width) && n_rows > 1) return e->fail(WDZ_EINVAL, "wdz_qcache_attention: rows overlap");
+  if (!aligned16(q_dev, ldq * (q_dtype == WDZ_BF16 ? 2 : 4)) || !aligned16(out_dev, ldo * (out_dtype == WDZ_BF16 ? 2 : 4)))
+    return e->fail(WDZ_EINVAL, "wdz_qcache_attention: rows must start on 16 bytes");
+  if (!(scale >= 0.0f) || scale > 3.0e38f) return e->fail(WDZ_EINVAL, "wdz_qcache_attention: scale %g", (double)scale);
+  p.q = q_dev; p.ldq = ldq; p.out = out_dev; p.ldo = ldo;
+  p.slots = slot_ids_dev; p.lens = lens_dev;
+  p.n_rows = n_rows; p.group = n_q_heads / p.c.n_heads; p.scale = scale; p.clear_skipped = clear_skipped != 0;
+  if ((rc = check_ready(e))) return rc;
+  DeviceScope on(e->device);
+  const dim3 grid((unsigned)(((int64_t)n_rows * n_q_heads + 3) / 4));
+  auto go = [&](auto kern) { launch_pdl(e, kern, grid, dim3(128), 0, (cudaStream_t)s, p); };
+  if (q_dtype == WDZ_BF16) { if (out_dtype == WDZ_BF16) go(qcache_attend_kernel<bf16, bf16>); else go(qcache_attend_kernel<bf16, float>); }
+  else { if (out_dtype == WDZ_BF16) go(qcache_attend_kernel<float, bf16>); else go(qcache_attend_kernel<float, float>); }
+  WDZ_LAUNCH_CHECK(e, "qcache_attend");
+  return WDZ_OK;
+}
+
+int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_dtype, int M, int K, const void* w_dev,
+                           const void* scale_dev, int group, const void* bias_dev, const float* residual_dev, int N,
+                           float* y_dev, wdz_stream s) {
+  if (!e) return WDZ_EINVAL;
+  int rc;
+  if (x_dtype != WDZ_F32 && x_dtype != WDZ_BF16) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: unknown type %d", x_dtype);
+  if (M < 0 || N < 1 || K < 1 || K > INT32_MAX - 128) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: %d x %d x %d", M, N, K);
+  if (group != 32 && group != 64 && group != 128) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: group %d (32, 64 or 128)", group);
+  if (M == 0) return WDZ_OK;
+  if (!x_dev || !w_dev || !scale_dev || !y_dev) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: null argument");
+  if (ldx < K && M > 1) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: rows overlap");
+  if (((uintptr_t)w_dev & 15) || ((uintptr_t)scale_dev & 7))
+    return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: weights must start on 16 bytes, scales on 8");
+  GemvPackedParams p{};
+  p.x = x_dev; p.ldx = ldx; p.W = (const uint32_t*)w_dev; p.scale = (const bf16*)scale_dev; p.bias = bias_dev;
+  p.residual = residual_dev; p.y = y_dev;
+  p.M = M; p.N = N; p.K = K; p.Kp = (K + 127) / 128 * 128; p.group = group;
+  if ((rc = check_ready(e))) return rc;
+  DeviceScope on(e->device);
+  const int sp = e->span_begin(WDZ_PROF_DEC_GEMM, (double)N * p.Kp * (0.5 + 2.0 / group), (cudaStream_t)s);
+  const dim3 grid((N + 3) / 4);
+  if (x_dtype == WDZ_BF16) launch_pdl(e, gemv_packed_kernel<bf16>, grid, dim3(128), 0, (cudaStream_t)s, p);
+  else launch_pdl(e, gemv_packed_kernel<float>, grid, dim3(128), 0, (cudaStream_t)s, p);
+  e->span_end(sp, (cudaStream_t)s);
+  WDZ_LAUNCH_CHECK(e, "gemv_packed");
   return WDZ_OK;
 }
 

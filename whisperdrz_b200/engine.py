@@ -11,6 +11,7 @@ import torch
 
 from . import capi, frontend
 from .dims import ModelDimensions
+from .lowbit import HEAD_DIM, PackedLinear, QCache
 
 _TORCH_DTYPE = {torch.float32: capi.WDZ_F32, torch.bfloat16: capi.WDZ_BF16}
 
@@ -111,6 +112,7 @@ class Engine:
         self.dims, self.dtype = dims, dtype
         self.device = torch.device(device)
         torch.cuda.set_device(self.device)
+        self._ordinal = torch.cuda.current_device()   # of a device given without its number, too
         self.n_slots = n_slots
         self.max_tokens = max_tokens or dims.n_text_ctx
         self.max_clips = max_clips
@@ -426,6 +428,142 @@ class Engine:
         self._check(self.lib.wdz_rules_argmax(self.h, logits.data_ptr(), None if rd is None else rd.data_ptr(),
                                               logits.shape[0], int(penalty), out.data_ptr(), self._stream()))
         return out
+
+    # ------------------------------------------------- 8-bit cache, 4-bit weights
+    def qcache(self, n_slots: int | None = None, n_tokens: int | None = None, n_heads: int | None = None) -> QCache:
+        """An empty 8-bit cache on the engine's device; by default the engine's slots, its encoder positions and the
+        decoder's heads (the shape of one layer's cross cache)."""
+        return QCache.empty(n_slots or self.n_slots, n_tokens or self.dims.n_audio_ctx, n_heads or self.dims.n_text_head,
+                            self.device)
+
+    def _rows(self, name: str, t: torch.Tensor, width: int) -> torch.Tensor:
+        """``t`` as rows [n, width] in a type and at places that the kernels take: no copy where it has them already."""
+        if t.dtype not in _TORCH_DTYPE:
+            raise ValueError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+        if t.dim() == 3:
+            t = t.flatten(1)
+        if t.dim() != 2 or t.shape[1] != width:
+            raise ValueError(f"{name} must be [rows, {width}], got {tuple(t.shape)}")
+        self._on_device(name, t.device)
+        if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width) or t.stride(0) * t.element_size() % 16 or t.data_ptr() % 16:
+            t = t.clone(memory_format=torch.contiguous_format)
+        return t
+
+    def _index(self, name: str, x, n: int) -> torch.Tensor:
+        """An int32 index tensor of ``n`` entries on the device; host sequences are uploaded."""
+        t = x if isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.is_cuda and x.is_contiguous() else self._i32(x)
+        self._on_device(name, t.device)
+        if t.dim() != 1 or t.shape[0] != n:
+            raise ValueError(f"{name} must have {n} entries, got {tuple(t.shape)}")
+        return t
+
+    def _on_device(self, name: str, device) -> None:
+        if device != self.device and (device.type, device.index) != (self.device.type, self._ordinal):
+            raise ValueError(f"{name} lies on {device}, the engine on {self.device}")
+
+    def qcache_store(self, cache: QCache, k: torch.Tensor, v: torch.Tensor, slots, positions, row_begin=None,
+                     max_run: int | None = None) -> None:
+        """Rounds rows of keys and values into an 8-bit cache, in place (what ``cross_kv`` and a decode step's append do
+        in 16 bits, model.py:98-147).
+
+        k, v: f32 or bf16 [n, heads * 64] (or [n, heads, 64]); columns of a fused product are taken as they lie.  Run i
+        is rows row_begin[i] .. row_begin[i + 1] (``None``: one row a run) and goes to tokens positions[i], ... of slot
+        slots[i].  A block of 64 tokens that a run enters at its first token gets the scale max|x| / 127 of the run's
+        own values; one that is entered later keeps the larger of that and its scale, and what it holds is rounded to
+        it.  A slot may be named once; ``max_run`` sizes the launch when row_begin is on the device (default: all
+        rows).  Non-finite values, places outside the cache and slots named twice are told by ``device_status()``;
+        slots outside the cache are skipped."""
+        width = cache.n_heads * HEAD_DIM
+        self._on_device("the cache", cache.device)
+        k, v = self._rows("k", k, width), self._rows("v", v, width)
+        if k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("k and v must have the same shape and type")
+        n = k.shape[0]
+        rb = None
+        if row_begin is None:
+            n_runs, most = n, 1
+        else:
+            if not isinstance(row_begin, torch.Tensor):
+                row_begin = [int(b) for b in row_begin]
+                if not row_begin or row_begin[0] < 0 or row_begin[-1] > n or any(b > c for b, c in zip(row_begin, row_begin[1:])):
+                    raise ValueError(f"row_begin must rise from 0 or more to at most {n}")
+                if max_run is None:
+                    max_run = max((c - b for b, c in zip(row_begin, row_begin[1:])), default=0)
+            n_runs = len(row_begin) - 1
+            if n_runs < 0:
+                raise ValueError("row_begin has one entry more than there are runs")
+            rb = self._index("row_begin", row_begin, n_runs + 1)
+            most = n if max_run is None else int(max_run)
+        if not isinstance(slots, torch.Tensor):
+            named = [int(x) for x in slots]
+            if len(set(named)) != len(named):
+                raise ValueError("qcache_store: a slot is named twice")
+        if n == 0 or n_runs == 0:
+            return
+        sl, ps = self._index("slots", slots, n_runs), self._index("positions", positions, n_runs)
+        self._check(self.lib.wdz_qcache_store(
+            self.h, cache.ref, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), _TORCH_DTYPE[k.dtype], n,
+            None if rb is None else rb.data_ptr(), sl.data_ptr(), ps.data_ptr(), n_runs, most, self._stream()))
+
+    def qcache_attention(self, q: torch.Tensor, cache: QCache, slots, lens, scale: float = HEAD_DIM ** -0.5,
+                         out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+        """Decode attention over an 8-bit cache (the cached branch of qkv_attention, model.py:336-359): row r's query
+        heads attend to the first lens[r] tokens of slot slots[r].
+
+        q: f32 or bf16 [n, q_heads * 64] (or [n, q_heads, 64]); q_heads is the cache's head count or a multiple of it up
+        to 8, consecutive query heads sharing a key head.  Returns [n, q_heads * 64] in ``out_dtype`` (default: the
+        engine's type), or fills ``out``.  Length 0 gives zeros; a row whose slot lies outside the cache is left as it
+        was (zeros when ``out`` is not given)."""
+        self._on_device("the cache", cache.device)
+        width = q.shape[1] if q.dim() == 2 else q.shape[1:].numel()
+        if width == 0 or width % (cache.n_heads * HEAD_DIM) or width // (cache.n_heads * HEAD_DIM) > 8:
+            raise ValueError(f"q must have 1 to 8 times the cache's {cache.n_heads} heads of {HEAD_DIM}, got {tuple(q.shape)}")
+        q = self._rows("q", q, width)
+        n = q.shape[0]
+        if out_dtype is not None and out_dtype not in _TORCH_DTYPE:
+            raise ValueError("out_dtype must be float32 or bfloat16")
+        clear = out is None
+        if clear:
+            out = torch.empty(n, width, dtype=out_dtype or self.dtype, device=self.device)
+        elif (out.dtype not in _TORCH_DTYPE or out_dtype not in (None, out.dtype) or tuple(out.shape) != (n, width)
+              or out.stride(1) != 1 or (n > 1 and out.stride(0) < width)
+              or out.stride(0) * out.element_size() % 16 or out.data_ptr() % 16):
+            raise ValueError(f"out must be [{n}, {width}] rows in float32 or bfloat16 that start on 16 bytes")
+        self._on_device("out", out.device)
+        if n == 0:
+            return out
+        sl, ln = self._index("slots", slots, n), self._index("lens", lens, n)
+        self._check(self.lib.wdz_qcache_attention(
+            self.h, cache.ref, q.data_ptr(), q.stride(0), _TORCH_DTYPE[q.dtype], width // HEAD_DIM, sl.data_ptr(),
+            ln.data_ptr(), n, scale, out.data_ptr(), out.stride(0), _TORCH_DTYPE[out.dtype], int(clear),
+            self._stream()))
+        return out
+
+    def linear_rows_packed(self, x: torch.Tensor, w: PackedLinear, residual: torch.Tensor | None = None,
+                           out: torch.Tensor | None = None) -> torch.Tensor:
+        """``linear_rows`` with 4-bit weights (``lowbit.pack_linear``): x f32 or bf16 [M, K] @ W[N, K].T (+ bias)
+        (+ residual f32 [M, N]) -> f32 [M, N].  ``residual`` and ``out`` may be the same tensor."""
+        self._on_device("the weights", w.device)
+        if x.dtype not in _TORCH_DTYPE or x.dim() != 2 or x.shape[1] != w.in_features:
+            raise ValueError(f"x must be [rows, {w.in_features}] in float32 or bfloat16, got {x.dtype} {tuple(x.shape)}")
+        self._on_device("x", x.device)
+        if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+            x = x.contiguous()
+        M, N = x.shape[0], w.out_features
+        for name, t in (("residual", residual), ("out", out)):
+            if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (M, N) or not t.is_contiguous()):
+                raise ValueError(f"{name} must be a contiguous float32 [{M}, {N}]")
+            if t is not None:
+                self._on_device(name, t.device)
+        y = out if out is not None else torch.empty(M, N, dtype=torch.float32, device=self.device)
+        b = w.bias
+        if b is not None and b.dtype != x.dtype:
+            b = b.to(x.dtype)
+        self._check(self.lib.wdz_linear_rows_packed(
+            self.h, x.data_ptr(), x.stride(0), _TORCH_DTYPE[x.dtype], M, w.in_features, w.weight.data_ptr(),
+            w.scale.data_ptr(), w.group, None if b is None else b.data_ptr(),
+            None if residual is None else residual.data_ptr(), N, y.data_ptr(), self._stream()))
+        return y
 
     # ------------------------------------------------------- word-timing alignment
     def align_configure(self, heads) -> None:
