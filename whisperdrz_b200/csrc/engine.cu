@@ -1919,10 +1919,47 @@ int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_d
   p.n_rows = n_rows; p.group = n_q_heads / p.c.n_heads; p.scale = scale; p.clear_skipped = clear_skipped != 0;
   if ((rc = check_ready(e))) return rc;
   DeviceScope on(e->device);
-  const dim3 grid((unsigned)(((int64_t)n_rows * n_q_heads + 3) / 4));
-  auto go = [&](auto kern) { launch_pdl(e, kern, grid, dim3(128), 0, (cudaStream_t)s, p); };
-  if (q_dtype == WDZ_BF16) { if (out_dtype == WDZ_BF16) go(qcache_attend_kernel<bf16, bf16>); else go(qcache_attend_kernel<bf16, float>); }
-  else { if (out_dtype == WDZ_BF16) go(qcache_attend_kernel<float, bf16>); else go(qcache_attend_kernel<float, float>); }
+  // CTAs per (row, key head): enough that the SMs have work, not more than there are tiles for their warps
+  const int64_t items = (int64_t)n_rows * p.c.n_heads;
+  const int most = p.group > 4 ? 8 : 16;
+  int warps = 4, cluster = 1;
+  while (cluster < most && items * cluster < 3 * e->sm_count && cluster * warps < p.c.n_blocks) cluster *= 2;
+  if (cluster == most && cluster * warps * 2 < p.c.n_blocks) warps = QC_MAX_WARPS;
+  if (items * cluster > INT32_MAX) return e->fail(WDZ_ECAPACITY, "wdz_qcache_attention: %d rows of %d heads", n_rows, p.c.n_heads);
+  auto go = [&](auto kern) -> int {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(items * cluster)); cfg.blockDim = dim3(warps * 32); cfg.stream = (cudaStream_t)s;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (cluster > 1) {
+      if (cluster > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+        cudaError_t ce = cudaGetLastError();
+        return e->fail(WDZ_ECUDA, "qcache_attend cluster attribute: %s", cudaGetErrorString(ce));
+      }
+      attr[n].id = cudaLaunchAttributeClusterDimension;
+      attr[n].val.clusterDim = {(unsigned)cluster, 1, 1};
+      ++n;
+    }
+    if (!(e->cfg.flags & WDZ_FLAG_NO_PDL)) {
+      attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[n].val.programmaticStreamSerializationAllowed = 1;
+      ++n;
+    }
+    cfg.attrs = attr; cfg.numAttrs = n;
+    cudaLaunchKernelEx(&cfg, kern, p, cluster);
+    return WDZ_OK;
+  };
+  auto by_group = [&](auto tq, auto to) -> int {
+    using TQ = decltype(tq);
+    using TO = decltype(to);
+    if (p.group == 1) return go(qcache_attend_kernel<TQ, TO, 1, true>);
+    if (p.group == 2) return go(qcache_attend_kernel<TQ, TO, 1, false>);
+    if (p.group <= 4) return go(qcache_attend_kernel<TQ, TO, 2, false>);
+    return go(qcache_attend_kernel<TQ, TO, 4, false>);
+  };
+  if (q_dtype == WDZ_BF16) rc = out_dtype == WDZ_BF16 ? by_group(bf16(), bf16()) : by_group(bf16(), 0.0f);
+  else rc = out_dtype == WDZ_BF16 ? by_group(0.0f, bf16()) : by_group(0.0f, 0.0f);
+  if (rc) return rc;
   WDZ_LAUNCH_CHECK(e, "qcache_attend");
   return WDZ_OK;
 }
