@@ -1970,7 +1970,7 @@ int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_
   if (!e) return WDZ_EINVAL;
   int rc;
   if (x_dtype != WDZ_F32 && x_dtype != WDZ_BF16) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: unknown type %d", x_dtype);
-  if (M < 0 || N < 1 || K < 1 || K > INT32_MAX - 128) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: %d x %d x %d", M, N, K);
+  if (M < 0 || M > 16 * 65535 || N < 1 || K < 1 || K > INT32_MAX - 128) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: %d x %d x %d", M, N, K);
   if (group != 32 && group != 64 && group != 128) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: group %d (32, 64 or 128)", group);
   if (M == 0) return WDZ_OK;
   if (!x_dev || !w_dev || !scale_dev || !y_dev) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: null argument");
@@ -1984,9 +1984,29 @@ int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_
   if ((rc = check_ready(e))) return rc;
   DeviceScope on(e->device);
   const int sp = e->span_begin(WDZ_PROF_DEC_GEMM, (double)N * p.Kp * (0.5 + 2.0 / group), (cudaStream_t)s);
-  const dim3 grid((N + 3) / 4);
-  if (x_dtype == WDZ_BF16) launch_pdl(e, gemv_packed_kernel<bf16>, grid, dim3(128), 0, (cudaStream_t)s, p);
-  else launch_pdl(e, gemv_packed_kernel<float>, grid, dim3(128), 0, (cudaStream_t)s, p);
+  const int tiles = (N + 15) / 16, segs = p.Kp / 128;
+  p.split = 1;
+  while (p.split < GP_WARPS && p.split < segs && (int64_t)tiles * p.split < 8ll * e->sm_count) p.split *= 2;
+  const int64_t esz = x_dtype == WDZ_BF16 ? 2 : 4;
+  p.vec = K % 8 == 0 && aligned16(x_dev, M > 1 ? ldx * esz : 0);
+  auto go = [&](auto kern, int rows_per_cta) {
+    const int per = GP_WARPS / p.split;
+    launch_pdl(e, kern, dim3((tiles + per - 1) / per, (M + rows_per_cta - 1) / rows_per_cta), dim3(GP_WARPS * 32), 0, (cudaStream_t)s, p);
+  };
+  auto by_group = [&](auto tx) {
+    using T = decltype(tx);
+    if (M <= 8) {
+      if (group == 32) go(gemv_packed_kernel<T, 1, 4>, 8);
+      else if (group == 64) go(gemv_packed_kernel<T, 1, 2>, 8);
+      else go(gemv_packed_kernel<T, 1, 1>, 8);
+    } else {
+      if (group == 32) go(gemv_packed_kernel<T, 2, 4>, 16);
+      else if (group == 64) go(gemv_packed_kernel<T, 2, 2>, 16);
+      else go(gemv_packed_kernel<T, 2, 1>, 16);
+    }
+  };
+  if (x_dtype == WDZ_BF16) by_group(bf16());
+  else by_group(0.0f);
   e->span_end(sp, (cudaStream_t)s);
   WDZ_LAUNCH_CHECK(e, "gemv_packed");
   return WDZ_OK;
