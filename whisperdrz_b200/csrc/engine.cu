@@ -12,6 +12,7 @@
 #include <cstring>
 #include <mutex>
 #include <string>
+#include <type_traits>
 #include <unordered_map>
 #include <vector>
 
@@ -1111,6 +1112,22 @@ int wdz_finalize(wdz_engine* e) {
       }
     }
   }
+  {
+    cudaError_t ce4 = cudaSuccess;
+    auto allow = [&](auto kern, int bytes) {
+      if (ce4 == cudaSuccess) ce4 = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    };
+    allow(gemv_packed_s8_kernel<1>, GP_S8_CHUNK * 1024); allow(gemv_packed_s8_kernel<2>, GP_S8_CHUNK * 1024);
+    allow(gemv_packed_s8_kernel<4>, GP_S8_CHUNK * 1024);
+    allow(gemv_packed_f32_kernel<1, 1>, GP_F32_CHUNK<1> * 2048); allow(gemv_packed_f32_kernel<1, 2>, GP_F32_CHUNK<1> * 2048);
+    allow(gemv_packed_f32_kernel<1, 4>, GP_F32_CHUNK<1> * 2048);
+    allow(gemv_packed_f32_kernel<4, 1>, GP_F32_CHUNK<4> * 8192); allow(gemv_packed_f32_kernel<4, 2>, GP_F32_CHUNK<4> * 8192);
+    allow(gemv_packed_f32_kernel<4, 4>, GP_F32_CHUNK<4> * 8192);
+    if (ce4 != cudaSuccess) {
+      cudaGetLastError();
+      return e->fail(WDZ_ECUDA, "gemv_packed smem attribute: %s", cudaGetErrorString(ce4));
+    }
+  }
   if (cudaFuncSetAttribute(dtw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) {
     cudaError_t ce3 = cudaGetLastError();
     return e->fail(WDZ_ECUDA, "dtw smem attribute: %s", cudaGetErrorString(ce3));
@@ -1989,24 +2006,27 @@ int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_
   while (p.split < GP_WARPS && p.split < segs && (int64_t)tiles * p.split < 8ll * e->sm_count) p.split *= 2;
   const int64_t esz = x_dtype == WDZ_BF16 ? 2 : 4;
   p.vec = K % 8 == 0 && aligned16(x_dev, M > 1 ? ldx * esz : 0);
-  auto go = [&](auto kern, int rows_per_cta) {
+  auto go = [&](auto kern, int rows_per_cta, size_t smem) {
     const int per = GP_WARPS / p.split;
-    launch_pdl(e, kern, dim3((tiles + per - 1) / per, (M + rows_per_cta - 1) / rows_per_cta), dim3(GP_WARPS * 32), 0, (cudaStream_t)s, p);
+    launch_pdl(e, kern, dim3((tiles + per - 1) / per, (M + rows_per_cta - 1) / rows_per_cta), dim3(GP_WARPS * 32), smem, (cudaStream_t)s, p);
   };
-  auto by_group = [&](auto tx) {
-    using T = decltype(tx);
-    if (M <= 8) {
-      if (group == 32) go(gemv_packed_kernel<T, 1, 4>, 8);
-      else if (group == 64) go(gemv_packed_kernel<T, 1, 2>, 8);
-      else go(gemv_packed_kernel<T, 1, 1>, 8);
-    } else {
-      if (group == 32) go(gemv_packed_kernel<T, 2, 4>, 16);
-      else if (group == 64) go(gemv_packed_kernel<T, 2, 2>, 16);
-      else go(gemv_packed_kernel<T, 2, 1>, 16);
-    }
+  auto by_group = [&](auto run) {
+    if (group == 32) run(std::integral_constant<int, 4>());
+    else if (group == 64) run(std::integral_constant<int, 2>());
+    else run(std::integral_constant<int, 1>());
   };
-  if (x_dtype == WDZ_BF16) by_group(bf16());
-  else by_group(0.0f);
+  auto held = [&](int chunk) { return (size_t)(segs < chunk ? segs : chunk); };   // segments of x in shared memory
+  if (x_dtype == WDZ_F32 && M <= 2) {
+    by_group([&](auto gs) { go(gemv_packed_f32_kernel<1, decltype(gs)::value>, 2, held(GP_F32_CHUNK<1>) * 2048); });
+  } else if (x_dtype == WDZ_F32) {
+    by_group([&](auto gs) { go(gemv_packed_f32_kernel<4, decltype(gs)::value>, 8, held(GP_F32_CHUNK<4>) * 4 * 2048); });
+  } else if (M <= GP_S8_ROWS) {
+    by_group([&](auto gs) { go(gemv_packed_s8_kernel<decltype(gs)::value>, GP_S8_ROWS, held(GP_S8_CHUNK) * 1024); });
+  } else if (M <= 8) {
+    by_group([&](auto gs) { go(gemv_packed_bf16_kernel<1, decltype(gs)::value>, 8, 0); });
+  } else {
+    by_group([&](auto gs) { go(gemv_packed_bf16_kernel<2, decltype(gs)::value>, 16, 0); });
+  }
   e->span_end(sp, (cudaStream_t)s);
   WDZ_LAUNCH_CHECK(e, "gemv_packed");
   return WDZ_OK;

@@ -6,12 +6,19 @@
 // A few rows: bound by the weights' bytes, and, since half a byte is a weight, nearly as much by the instructions that
 // take them apart.  A warp owns 16 features and reads 128 weights of each at a time as 16-byte pieces, straight into
 // registers: lane (g, t) = (lane / 4, lane % 4) has words 4 t .. 4 t + 3 of features g and g + 8, which is what the A
-// operand of mma.m16n8k16 wants from it for four groups of 32 weights.  A word becomes four pairs of bf16 with a shift,
-// a mask and one fused add each: bits u placed under the exponent of 128 are 128 + u, minus 136 is the weight, exactly.
-// x is the B operand, eight rows a tile: bf16 rows as they lie, f32 rows cut into three bf16 pieces (8 + 8 + 8 bits) that
-// add up to the value.  Products are exact and their sums fp32; a group's sum is multiplied by its scale in fp32.
-// K is split over the warps of a CTA when there are too few features to fill the SMs; the partial sums meet in shared
-// memory in a fixed order.
+// operand of a matrix instruction wants from it for four groups of 32 weights.  K is split over the warps of a CTA when
+// there are too few features to fill the SMs; the partial sums meet in shared memory in a fixed order.
+//
+//   gemv_packed_s8_kernel    bf16 rows, up to two.  m16n8k32 on bytes: a word becomes two operands with three
+//       instructions (a nibble in a byte's upper half is 16 times a signed weight).  x is written as a whole number of
+//       32 bits times a scale of its row, four signed bytes that take four columns: exact for values down to 2^-23 of the
+//       row's largest, off by at most 2^-32 of that below.  Sums of products of bytes are exact.
+//   gemv_packed_bf16_kernel  bf16 rows, three and more.  m16n8k16 on bf16: a row is one column, taken as it lies.  A word
+//       becomes four pairs of bf16 with a shift, a mask and one fused add each: bits u placed under the exponent of 128
+//       are 128 + u, minus 136 is the weight, exactly.
+//   gemv_packed_f32_kernel   f32 rows: the same, a row cut into three bf16 pieces (8 + 8 + 8 bits) that add up to it and
+//       take three columns; whole numbers would not do for rows whose largest value is far above the rest.
+// Either way a group's sum is multiplied by its scale in fp32.
 #pragma once
 #include "common.cuh"
 #include "gemv_mma.cuh"
@@ -31,7 +38,12 @@ struct GemvPackedParams {
 };
 
 constexpr int GP_WARPS = 8;
-constexpr int GP_AHEAD = 4;   // segments of 128 weights that a warp has under way
+constexpr int GP_AHEAD = 4;   // segments of 128 weights that a warp of the byte kernel has under way
+
+__device__ __forceinline__ void mma_s8_16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 
 // One 32-bit word of weights -> pairs (element 2 j, element 2 j + 1), j = 0..3, as bf16.
 __device__ __forceinline__ void gp_unpack(uint32_t w, uint32_t (&r)[4]) {
@@ -45,27 +57,29 @@ __device__ __forceinline__ void gp_unpack(uint32_t w, uint32_t (&r)[4]) {
   }
 }
 
-// Eight neighbouring values of a row of x from k0 on, zeros behind its end, as pairs of bf16 (PIECES of them a value).
-template <typename T, int PIECES>
-__device__ __forceinline__ void gp_row(const T* row, int k0, int K, bool vec, uint32_t (&b)[PIECES][4]);
-template <>
-__device__ __forceinline__ void gp_row<bf16, 1>(const bf16* row, int k0, int K, bool vec, uint32_t (&b)[1][4]) {
+// Eight neighbouring values of a row of x from k0 on, zeros behind its end.
+__device__ __forceinline__ uint4 gp_row(const bf16* row, int k0, int K, bool vec) {
+  uint4 v = make_uint4(0, 0, 0, 0);
   if (vec) {
-    uint4 v = make_uint4(0, 0, 0, 0);
     if (k0 < K) v = __ldg(reinterpret_cast<const uint4*>(row + k0));
-    b[0][0] = v.x; b[0][1] = v.y; b[0][2] = v.z; b[0][3] = v.w;
-  } else {
-    const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t lo = k0 + 2 * j < K ? r[k0 + 2 * j] : 0, hi = k0 + 2 * j + 1 < K ? r[k0 + 2 * j + 1] : 0;
-      b[0][j] = lo | hi << 16;
-    }
+    return v;
   }
+  const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t lo = k0 + 2 * j < K ? r[k0 + 2 * j] : 0, hi = k0 + 2 * j + 1 < K ? r[k0 + 2 * j + 1] : 0;
+    w[j] = lo | hi << 16;
+  }
+  return v;
 }
-template <>
-__device__ __forceinline__ void gp_row<float, 3>(const float* row, int k0, int K, bool vec, uint32_t (&b)[3][4]) {
-  float v[8];
+__device__ __forceinline__ void gp_row8(const bf16* row, int k0, int K, bool vec, float (&v)[8]) {
+  const uint4 u = gp_row(row, k0, K, vec);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ void gp_row8(const float* row, int k0, int K, bool vec, float (&v)[8]) {
   if (vec) {
     float4 lo = make_float4(0, 0, 0, 0), hi = lo;
     if (k0 < K) { lo = __ldg(reinterpret_cast<const float4*>(row + k0)); hi = __ldg(reinterpret_cast<const float4*>(row + k0 + 4)); }
@@ -74,25 +88,278 @@ __device__ __forceinline__ void gp_row<float, 3>(const float* row, int k0, int K
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = k0 + i < K ? row[k0 + i] : 0.0f;
   }
-#pragma unroll
-  for (int piece = 0; piece < 3; ++piece) {   // the upper 16 bits of what is left, cut off, not rounded: nothing overflows
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t x0 = __float_as_uint(v[2 * j]), x1 = __float_as_uint(v[2 * j + 1]);
-      b[piece][j] = __byte_perm(x0, x1, 0x7632);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float top = __uint_as_float(__float_as_uint(v[i]) & 0xffff0000u);
-      v[i] = fabsf(v[i]) == INFINITY ? 0.0f : v[i] - top;
-    }
+}
+
+// The scales of one segment of a feature, GS of them.
+template <int GS> struct GpScale;
+template <> struct GpScale<1> {
+  uint32_t v;
+  __device__ void load(const bf16* p) { v = *reinterpret_cast<const uint16_t*>(p); }
+  __device__ float get(int) const { return __uint_as_float(v << 16); }
+};
+template <> struct GpScale<2> {
+  uint32_t v;
+  __device__ void load(const bf16* p) { v = __ldg(reinterpret_cast<const uint32_t*>(p)); }
+  __device__ float get(int i) const { return __uint_as_float(i & 1 ? v & 0xffff0000u : v << 16); }
+};
+template <> struct GpScale<4> {
+  uint2 v;
+  __device__ void load(const bf16* p) { v = __ldg(reinterpret_cast<const uint2*>(p)); }
+  __device__ float get(int i) const { const uint32_t w = i & 2 ? v.y : v.x; return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16); }
+};
+
+// The 16 features' sums of `split` warps, plus bias and residual, for rows m0 .. m0 + rows.
+template <typename T, int ROWS>
+__device__ __forceinline__ void gp_finish(const GemvPackedParams& p, const float (&red)[GP_WARPS][ROWS][17], int m0) {
+  const int rows = min(ROWS, p.M - m0), cols = 16 * (GP_WARPS / p.split), n_first = blockIdx.x * cols;
+  for (int i = threadIdx.x; i < rows * cols; i += GP_WARPS * 32) {
+    const int row = i / cols, col = i % cols, n = n_first + col;
+    if (n >= p.N) continue;
+    float v = 0.0f;
+    for (int w = 0; w < p.split; ++w) v += red[(col >> 4) * p.split + w][row][col & 15];
+    if (p.bias) v += to_f(reinterpret_cast<const T*>(p.bias)[n]);
+    const int64_t at = (int64_t)(m0 + row) * p.N + n;
+    if (p.residual) v += p.residual[at];
+    p.y[at] = v;
   }
 }
 
+constexpr float GP_S8_STEPS = 127.0f * 16777216.0f;   // a row's largest value in steps: rounding up leaves its top byte a byte
+constexpr int GP_S8_ROWS = 2, GP_S8_CHUNK = 64;       // rows of a CTA, segments of x that one pass keeps in shared memory (64 KB)
+template <int PAIRS> constexpr int GP_F32_CHUNK = PAIRS == 1 ? 40 : 10;   // the same (80 KB)
+
+// Block = 8 warps; grid = (tiles of 16 features x split / 8, rows / 2).  GS: scales of a segment of 128 weights.
+template <int GS>
+__global__ void __launch_bounds__(GP_WARPS * 32) gemv_packed_s8_kernel(GemvPackedParams p) {
+  extern __shared__ __align__(16) uint2 xs[];   // [segment][i][lane]: a lane's two operand words
+  __shared__ float red[GP_WARPS][GP_S8_ROWS][17];
+  __shared__ float tops[GP_WARPS][GP_S8_ROWS];
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int part = warp % p.split, tile = blockIdx.x * (GP_WARPS / p.split) + warp / p.split;
+  const int m0 = blockIdx.y * GP_S8_ROWS, segs = p.Kp >> 7, rows = min(GP_S8_ROWS, p.M - m0);
+  const int na = min(tile * 16 + g, p.N - 1), nb = min(tile * 16 + g + 8, p.N - 1);
+  const uint4* wa = reinterpret_cast<const uint4*>(p.W + (int64_t)na * (p.Kp >> 3)) + t;   // a segment is four uint4
+  const uint4* wb = reinterpret_cast<const uint4*>(p.W + (int64_t)nb * (p.Kp >> 3)) + t;
+  const bf16* sa = p.scale + (int64_t)na * segs * GS;
+  const bf16* sb = p.scale + (int64_t)nb * segs * GS;
+  const bf16* x = reinterpret_cast<const bf16*>(p.x) + (int64_t)m0 * p.ldx;
+  pdl_wait();
+
+  float sum[2] = {0.0f, 0.0f};
+  for (int first = 0; first < segs; first += GP_S8_CHUNK) {
+    const int here = min(GP_S8_CHUNK, segs - first), last = first + here;
+    uint4 a[GP_AHEAD], b[GP_AHEAD];
+    GpScale<GS> fa[GP_AHEAD], fb[GP_AHEAD];
+    auto fetch = [&](int u, int sg) {
+      if (sg < last) {
+        a[u] = __ldg(wa + 4 * sg);
+        b[u] = __ldg(wb + 4 * sg);
+        fa[u].load(sa + sg * GS);
+        fb[u].load(sb + sg * GS);
+      }
+    };
+#pragma unroll
+    for (int u = 0; u < GP_AHEAD; ++u) fetch(u, first + part + u * p.split);   // under way while x is taken apart
+
+    // largest value of each row, 8 values a thread and step
+    const int units = here * 16;
+    float top[GP_S8_ROWS];
+#pragma unroll
+    for (int m = 0; m < GP_S8_ROWS; ++m) {
+      top[m] = 0.0f;
+      if (m < rows)
+        for (int i = threadIdx.x; i < units; i += GP_WARPS * 32) {
+          float v[8];
+          gp_row8(x + (int64_t)m * p.ldx, first * 128 + 8 * i, p.K, p.vec, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top[m] = fabsf(v[j]) <= 3.402823466e38f ? fmaxf(top[m], fabsf(v[j])) : INFINITY;
+        }
+    }
+    __syncthreads();   // the pass before has read xs and tops
+#pragma unroll
+    for (int m = 0; m < GP_S8_ROWS; ++m) {
+      top[m] = warp_max(top[m]);
+      if (lane == 0) tops[warp][m] = top[m];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < GP_S8_ROWS; ++m) {
+#pragma unroll
+      for (int w = 0; w < GP_WARPS; ++w) top[m] = fmaxf(top[m], tops[w][m]);
+      if (m < rows) {
+        const float lift = top[m] < 1e-20f ? 18446744073709551616.0f : 1.0f;   // 2^64: keeps the quotient finite
+        const float steps = top[m] > 0.0f ? GP_S8_STEPS / (top[m] * lift) * lift : 0.0f;
+        for (int i = threadIdx.x; i < units; i += GP_WARPS * 32) {
+          float v[8];
+          gp_row8(x + (int64_t)m * p.ldx, first * 128 + 8 * i, p.K, p.vec, v);
+          // unit = word i of lane tt of a segment; the bytes' lower nibbles are elements 0 4 1 5, the upper 2 6 3 7
+          const int sg = i >> 4, wi = i & 15, at = wi >> 2, tt = wi & 3;
+          uint32_t n[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) n[j] = (uint32_t)__float2int_rn(v[j] * steps) + 0x80808080u;   // bytes + 128
+          uint2 d[4];   // columns d1, d0, d3, d2
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t e0 = n[2 * h], e1 = n[2 * h + 4], e2 = n[2 * h + 1], e3 = n[2 * h + 5];
+            const uint32_t x01 = __byte_perm(e0, e1, 0x5140), x23 = __byte_perm(e2, e3, 0x5140);
+            const uint32_t y01 = __byte_perm(e0, e1, 0x7362), y23 = __byte_perm(e2, e3, 0x7362);
+            (h ? d[0].y : d[0].x) = __byte_perm(x01, x23, 0x7632) ^ 0x80808080u;
+            (h ? d[1].y : d[1].x) = __byte_perm(x01, x23, 0x5410) ^ 0x80808080u;
+            (h ? d[2].y : d[2].x) = __byte_perm(y01, y23, 0x7632) ^ 0x80808080u;
+            (h ? d[3].y : d[3].x) = __byte_perm(y01, y23, 0x5410) ^ 0x80808080u;
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) xs[(sg * 4 + at) * 32 + (m * 4 + q) * 4 + tt] = d[q];
+        }
+      }
+    }
+    __syncthreads();
+
+    float acc[2] = {0.0f, 0.0f};
+    const bool mine = (g >> 2) < rows;
+    for (int base = first + part; base < last; base += GP_AHEAD * p.split) {
+#pragma unroll
+      for (int u = 0; u < GP_AHEAD; ++u) {
+        const int sg = base + u * p.split;
+        if (sg < last) {
+          const uint4 a_now = a[u], b_now = b[u];
+          const GpScale<GS> fa_now = fa[u], fb_now = fb[u];
+          fetch(u, sg + GP_AHEAD * p.split);
+          const uint32_t* aw = reinterpret_cast<const uint32_t*>(&a_now);
+          const uint32_t* bw = reinterpret_cast<const uint32_t*>(&b_now);
+          const uint2* xq = xs + (sg - first) * 128 + lane;
+          int c[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint2 xb = make_uint2(0, 0);
+            if (mine) xb = xq[32 * i];
+            mma_s8_16832(c, ((aw[i] << 4) ^ 0x80808080u) & 0xf0f0f0f0u, ((bw[i] << 4) ^ 0x80808080u) & 0xf0f0f0f0u,
+                         (aw[i] ^ 0x80808080u) & 0xf0f0f0f0u, (bw[i] ^ 0x80808080u) & 0xf0f0f0f0u, xb.x, xb.y);
+            if ((i + 1) % (4 / GS) == 0) {   // the end of a group: columns (d1, d0) or (d3, d2) fold into one number
+              acc[0] = fmaf((float)(c[0] * 256 + c[1]), fa_now.get(i / (4 / GS)), acc[0]);
+              acc[1] = fmaf((float)(c[2] * 256 + c[3]), fb_now.get(i / (4 / GS)), acc[1]);
+              c[0] = c[1] = c[2] = c[3] = 0;
+            }
+          }
+        }
+      }
+    }
+    // a step of the row, / 16 for the shifted nibble; an infinite or NaN row: infinity times zero is NaN
+    const float step = (t >> 1 ? top[1] : top[0]) * (1.0f / (16.0f * GP_S8_STEPS)) * (t & 1 ? 65536.0f : 1.0f);
+    sum[0] = fmaf(acc[0], step, sum[0]);
+    sum[1] = fmaf(acc[1], step, sum[1]);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float v = sum[h] + __shfl_xor_sync(0xffffffffu, sum[h], 1);
+    if (!(t & 1)) red[warp][t >> 1][g + 8 * h] = v;
+  }
+  __syncthreads();
+  gp_finish<bf16>(p, red, m0);
+}
+
+// PAIRS: pairs of rows a CTA takes.  Block = 8 warps; grid = (tiles of 16 features x split / 8, rows / (2 PAIRS)).
+template <int PAIRS, int GS>
+__global__ void __launch_bounds__(GP_WARPS * 32) gemv_packed_f32_kernel(GemvPackedParams p) {
+  extern __shared__ __align__(16) uint4 xf[];   // [segment][pair][i][lane]: eight values of a lane's column
+  __shared__ float red[GP_WARPS][2 * PAIRS][17];
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int part = warp % p.split, tile = blockIdx.x * (GP_WARPS / p.split) + warp / p.split;
+  const int m0 = blockIdx.y * 2 * PAIRS, segs = p.Kp >> 7, rows = min(2 * PAIRS, p.M - m0);
+  const int na = min(tile * 16 + g, p.N - 1), nb = min(tile * 16 + g + 8, p.N - 1);
+  const uint4* wa = reinterpret_cast<const uint4*>(p.W + (int64_t)na * (p.Kp >> 3)) + t;
+  const uint4* wb = reinterpret_cast<const uint4*>(p.W + (int64_t)nb * (p.Kp >> 3)) + t;
+  const bf16* sa = p.scale + (int64_t)na * segs * GS;
+  const bf16* sb = p.scale + (int64_t)nb * segs * GS;
+  const float* x = reinterpret_cast<const float*>(p.x) + (int64_t)m0 * p.ldx;
+  pdl_wait();
+
+  float acc[PAIRS][4];
+#pragma unroll
+  for (int q = 0; q < PAIRS; ++q)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[q][j] = 0.0f;
+  for (int first = 0; first < segs; first += GP_F32_CHUNK<PAIRS>) {
+    const int here = min(GP_F32_CHUNK<PAIRS>, segs - first), last = first + here;
+    uint4 a[2], b[2];
+    GpScale<GS> fa[2], fb[2];
+    auto fetch = [&](int u, int sg) {
+      if (sg < last) {
+        a[u] = __ldg(wa + 4 * sg);
+        b[u] = __ldg(wb + 4 * sg);
+        fa[u].load(sa + sg * GS);
+        fb[u].load(sb + sg * GS);
+      }
+    };
+    fetch(0, first + part);
+    fetch(1, first + part + p.split);
+    __syncthreads();   // the pass before has read xf
+    for (int i = threadIdx.x; i < here * 16 * rows; i += GP_WARPS * 32) {
+      const int m = i / (here * 16), unit = i % (here * 16), sg = unit >> 4, at = (unit & 15) >> 2, tt = unit & 3;
+      float v[8];
+      gp_row8(x + (int64_t)m * p.ldx, first * 128 + 8 * unit, p.K, p.vec, v);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {   // the upper 16 bits of what is left, cut off, not rounded: nothing overflows
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = __byte_perm(__float_as_uint(v[2 * j]), __float_as_uint(v[2 * j + 1]), 0x7632);
+        xf[((sg * PAIRS + (m >> 1)) * 4 + at) * 32 + ((m & 1) * 4 + q) * 4 + tt] = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float cut = __uint_as_float(__float_as_uint(v[j]) & 0xffff0000u);
+          v[j] = fabsf(v[j]) == INFINITY ? 0.0f : v[j] - cut;
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll 2
+    for (int sg = first + part, u = 0; sg < last; sg += p.split, u ^= 1) {
+      const uint4 a_now = a[u], b_now = b[u];
+      const GpScale<GS> fa_now = fa[u], fb_now = fb[u];
+      fetch(u, sg + 2 * p.split);
+      const uint32_t* aw = reinterpret_cast<const uint32_t*>(&a_now);
+      const uint32_t* bw = reinterpret_cast<const uint32_t*>(&b_now);
+      float c[PAIRS][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t ra[4], rb[4];
+        gp_unpack(aw[i], ra);
+        gp_unpack(bw[i], rb);
+#pragma unroll
+        for (int q = 0; q < PAIRS; ++q) {
+          uint4 xb = make_uint4(0, 0, 0, 0);
+          if ((g & 3) != 3 && 2 * q + (g >> 2) < rows) xb = xf[(((sg - first) * PAIRS + q) * 4 + i) * 32 + lane];
+          if (i % (4 / GS) == 0) c[q][0] = c[q][1] = c[q][2] = c[q][3] = 0.0f;
+          mma_bf16_16816(c[q], ra[0], rb[0], ra[1], rb[1], xb.x, xb.y);
+          mma_bf16_16816(c[q], ra[2], rb[2], ra[3], rb[3], xb.z, xb.w);
+          if ((i + 1) % (4 / GS) == 0) {
+            const float sa_g = fa_now.get(i / (4 / GS)), sb_g = fb_now.get(i / (4 / GS));
+            acc[q][0] = fmaf(sa_g, c[q][0], acc[q][0]);
+            acc[q][1] = fmaf(sa_g, c[q][1], acc[q][1]);
+            acc[q][2] = fmaf(sb_g, c[q][2], acc[q][2]);
+            acc[q][3] = fmaf(sb_g, c[q][3], acc[q][3]);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < PAIRS; ++q)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {   // the pieces' columns: two in a lane, the third in the next
+      const float two = acc[q][2 * h] + acc[q][2 * h + 1];
+      const float v = two + __shfl_xor_sync(0xffffffffu, two, 1);
+      if (!(t & 1)) red[warp][2 * q + (t >> 1)][g + 8 * h] = v;
+    }
+  __syncthreads();
+  gp_finish<float>(p, red, m0);
+}
+
 // Block = 8 warps; grid = (tiles of 16 features x split / 8, rows / (8 NT)).  GS: scales of a segment of 128 weights.
-template <typename T, int NT, int GS>
-__global__ void __launch_bounds__(GP_WARPS * 32) gemv_packed_kernel(GemvPackedParams p) {
-  constexpr int PIECES = sizeof(T) == 2 ? 1 : 3;
+template <int NT, int GS>
+__global__ void __launch_bounds__(GP_WARPS * 32) gemv_packed_bf16_kernel(GemvPackedParams p) {
   __shared__ float red[GP_WARPS][8 * NT][17];
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -103,6 +370,7 @@ __global__ void __launch_bounds__(GP_WARPS * 32) gemv_packed_kernel(GemvPackedPa
   const uint4* wb = reinterpret_cast<const uint4*>(p.W + (int64_t)nb * (p.Kp >> 3)) + t;
   const bf16* sa = p.scale + (int64_t)na * segs * GS;
   const bf16* sb = p.scale + (int64_t)nb * segs * GS;
+  const bf16* x = reinterpret_cast<const bf16*>(p.x);
   pdl_wait();
 
   float acc[NT][4];
@@ -111,44 +379,61 @@ __global__ void __launch_bounds__(GP_WARPS * 32) gemv_packed_kernel(GemvPackedPa
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
 
-  for (int base = part; base < segs; base += GP_AHEAD * p.split) {
-    uint4 a[GP_AHEAD], b[GP_AHEAD];
-    float fa[GP_AHEAD][GS], fb[GP_AHEAD][GS];
-#pragma unroll
-    for (int u = 0; u < GP_AHEAD; ++u) {
-      const int sg = min(base + u * p.split, segs - 1);   // the last ones are read again and left out below
+  // weights two segments ahead, x one: both are under way while a segment is worked on
+  uint4 a[2], b[2], xn[NT][4];
+  GpScale<GS> fa[2], fb[2];
+  auto fetch_w = [&](int u, int sg) {
+    if (sg < segs) {
       a[u] = __ldg(wa + 4 * sg);
       b[u] = __ldg(wb + 4 * sg);
-#pragma unroll
-      for (int i = 0; i < GS; ++i) { fa[u][i] = to_f(sa[sg * GS + i]); fb[u][i] = to_f(sb[sg * GS + i]); }
+      fa[u].load(sa + sg * GS);
+      fb[u].load(sb + sg * GS);
     }
+  };
+  auto fetch_x = [&](int sg) {
 #pragma unroll
-    for (int u = 0; u < GP_AHEAD; ++u) {
-      const int sg = base + u * p.split;
-      if (sg < segs) {
-        const uint32_t* aw = reinterpret_cast<const uint32_t*>(&a[u]);
-        const uint32_t* bw = reinterpret_cast<const uint32_t*>(&b[u]);
+    for (int nt = 0; nt < NT; ++nt) {
+      const int m = m0 + 8 * nt + g;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t ra[4], rb[4];
-          gp_unpack(aw[i], ra);
-          gp_unpack(bw[i], rb);
+      for (int i = 0; i < 4; ++i) {
+        xn[nt][i] = make_uint4(0, 0, 0, 0);
+        if (m < p.M && sg < segs) xn[nt][i] = gp_row(x + (int64_t)m * p.ldx, sg * 128 + 32 * i + 8 * t, p.K, p.vec);
+      }
+    }
+  };
+  fetch_w(0, part);
+  fetch_w(1, part + p.split);
+  fetch_x(part);
+#pragma unroll 2
+  for (int sg = part, u = 0; sg < segs; sg += p.split, u ^= 1) {
+    const uint4 wa_now = a[u], wb_now = b[u];
+    const GpScale<GS> fa_now = fa[u], fb_now = fb[u];
+    uint4 xc[NT][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const int m = m0 + 8 * nt + g;
-            uint32_t xb[PIECES][4] = {};
-            if (m < p.M) gp_row<T, PIECES>(reinterpret_cast<const T*>(p.x) + (int64_t)m * p.ldx, sg * 128 + 32 * i + 8 * t, p.K, p.vec, xb);
-            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int q = PIECES - 1; q >= 0; --q) {
-              mma_bf16_16816(c, ra[0], rb[0], ra[1], rb[1], xb[q][0], xb[q][1]);
-              mma_bf16_16816(c, ra[2], rb[2], ra[3], rb[3], xb[q][2], xb[q][3]);
-            }
-            acc[nt][0] = fmaf(fa[u][i * GS / 4], c[0], acc[nt][0]);
-            acc[nt][1] = fmaf(fa[u][i * GS / 4], c[1], acc[nt][1]);
-            acc[nt][2] = fmaf(fb[u][i * GS / 4], c[2], acc[nt][2]);
-            acc[nt][3] = fmaf(fb[u][i * GS / 4], c[3], acc[nt][3]);
-          }
+      for (int i = 0; i < 4; ++i) xc[nt][i] = xn[nt][i];
+    fetch_w(u, sg + 2 * p.split);
+    fetch_x(sg + p.split);
+    const uint32_t* aw = reinterpret_cast<const uint32_t*>(&wa_now);
+    const uint32_t* bw = reinterpret_cast<const uint32_t*>(&wb_now);
+    float c[NT][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t ra[4], rb[4];
+      gp_unpack(aw[i], ra);
+      gp_unpack(bw[i], rb);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (i % (4 / GS) == 0) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
+        mma_bf16_16816(c[nt], ra[0], rb[0], ra[1], rb[1], xc[nt][i].x, xc[nt][i].y);
+        mma_bf16_16816(c[nt], ra[2], rb[2], ra[3], rb[3], xc[nt][i].z, xc[nt][i].w);
+        if ((i + 1) % (4 / GS) == 0) {   // the end of a group
+          const float sa_g = fa_now.get(i / (4 / GS)), sb_g = fb_now.get(i / (4 / GS));
+          acc[nt][0] = fmaf(sa_g, c[nt][0], acc[nt][0]);
+          acc[nt][1] = fmaf(sa_g, c[nt][1], acc[nt][1]);
+          acc[nt][2] = fmaf(sb_g, c[nt][2], acc[nt][2]);
+          acc[nt][3] = fmaf(sb_g, c[nt][3], acc[nt][3]);
         }
       }
     }
@@ -161,17 +446,7 @@ __global__ void __launch_bounds__(GP_WARPS * 32) gemv_packed_kernel(GemvPackedPa
     red[warp][8 * nt + 2 * t + 1][g + 8] = acc[nt][3];
   }
   __syncthreads();
-  const int rows = min(8 * NT, p.M - m0), cols = 16 * (GP_WARPS / p.split), n_first = blockIdx.x * cols;
-  for (int i = threadIdx.x; i < rows * cols; i += GP_WARPS * 32) {
-    const int row = i / cols, col = i % cols, n = n_first + col;
-    if (n >= p.N) continue;
-    float v = 0.0f;
-    for (int w = 0; w < p.split; ++w) v += red[(col >> 4) * p.split + w][row][col & 15];
-    if (p.bias) v += to_f(reinterpret_cast<const T*>(p.bias)[n]);
-    const int64_t at = (int64_t)(m0 + row) * p.N + n;
-    if (p.residual) v += p.residual[at];
-    p.y[at] = v;
-  }
+  gp_finish<bf16>(p, red, m0);
 }
 
 }  // namespace wdz

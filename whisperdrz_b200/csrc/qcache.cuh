@@ -8,6 +8,7 @@
 #pragma once
 #include "../../include/wdz.h"
 #include "common.cuh"
+#include "gemv_packed.cuh"
 
 namespace wdz {
 
@@ -121,14 +122,14 @@ struct QcAttendParams {
 // cores would cost more instructions than there are issue slots at the memory's rate (about 1400 a tile of 8 KB and
 // scheduler), so both products run on the integer matrix instruction m16n8k32, which takes the cache's bytes as they lie:
 //
-//   scores   A = 16 tokens x 32 values of K (s8), B = the query, written as a whole number of 24 bits times a scale,
-//            N = 65536 d2 + 256 d1 + d0 with signed bytes d: three of the instruction's eight columns.  Sums of
+//   scores   A = 16 tokens x 32 values of K (s8), B = the query, written as a whole number of 32 bits times a scale,
+//            N = 2^24 d3 + 2^16 d2 + 2^8 d1 + d0 with signed bytes d: four of the instruction's eight columns.  Sums of
 //            products of bytes are exact, so a score has the precision of an fp32 query.
-//   output   A = 16 values x 32 tokens of V (s8), B = the softmax weights of the tokens, p in [0, 1] as
-//            65536 d2 + 256 d1 + d0 in units of 2^-23, unsigned bytes.
+//   output   A = 16 values x 32 tokens of V (s8), B = the softmax weights of the tokens, p in [0, 1] as four unsigned
+//            bytes in units of 2^-32.
 //
-// A query head takes four columns (d1, d0, d2, nothing): the two columns that a lane of the result holds are then
-// (d1, d0) or (d2, nothing), and it folds them as 256 a + b in 32 bits.  Two heads of a group fill the eight columns.
+// A query head's columns are d1, d0, d3, d2: the two columns that a lane of the result holds are (d1, d0) or (d3, d2),
+// and it folds them as 256 a + b in 32 bits.  Two heads of a group fill the eight columns.
 //
 // Tile = 64 tokens = one scale.  Lane (g, t) = (lane / 4, lane % 4).  Rows and contraction labels of the instruction
 // are names only, so they are given out such that loads are whole 16- or 8-byte pieces of a token and no byte of K moves:
@@ -137,11 +138,9 @@ struct QcAttendParams {
 //   p    the four tokens (ks, r, b = 0..3, t) are the scores j = 4 ks + b of the lanes g = 4 r + t: one lane packs them
 //        and one shuffle brings each word to its column.
 constexpr int QC_MAX_WARPS = 8;
+constexpr float QC_STEPS = 127.0f * 16777216.0f;   // a query's largest value in steps: rounding up leaves d3 a byte
+constexpr float QC_ONE = 4294967040.0f;            // the weight 1 in steps: the largest fp32 below 2^32
 
-__device__ __forceinline__ void qc_mma_ss(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ void qc_mma_su(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -254,23 +253,19 @@ __global__ void __launch_bounds__(QC_MAX_WARPS * 32) qcache_attend_kernel(QcAtte
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const float lift = top < 1e-20f ? 18446744073709551616.0f : 1.0f;   // 2^64: keeps the quotient below finite
-    const float steps = top > 0.0f ? 8323072.0f / (top * lift) * lift : 0.0f;   // 127 x 65536: rounding up leaves d2 a byte
-    const int digit = g & 3;   // column's byte: d1, d0, d2, nothing
+    const float steps = top > 0.0f ? QC_STEPS / (top * lift) * lift : 0.0f;
+    const int digit = (g & 3) ^ 1;   // columns d1, d0, d3, d2
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      uint32_t word = 0;
+      uint32_t n[4];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int n = __float2int_rn(x[4 * w + b] * steps);
-        const int d0 = (int)(int8_t)n, n1 = (n - d0) >> 8, d1 = (int)(int8_t)n1, d2 = (n1 - d1) >> 8;
-        const int d = digit == 0 ? d1 : digit == 1 ? d0 : digit == 2 ? d2 : 0;
-        word |= (uint32_t)(d & 255) << (8 * b);
-      }
-      qb[nt][w] = word;
+      for (int b = 0; b < 4; ++b) n[b] = ((uint32_t)__float2int_rn(x[4 * w + b] * steps) + 0x80808080u) >> (8 * digit);
+      const uint32_t lo = __byte_perm(n[0], n[1], 0x0040), hi = __byte_perm(n[2], n[3], 0x0040);
+      qb[nt][w] = __byte_perm(lo, hi, 0x5410) ^ 0x80808080u;   // the digits are bytes less 128
     }
     // an infinite or NaN query: infinity times zero makes the row NaN
-    const float mul = (top * lift) * (1.0f / 8323072.0f) * (p.scale * 1.4426950408889634f) / lift;
-    q_mul[nt] = __shfl_sync(0xffffffffu, mul, 16 * (t >> 1)) * (t & 1 ? 256.0f : 1.0f);   // of the head whose scores this lane gets
+    const float mul = (top * lift) * (1.0f / QC_STEPS) * (p.scale * 1.4426950408889634f) / lift;
+    q_mul[nt] = __shfl_sync(0xffffffffu, mul, 16 * (t >> 1)) * (t & 1 ? 65536.0f : 1.0f);   // of the head whose scores this lane gets
   }
 
   float m[NT], l[NT], acc[NT][8];
@@ -293,8 +288,8 @@ __global__ void __launch_bounds__(QC_MAX_WARPS * 32) qcache_attend_kernel(QcAtte
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         int c[4] = {0, 0, 0, 0};
-        qc_mma_ss(c, k[2 * i].x, k[2 * i + 1].x, k[2 * i].y, k[2 * i + 1].y, qb[nt][0], qb[nt][1]);
-        qc_mma_ss(c, k[2 * i].z, k[2 * i + 1].z, k[2 * i].w, k[2 * i + 1].w, qb[nt][2], qb[nt][3]);
+        mma_s8_16832(c, k[2 * i].x, k[2 * i + 1].x, k[2 * i].y, k[2 * i + 1].y, qb[nt][0], qb[nt][1]);
+        mma_s8_16832(c, k[2 * i].z, k[2 * i + 1].z, k[2 * i].w, k[2 * i + 1].w, qb[nt][2], qb[nt][3]);
         s[2 * i] = (float)(c[0] * 256 + c[1]) * mul;
         s[2 * i + 1] = (float)(c[2] * 256 + c[3]) * mul;
       }
@@ -319,25 +314,25 @@ __global__ void __launch_bounds__(QC_MAX_WARPS * 32) qcache_attend_kernel(QcAtte
       for (int j = 0; j < 8; ++j) {
         const float w = qc_ex2(s[j] - m_new);
         sum += w;
-        n[j] = __float_as_uint(w + 1.0f) - 0x3f800000u;   // w in units of 2^-23, rounded by the sum
+        n[j] = __float2uint_rn(w * QC_ONE);
       }
       l[nt] = fmaf(l[nt], alpha[nt], sum);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {   // tokens 32 h ..
         const uint32_t x01 = __byte_perm(n[4 * h], n[4 * h + 1], 0x5140), x23 = __byte_perm(n[4 * h + 2], n[4 * h + 3], 0x5140);
-        const uint32_t y01 = __byte_perm(n[4 * h], n[4 * h + 1], 0x0062), y23 = __byte_perm(n[4 * h + 2], n[4 * h + 3], 0x0062);
-        const uint32_t d0 = __byte_perm(x01, x23, 0x5410), d1 = __byte_perm(x01, x23, 0x7632), d2 = __byte_perm(y01, y23, 0x5410);
+        const uint32_t y01 = __byte_perm(n[4 * h], n[4 * h + 1], 0x7362), y23 = __byte_perm(n[4 * h + 2], n[4 * h + 3], 0x7362);
+        const uint32_t d0 = __byte_perm(x01, x23, 0x5410), d1 = __byte_perm(x01, x23, 0x7632);
+        const uint32_t d2 = __byte_perm(y01, y23, 0x5410), d3 = __byte_perm(y01, y23, 0x7632);
 #pragma unroll
         for (int rr = 0; rr < 2; ++rr) {
           const int from = (4 * rr + t) * 4;
           if (ONE) {
-            const uint32_t give = t == 0 ? d1 : t == 1 ? d0 : d2;
-            const uint32_t got = __shfl_sync(0xffffffffu, give, from + (g & 3));
-            pb[nt][2 * h + rr] = g < 3 ? got : 0u;
+            const uint32_t got = __shfl_sync(0xffffffffu, t & 2 ? (t & 1 ? d2 : d3) : (t & 1 ? d0 : d1), from + (g & 3));
+            pb[nt][2 * h + rr] = g < 4 ? got : 0u;
           } else {
-            const uint32_t got = __shfl_sync(0xffffffffu, t & 1 ? d0 : d1, from + 2 * (g >> 2) + (g & 1));
-            const uint32_t got2 = __shfl_sync(0xffffffffu, d2, from + 2 * (g >> 2));
-            pb[nt][2 * h + rr] = (g & 3) < 2 ? got : (g & 3) == 2 ? got2 : 0u;
+            const uint32_t low = __shfl_sync(0xffffffffu, t & 1 ? d0 : d1, from + 2 * (g >> 2) + (g & 1));
+            const uint32_t high = __shfl_sync(0xffffffffu, t & 1 ? d2 : d3, from + 2 * (g >> 2) + (g & 1));
+            pb[nt][2 * h + rr] = g & 2 ? high : low;
           }
         }
       }
@@ -358,7 +353,7 @@ __global__ void __launch_bounds__(QC_MAX_WARPS * 32) qcache_attend_kernel(QcAtte
         a[w][4 * half + 3] = __byte_perm(t2, t3, 0x7632);
       }
     }
-    const float v_now = v_mul * (t & 1 ? 256.0f : 1.0f) * 1.1920928955078125e-7f;   // 2^-23
+    const float v_now = v_mul * ((t & 1 ? 65536.0f : 1.0f) / QC_ONE);
     if (more) load_v(next);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
