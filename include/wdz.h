@@ -343,7 +343,10 @@ int wdz_qcache_store(wdz_engine* e, const wdz_qcache* cache, const void* k_dev, 
  * zeroed when clear_skipped != 0. */
 int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_dev, int64_t ldq, int q_dtype, int n_q_heads,
                          const int32_t* slot_ids_dev, const int32_t* lens_dev, int n_rows, float scale, void* out_dev,
-                         int64_t ldo, int out_dtype, int clear_skipped, wdz_stream s);
+                         int64_t ldo, int out_dtype, int clear_skipped, void* scratch_dev, size_t scratch_bytes, wdz_stream s);
+/* Bytes of scratch (16-byte aligned, contents irrelevant, the call's own until it has run) with which the call
+ * above takes a few long rows apart over all SMs; 0 where it wants none.  Without it those rows are slower. */
+int64_t wdz_qcache_attention_scratch(const wdz_engine* e, const wdz_qcache* cache, int n_q_heads, int n_rows);
 /* wdz_linear_rows with 4-bit weights: y f32 [M][N] = x[M][K] W^T (+ bias, x_dtype [N]) (+ residual f32 [M][N], which
  * may be y), W[n][k] = (u - 8) * scale[n][k / group], group 32, 64 or 128.  w_dev: K is padded to Kp, a multiple of
  * 128, with u = 8; row n is Kp / 8 32-bit words; of every 128 weights word 4 t + i (t, i < 4) holds elements

@@ -37,7 +37,7 @@ def host():
     """The Python calls without a device behind them: what they refuse, they refuse before they reach the library."""
     from whisperdrz_b200.engine import Engine
     e = Engine.__new__(Engine)
-    e.device, e._ordinal, e.dtype, e.h = torch.device("cpu"), 0, torch.float32, None
+    e.device, e._ordinal, e.dtype, e.h = torch.device("cpu"), -1, torch.float32, None
     return e
 
 
@@ -96,6 +96,11 @@ def test_qcache_takes_a_layer_of_a_larger_allocation_and_refuses_the_rest():
 def test_python_calls_refuse_bad_arguments(host):
     c = _cache()
     rows = torch.zeros(3, 128)
+    good = (lambda: host.qcache_store(c, rows, rows, [0, 1, 2], [0, 0, 0]), lambda: host.qcache_attention(rows, c, [0, 1, 5], [1, 1, 1]),
+            lambda: host.linear_rows_packed(torch.zeros(2, 130), pack_linear(torch.zeros(4, 130), 64)))
+    for call in good:                        # good arguments get as far as the library, which this host does not have
+        with pytest.raises(AttributeError):
+            call()
     for bad in (dict(k=rows[:, :64]), dict(k=rows.double()), dict(v=rows[:2]), dict(v=rows.bfloat16()), dict(slots=[0, 0, 1]),
                 dict(slots=[0, 1]), dict(positions=[0]), dict(row_begin=[0, 4]), dict(row_begin=[0, 2, 1], slots=[0, 1], positions=[0, 0]),
                 dict(row_begin=[-1, 2], slots=[0], positions=[0]), dict(row_begin=[])):
@@ -129,7 +134,7 @@ def test_abi_refuses_bad_arguments_before_it_looks_at_the_engine(lib, handle):
         return lib.wdz_qcache_store(handle, C.byref(cache or _desc()), k, ldk, v, ldv, dtype, n, rb, sl, ps, runs, most, None)
 
     def attend(cache=None, q=4096, ldq=128, qt=f32, hq=2, sl=64, ln=64, n=3, scale=0.125, out=8192, ldo=128, ot=bf16):
-        return lib.wdz_qcache_attention(handle, C.byref(cache or _desc()), q, ldq, qt, hq, sl, ln, n, scale, out, ldo, ot, 0, None)
+        return lib.wdz_qcache_attention(handle, C.byref(cache or _desc()), q, ldq, qt, hq, sl, ln, n, scale, out, ldo, ot, 0, None, 0, None)
 
     def linear(x=4096, ldx=130, xt=f32, M=2, K=130, w=4096, sc=4096, g=64, b=None, r=None, N=4, y=4096):
         return lib.wdz_linear_rows_packed(handle, x, ldx, xt, M, K, w, sc, g, b, r, N, y, None)

@@ -95,7 +95,8 @@ SYMBOLS = {
     "wdz_align_capacity": (I, [P, I]),
     "wdz_align_matrix": (I, [P, P, P, P, P, I, I, P, P]),
     "wdz_qcache_store": (I, [P, C.POINTER(QCacheDesc), P, I64, P, I64, I, I, P, P, P, I, I, P]),
-    "wdz_qcache_attention": (I, [P, C.POINTER(QCacheDesc), P, I64, I, I, P, P, I, C.c_float, P, I64, I, I, P]),
+    "wdz_qcache_attention": (I, [P, C.POINTER(QCacheDesc), P, I64, I, I, P, P, I, C.c_float, P, I64, I, I, P, SZ, P]),
+    "wdz_qcache_attention_scratch": (I64, [P, C.POINTER(QCacheDesc), I, I]),
     "wdz_linear_rows_packed": (I, [P, P, I64, I, I, I, P, P, I, P, P, I, P, P]),
     "wdz_dtw": (I, [P, P, I64, I64, P, P, P, P, P, I, I, I, I, P, P, P, P]),
 }

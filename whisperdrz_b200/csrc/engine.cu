@@ -1123,9 +1123,21 @@ int wdz_finalize(wdz_engine* e) {
     allow(gemv_packed_f32_kernel<1, 4>, GP_F32_CHUNK<1> * 2048);
     allow(gemv_packed_f32_kernel<4, 1>, GP_F32_CHUNK<4> * 8192); allow(gemv_packed_f32_kernel<4, 2>, GP_F32_CHUNK<4> * 8192);
     allow(gemv_packed_f32_kernel<4, 4>, GP_F32_CHUNK<4> * 8192);
+    auto attend = [&](auto tq, auto to) {
+      using TQ = decltype(tq);
+      using TO = decltype(to);
+      auto open = [&](auto kern) {
+        allow(kern, 227 * 1024);
+        // CTAs of one to four warps share an SM by their rings: always the largest share of it as shared memory
+        if (ce4 == cudaSuccess) ce4 = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+      };
+      open(qcache_attend_kernel<TQ, TO, 1, true>); open(qcache_attend_kernel<TQ, TO, 1, false>);
+      open(qcache_attend_kernel<TQ, TO, 2, false>); open(qcache_attend_kernel<TQ, TO, 4, false>);
+    };
+    attend(bf16(), bf16()); attend(bf16(), 0.0f); attend(0.0f, bf16()); attend(0.0f, 0.0f);
     if (ce4 != cudaSuccess) {
       cudaGetLastError();
-      return e->fail(WDZ_ECUDA, "gemv_packed smem attribute: %s", cudaGetErrorString(ce4));
+      return e->fail(WDZ_ECUDA, "low-bit kernel attribute: %s", cudaGetErrorString(ce4));
     }
   }
   if (cudaFuncSetAttribute(dtw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) {
@@ -1876,7 +1888,39 @@ int qcache_view(wdz_engine* e, const char* who, const wdz_qcache* c, QcView* v) 
   return WDZ_OK;
 }
 
+// How a launch of qcache_attend_kernel is cut: warps to a CTA, CTAs to a cluster, lone CTAs (parts) to an item.
+struct QcAttendPlan { int warps, cluster, parts; };
+
+QcAttendPlan qcache_attend_plan(const wdz_engine* e, int64_t items, int tiles) {
+  QcAttendPlan plan{4, 1, 1};
+  const int64_t sms = e->sm_count;
+  if (items * 4 <= sms * 8) {
+    while (plan.cluster < 8 && items * plan.cluster * 4 < sms * 8 && plan.cluster * 4 < tiles) plan.cluster *= 2;
+    if (plan.cluster == 8 && tiles > 8 * 4 * 4) {
+      // more than four tiles a warp: as many CTAs as the SMs take at four each, every warp with as many tiles as the next
+      int64_t parts = sms * 4 / items;
+      if (parts > QC_MAX_PARTS) parts = QC_MAX_PARTS;
+      const int64_t each = (tiles + 4 * parts - 1) / (4 * parts);
+      parts = (tiles + 4 * each - 1) / (4 * each);
+      if (parts > 8) plan.parts = (int)parts, plan.cluster = 1;
+    }
+  } else if (tiles <= 12) {
+    plan.warps = tiles <= 8 ? 1 : 2;
+  } else if (items > sms * 4 && items <= sms * 5) {
+    plan.warps = 3;
+  }
+  return plan;
+}
+
 }  // namespace
+
+int64_t wdz_qcache_attention_scratch(const wdz_engine* e, const wdz_qcache* cache, int n_q_heads, int n_rows) {
+  if (!e || !cache || n_rows < 0 || cache->n_heads < 1 || cache->n_blocks < 1 || n_q_heads < 1) return WDZ_EINVAL;
+  const int group = n_q_heads / cache->n_heads, pairs = group <= 2 ? 1 : group <= 4 ? 2 : 4;
+  const int64_t items = (int64_t)n_rows * cache->n_heads;
+  const QcAttendPlan plan = qcache_attend_plan(e, items, cache->n_blocks);
+  return plan.parts > 1 ? (int64_t)sizeof(float) * items * plan.parts * 2 * pairs * (QC_HD + 2) : 0;
+}
 
 int wdz_qcache_store(wdz_engine* e, const wdz_qcache* cache, const void* k_dev, int64_t ldk, const void* v_dev, int64_t ldv,
                      int dtype, int n_rows, const int32_t* row_begin_dev, const int32_t* slot_ids_dev,
@@ -1901,20 +1945,28 @@ int wdz_qcache_store(wdz_engine* e, const wdz_qcache* cache, const void* k_dev, 
   p.row_begin = row_begin_dev; p.slots = slot_ids_dev; p.positions = positions_dev;
   if ((rc = check_ready(e))) return rc;
   DeviceScope on(e->device);
+  if (!row_begin_dev) {
+    if (dtype == WDZ_BF16) launch_pdl(e, qcache_step_kernel<bf16>, dim3(n_runs), dim3(320), 0, (cudaStream_t)s, p, e->status);
+    else launch_pdl(e, qcache_step_kernel<float>, dim3(n_runs), dim3(320), 0, (cudaStream_t)s, p, e->status);
+    WDZ_LAUNCH_CHECK(e, "qcache_step");
+    return WDZ_OK;
+  }
   if (max_run > n_rows) max_run = n_rows;
-  int blocks = row_begin_dev ? (max_run + 2 * QC_BLOCK - 2) / QC_BLOCK : 1;   // a run may start at a block's last token
+  int blocks = (max_run + 2 * QC_BLOCK - 2) / QC_BLOCK;   // a run may start at a block's last token
   if (blocks < 1) blocks = 1;
   if (blocks > p.c.n_blocks) blocks = p.c.n_blocks;
-  const dim3 grid(blocks, 2 * p.c.n_heads, n_runs);
-  if (dtype == WDZ_BF16) launch_pdl(e, qcache_store_kernel<bf16>, grid, dim3(64), 0, (cudaStream_t)s, p, e->status);
-  else launch_pdl(e, qcache_store_kernel<float>, grid, dim3(64), 0, (cudaStream_t)s, p, e->status);
+  // a unit in one warp's registers: 64 of them in bf16; twice that in f32 is shared by two warps
+  const int share = dtype == WDZ_BF16 ? 1 : 2, units = 4 / share;
+  const dim3 grid(blocks, (2 * p.c.n_heads + units - 1) / units, n_runs);
+  if (dtype == WDZ_BF16) launch_pdl(e, qcache_store_kernel<bf16, 1>, grid, dim3(128), 0, (cudaStream_t)s, p, e->status);
+  else launch_pdl(e, qcache_store_kernel<float, 2>, grid, dim3(128), 0, (cudaStream_t)s, p, e->status);
   WDZ_LAUNCH_CHECK(e, "qcache_store");
   return WDZ_OK;
 }
 
 int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_dev, int64_t ldq, int q_dtype, int n_q_heads,
                          const int32_t* slot_ids_dev, const int32_t* lens_dev, int n_rows, float scale, void* out_dev,
-                         int64_t ldo, int out_dtype, int clear_skipped, wdz_stream s) {
+                         int64_t ldo, int out_dtype, int clear_skipped, void* scratch_dev, size_t scratch_bytes, wdz_stream s) {
   if (!e) return WDZ_EINVAL;
   int rc;
   QcAttendParams p{};
@@ -1936,25 +1988,25 @@ int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_d
   p.n_rows = n_rows; p.group = n_q_heads / p.c.n_heads; p.scale = scale; p.clear_skipped = clear_skipped != 0;
   if ((rc = check_ready(e))) return rc;
   DeviceScope on(e->device);
-  // CTAs per (row, key head): enough that the SMs have work, not more than there are tiles for their warps
   const int64_t items = (int64_t)n_rows * p.c.n_heads;
-  const int most = p.group > 4 ? 8 : 16;
-  int warps = 4, cluster = 1;
-  while (cluster < most && items * cluster < 3 * e->sm_count && cluster * warps < p.c.n_blocks) cluster *= 2;
-  if (cluster == most && cluster * warps * 2 < p.c.n_blocks) warps = QC_MAX_WARPS;
-  if (items * cluster > INT32_MAX) return e->fail(WDZ_ECAPACITY, "wdz_qcache_attention: %d rows of %d heads", n_rows, p.c.n_heads);
+  const int pairs = p.group <= 2 ? 1 : p.group <= 4 ? 2 : 4, step = 2 * pairs * (QC_HD + 2);
+  QcAttendPlan plan = qcache_attend_plan(e, items, p.c.n_blocks);
+  if (plan.parts > 1) {
+    const size_t need = sizeof(float) * (size_t)items * plan.parts * step;
+    if (scratch_dev && scratch_bytes >= need && !((uintptr_t)scratch_dev & 15)) p.part = (float*)scratch_dev;
+    else plan.parts = 1, plan.cluster = 8;
+  }
+  if (items * plan.cluster * plan.parts > INT32_MAX)
+    return e->fail(WDZ_ECAPACITY, "wdz_qcache_attention: %d rows of %d heads", n_rows, p.c.n_heads);
   auto go = [&](auto kern) -> int {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(items * cluster)); cfg.blockDim = dim3(warps * 32); cfg.stream = (cudaStream_t)s;
+    cfg.dynamicSmemBytes = (size_t)plan.warps * QC_RING + sizeof(float) * step * (plan.warps + (plan.cluster > 1 ? plan.cluster : 0));
+    cfg.gridDim = dim3((unsigned)(items * plan.cluster * plan.parts)); cfg.blockDim = dim3(plan.warps * 32); cfg.stream = (cudaStream_t)s;
     cudaLaunchAttribute attr[2];
     int n = 0;
-    if (cluster > 1) {
-      if (cluster > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
-        cudaError_t ce = cudaGetLastError();
-        return e->fail(WDZ_ECUDA, "qcache_attend cluster attribute: %s", cudaGetErrorString(ce));
-      }
+    if (plan.cluster > 1) {
       attr[n].id = cudaLaunchAttributeClusterDimension;
-      attr[n].val.clusterDim = {(unsigned)cluster, 1, 1};
+      attr[n].val.clusterDim = {(unsigned)plan.cluster, 1, 1};
       ++n;
     }
     if (!(e->cfg.flags & WDZ_FLAG_NO_PDL)) {
@@ -1963,7 +2015,7 @@ int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_d
       ++n;
     }
     cfg.attrs = attr; cfg.numAttrs = n;
-    cudaLaunchKernelEx(&cfg, kern, p, cluster);
+    cudaLaunchKernelEx(&cfg, kern, p, plan.cluster, plan.parts, e->status);
     return WDZ_OK;
   };
   auto by_group = [&](auto tq, auto to) -> int {
@@ -1978,6 +2030,12 @@ int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_d
   else rc = out_dtype == WDZ_BF16 ? by_group(0.0f, bf16()) : by_group(0.0f, 0.0f);
   if (rc) return rc;
   WDZ_LAUNCH_CHECK(e, "qcache_attend");
+  if (plan.parts > 1) {
+    const dim3 grid((unsigned)(items * p.group));
+    if (out_dtype == WDZ_BF16) launch_pdl(e, qcache_merge_kernel<bf16>, grid, dim3(256), 0, (cudaStream_t)s, p, plan.parts, step);
+    else launch_pdl(e, qcache_merge_kernel<float>, grid, dim3(256), 0, (cudaStream_t)s, p, plan.parts, step);
+    WDZ_LAUNCH_CHECK(e, "qcache_merge");
+  }
   return WDZ_OK;
 }
 

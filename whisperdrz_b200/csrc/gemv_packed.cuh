@@ -130,7 +130,7 @@ template <int PAIRS> constexpr int GP_F32_CHUNK = PAIRS == 1 ? 40 : 10;   // the
 
 // Block = 8 warps; grid = (tiles of 16 features x split / 8, rows / 2).  GS: scales of a segment of 128 weights.
 template <int GS>
-__global__ void __launch_bounds__(GP_WARPS * 32) gemv_packed_s8_kernel(GemvPackedParams p) {
+__global__ void __launch_bounds__(GP_WARPS * 32, 3) gemv_packed_s8_kernel(GemvPackedParams p) {
   extern __shared__ __align__(16) uint2 xs[];   // [segment][i][lane]: a lane's two operand words
   __shared__ float red[GP_WARPS][GP_S8_ROWS][17];
   __shared__ float tops[GP_WARPS][GP_S8_ROWS];

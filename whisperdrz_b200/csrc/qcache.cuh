@@ -2,11 +2,12 @@
 //
 //   value(slot, head, token, c) = int8[slot][head][token][c] * scale[slot][head][token / 64]     (K and V alike)
 //
-//   qcache_store_kernel  - rounds rows into the cache: s = max|x| / 127 over the 64 tokens x 64 values of a block,
-//       q = rint(x / s).  A block that is continued keeps the larger scale, and what it held is rounded to it.
-//   qcache_attend_kernel - one query row per (slot, length): softmax(scale * q K^T) V over the slot's first tokens.
+//   qcache_store_kernel, qcache_step_kernel - round rows into the cache: s = max|x| / 127 over the 64 tokens x 64 values
+//       of a block, q = rint(x / s).  A block that is continued keeps the larger scale, and what it held is rounded to it.
+//   qcache_attend_kernel, qcache_merge_kernel - one query row per (slot, length): softmax(scale * q K^T) V over the slot's first tokens.
 #pragma once
 #include "../../include/wdz.h"
+#include "attention.cuh"
 #include "common.cuh"
 #include "gemv_packed.cuh"
 
@@ -31,8 +32,15 @@ struct QcStoreParams {
   const int *row_begin, *slots, *positions;
 };
 
-// rint(x / s), half to even, exactly: the rounded product with 1 / s is at most one off, and the remainder
-// x - q s has so few bits that the fused multiply-add gives it without rounding wherever it decides.
+// ---- store ---------------------------------------------------------------------------------------------------------
+// Bound by the rows' bytes (2 or 4 a value) and the cache's (1).  rint(x / s) has to be exact, a value next to a half step
+// included, at a few instructions a value: x (1 / s) is rounded to a whole number q by one fused multiply-add with
+// 1.5 2^23; 1 / s is off by 2^-24, so q is at most one off and only near a half step.  The remainder d = x - q s has so few
+// bits that one more fused multiply-add gives it without rounding wherever it decides (q s is a multiple of s's last bit,
+// x of s's last bit / 2 or less, and |d| <= s / 2 needs 24 of those); |d| < s / 2 everywhere proves q right, and where a
+// lane sees anything else (ties, NaN) its values are settled one by one by qc_code.
+
+// rint(x / s), half to even, settled by the remainder.
 __device__ __forceinline__ int qc_code(float x, float s, float inv) {
   const float lim = fminf(fmaxf(x * inv, -127.0f), 127.0f);   // infinities saturate; NaN becomes a bound and is set aside below
   float q = rintf(lim);
@@ -44,69 +52,282 @@ __device__ __forceinline__ int qc_code(float x, float s, float inv) {
   return x == x ? (int)q : 0;
 }
 
-// rint(q * s_old / s_new): both products fit a double, and the quotient is never nearer to a half than its rounding.
-__device__ __forceinline__ int qc_recode(int q, double s_old, double s_new) {
-  return __double2int_rn(__ddiv_rn((double)q * s_old, s_new));
+// Eight values -> eight bytes.
+__device__ __forceinline__ uint2 qc_code8(const float (&x)[8], float s, float inv) {
+  constexpr float MAGIC = 12582912.0f;   // 1.5 2^23
+  uint32_t n[8];
+  float worst = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float t = fmaf(x[i], inv, MAGIC);
+    n[i] = __float_as_uint(t);
+    worst = fmaxf(worst, fabsf(fmaf(MAGIC - t, s, x[i])));
+  }
+  if (!(worst < 0.5f * s)) {   // a NaN is lost in the maximum: rows that hold one come here with s negated
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n[i] = (uint32_t)qc_code(x[i], fabsf(s), inv);
+  }
+  const uint32_t a = __byte_perm(n[0], n[1], 0x0040), b = __byte_perm(n[2], n[3], 0x0040);
+  const uint32_t c = __byte_perm(n[4], n[5], 0x0040), d = __byte_perm(n[6], n[7], 0x0040);
+  return make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410));
+}
+
+// rint(q s_old / s_new), half to even, of eight bytes.  The rounded quotient is at most one off; both products are exact
+// in 64 bits, and so is their difference wherever it decides.
+__device__ __forceinline__ uint2 qc_recode8(uint2 w, float s_old, float s_new) {
+  const float r = __fdiv_rn(s_old, s_new);
+  const double so = s_old, sn = s_new, half = 0.5 * sn;
+  uint32_t out[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t word = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int q = (int)(int8_t)((h ? w.y : w.x) >> (8 * b));
+      int n = __float2int_rn((float)q * r);
+      const double d = (double)q * so - (double)n * sn;
+      const bool odd = n & 1;
+      if (d > half || (d == half && odd)) ++n;
+      else if (d < -half || (d == -half && odd)) --n;
+      word |= (uint32_t)(n & 255) << (8 * b);
+    }
+    out[h] = word;
+  }
+  return make_uint2(out[0], out[1]);
 }
 
 __device__ __forceinline__ void qc_report(DevStatus* st, int code, int detail) {
   if (atomicCAS(&st->code, 0, code) == 0) st->detail = detail;
 }
 
-// Block = 64 threads (a thread per value of the head); grid = (blocks of the longest run, head and K / V, run).
+// Eight neighbouring values of a row, as they lie.
+template <typename T> struct QcRaw;
+template <> struct QcRaw<bf16> {
+  uint4 v;
+  __device__ void load(const void* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ void clear() { v = make_uint4(0, 0, 0, 0); }
+  __device__ void get(float (&x)[8]) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  }
+  // the largest magnitude's bits as fp32's, infinities and NaN above all numbers
+  __device__ uint32_t top() const {
+    const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+    return max(m << 16, m & 0xffff0000u);
+  }
+};
+template <> struct QcRaw<float> {
+  float4 a, b;
+  __device__ void load(const void* p) { a = reinterpret_cast<const float4*>(p)[0]; b = reinterpret_cast<const float4*>(p)[1]; }
+  __device__ void clear() { a = b = make_float4(0, 0, 0, 0); }
+  __device__ void get(float (&x)[8]) const {
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+  __device__ uint32_t top() const {
+    float x[8];
+    get(x);
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    return m;
+  }
+};
 template <typename T>
-__global__ void __launch_bounds__(64) qcache_store_kernel(QcStoreParams p, DevStatus* status) {
-  pdl_trigger();
-  pdl_wait();
-  __shared__ float red[2];
-  const int run = blockIdx.z, head = blockIdx.y >> 1, c = threadIdx.x;
-  const bool is_v = blockIdx.y & 1;
-  const int slot = p.slots[run], p0 = p.positions[run];
-  const int r0 = p.row_begin ? p.row_begin[run] : run, r1 = p.row_begin ? p.row_begin[run + 1] : run + 1;
-  const int room = p.c.n_blocks * QC_BLOCK;
-  if (slot < 0 || slot >= p.c.n_slots || r1 <= r0) return;
-  int dup = 0;
-  for (int j = run + 1 + threadIdx.x; j < p.n_runs; j += 64) dup |= p.slots[j] == slot;
-  if (r0 < 0 || r1 > p.n_rows || p0 < 0 || p0 > room - (r1 - r0) || __syncthreads_or(dup)) {
-    if (threadIdx.x == 0) qc_report(status, WDZ_EINVAL, 2000000 + run);
-    return;
+__device__ __forceinline__ uint32_t qc_finite_top(const QcRaw<T>& r) {   // the same without infinities and NaN
+  float x[8];
+  r.get(x);
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
+    if (u < 0x7f800000u) m = max(m, u);
   }
-  const int p1 = p0 + (r1 - r0);
-  int8_t* cv = (is_v ? p.c.v : p.c.k) + slot * p.c.slot_stride + (int64_t)head * room * QC_HD;
-  float* cs = (is_v ? p.c.vs : p.c.ks) + slot * p.c.scale_stride + (int64_t)head * p.c.n_blocks;
-  const T* src = reinterpret_cast<const T*>(is_v ? p.v : p.k) + head * QC_HD + c;
-  const int64_t ld = is_v ? p.ldv : p.ldk;
-  bool bad = false;
-  for (int b = p0 / QC_BLOCK + blockIdx.x; b * QC_BLOCK < p1; b += gridDim.x) {
-    const int lo = max(p0, b * QC_BLOCK), hi = min(p1, (b + 1) * QC_BLOCK);
-    float top = 0.0f;
-    for (int t = lo; t < hi; ++t) {
-      const float x = to_f(src[(int64_t)(r0 + t - p0) * ld]);
-      if (fabsf(x) <= 3.402823466e38f) top = fmaxf(top, fabsf(x)); else bad = true;
-    }
-    top = warp_max(top);
-    __syncthreads();
-    if ((c & 31) == 0) red[c >> 5] = top;
-    __syncthreads();
-    top = fmaxf(red[0], red[1]);
-    const float old = lo > b * QC_BLOCK ? cs[b] : 0.0f;
-    const float now = fmaxf(old, top >= QC_TINY ? __fdiv_rn(top, 127.0f) : 0.0f);
-    if (now > old && lo > b * QC_BLOCK)
-      for (int t = b * QC_BLOCK; t < lo; ++t) {
-        int8_t* q = cv + (int64_t)t * QC_HD + c;
-        *q = (int8_t)qc_recode(*q, old, now);
-      }
-    const float inv = now > 0.0f ? 1.0f / now : 0.0f;
-    for (int t = lo; t < hi; ++t) {
-      const float x = to_f(src[(int64_t)(r0 + t - p0) * ld]);
-      cv[(int64_t)t * QC_HD + c] = now > 0.0f ? (int8_t)qc_code(x, now, inv) : (int8_t)0;
-    }
-    __syncthreads();
-    if (c == 0) cs[b] = now;
-  }
-  if (bad) qc_report(status, WDZ_ENAN, 2000000 + run);
+  return m;
 }
 
+// A run's place; ok is false (and reported, unless its slot is outside or it is empty) where it cannot be stored.
+struct QcRun {
+  int slot, p0, p1, r0;
+  bool ok;
+  __device__ QcRun(const QcStoreParams& p, int run, bool reports, DevStatus* status) {   // by all threads of the block
+    slot = p.slots[run];
+    p0 = p.positions[run];
+    r0 = p.row_begin ? p.row_begin[run] : run;
+    const int r1 = p.row_begin ? p.row_begin[run + 1] : run + 1, room = p.c.n_blocks * QC_BLOCK;
+    int again = 0;
+    for (int j = run + 1 + threadIdx.x; j < p.n_runs; j += blockDim.x) again |= p.slots[j] == slot;
+    again = __syncthreads_or(again);   // a later run names the slot: the last one counts
+    ok = slot >= 0 && slot < p.c.n_slots && r1 > r0;
+    if (ok && (r0 < 0 || r1 > p.n_rows || p0 < 0 || p0 > room - (r1 - r0) || again)) {
+      if (reports && threadIdx.x == 0) qc_report(status, WDZ_EINVAL, 2000000 + run);
+      ok = false;
+    }
+    p1 = ok ? p0 + (r1 - r0) : 0;
+  }
+};
+
+// Where a head's K or V lies.
+struct QcPlace {
+  int8_t* q;
+  float* s;
+  __device__ QcPlace(const QcView& c, int slot, int head, bool is_v) {
+    q = (is_v ? c.v : c.k) + slot * c.slot_stride + (int64_t)head * c.n_blocks * (QC_BLOCK * QC_HD);
+    s = (is_v ? c.vs : c.ks) + slot * c.scale_stride + (int64_t)head * c.n_blocks;
+  }
+};
+
+__device__ __forceinline__ float qc_scale(uint32_t top_bits) {
+  const float top = __uint_as_float(top_bits);
+  return top >= QC_TINY ? __fdiv_rn(top, 127.0f) : 0.0f;
+}
+
+// Runs of any length.  A unit is a block of 64 tokens of one head, K or V: SHARE warps hold it in registers between the
+// maximum and the rounding, so the rows are read once; a lane has 8 neighbouring values of a token, four tokens at a time.
+// Block = 4 warps; grid = (blocks of the longest run, groups of 4 / SHARE units of heads and K / V, run).
+template <typename T, int SHARE>
+__global__ void __launch_bounds__(128) qcache_store_kernel(QcStoreParams p, DevStatus* status) {
+  constexpr int TOKENS = QC_BLOCK / SHARE, STEPS = TOKENS / 4;
+  __shared__ uint32_t tops[4];
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % SHARE;
+  const int unit = blockIdx.y * (4 / SHARE) + warp / SHARE;
+  const bool has = unit < 2 * p.c.n_heads;
+  const bool is_v = has && unit >= p.c.n_heads;
+  const int head = has ? (is_v ? unit - p.c.n_heads : unit) : 0;
+  pdl_wait();
+  const QcRun run(p, blockIdx.z, blockIdx.x == 0 && blockIdx.y == 0, status);
+  if (!run.ok) return;
+  const QcPlace place(p.c, run.slot, head, is_v);
+  const int64_t ld = (is_v ? p.ldv : p.ldk) * (int64_t)sizeof(T);
+  const char* src = reinterpret_cast<const char*>(is_v ? p.v : p.k) + (int64_t)(head * QC_HD + 8 * (lane & 7)) * sizeof(T);
+  for (int b = run.p0 / QC_BLOCK + blockIdx.x; b * QC_BLOCK < run.p1; b += gridDim.x) {
+    const int lo = max(run.p0, b * QC_BLOCK), hi = min(run.p1, (b + 1) * QC_BLOCK);
+    const int t0 = b * QC_BLOCK + part * TOKENS + (lane >> 3);   // this lane's tokens: t0, t0 + 4, ..
+    QcRaw<T> raw[STEPS];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int t = t0 + 4 * i;
+      raw[i].clear();
+      if (has && t >= lo && t < hi) raw[i].load(src + (int64_t)(run.r0 + t - run.p0) * ld);
+    }
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) top = max(top, raw[i].top());
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (SHARE > 1) {
+      __syncthreads();
+      if (lane == 0) tops[warp] = top;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < SHARE; ++i) top = max(top, tops[warp - part + i]);
+    }
+    const bool odd = top >= 0x7f800000u;
+    if (odd) {   // an infinity or a NaN: the scale goes by the rest
+      top = 0;
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) top = max(top, qc_finite_top(raw[i]));
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) qc_report(status, WDZ_ENAN, 2000000 + (int)blockIdx.z);
+    }
+    if (SHARE > 1) {
+      if (__syncthreads_or(odd)) {
+        if (lane == 0) tops[warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < SHARE; ++i) top = max(top, tops[warp - part + i]);
+      }
+    }
+    const bool entered = lo > b * QC_BLOCK;   // behind the block's first token: what it holds stays
+    const float old = has && entered ? place.s[b] : 0.0f, now = fmaxf(old, qc_scale(top));
+    if (has) {
+      if (now > old && entered)
+        for (int t = b * QC_BLOCK + part * 4 + (lane >> 3); t < lo; t += 4 * SHARE) {
+          uint2* at = reinterpret_cast<uint2*>(place.q + (int64_t)t * QC_HD + 8 * (lane & 7));
+          *at = qc_recode8(*at, old, now);
+        }
+      const float inv = now > 0.0f ? __fdiv_rn(1.0f, now) : 0.0f, sign = odd ? -now : now;
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const int t = t0 + 4 * i;
+        if (t >= lo && t < hi) {
+          float x[8];
+          raw[i].get(x);
+          *reinterpret_cast<uint2*>(place.q + (int64_t)t * QC_HD + 8 * (lane & 7)) = now > 0.0f ? qc_code8(x, sign, inv) : make_uint2(0, 0);
+        }
+      }
+    }
+    if (SHARE > 1) __syncthreads(); else __syncwarp();   // every part has read the old scale
+    if (has && part == 0 && lane == 0) place.s[b] = now;
+  }
+}
+
+// One row a run (a decode step).  Block = a run; eight threads a head of K or V.  Where a scale grows, the whole block
+// rounds the unit's earlier tokens to it together: alone, its eight threads would take up to 63 turns.
+template <typename T>
+__global__ void __launch_bounds__(320) qcache_step_kernel(QcStoreParams p, DevStatus* status) {
+  constexpr int UNITS = 320 / 8;
+  __shared__ float olds[UNITS], news[UNITS];
+  __shared__ int grown[UNITS], n_grown;
+  pdl_trigger();
+  const int c = threadIdx.x & 7, mine = threadIdx.x >> 3, units = 2 * p.c.n_heads;
+  pdl_wait();
+  const QcRun run(p, blockIdx.x, true, status);
+  if (!run.ok) return;
+  const int b = run.p0 / QC_BLOCK, kept = run.p0 % QC_BLOCK;
+  for (int first = 0; first < units; first += UNITS) {
+    const int unit = first + mine;
+    const bool has = unit < units, is_v = unit >= p.c.n_heads;
+    const int head = has ? (is_v ? unit - p.c.n_heads : unit) : 0;
+    const QcPlace place(p.c, run.slot, head, is_v);
+    __syncthreads();
+    if (threadIdx.x == 0) n_grown = 0;
+    QcRaw<T> raw;
+    raw.clear();
+    float old = 0.0f;
+    if (has) {
+      raw.load(reinterpret_cast<const T*>(is_v ? p.v : p.k) + (int64_t)run.r0 * (is_v ? p.ldv : p.ldk) + head * QC_HD + 8 * c);
+      if (kept) old = place.s[b];
+    }
+    uint32_t top = raw.top();
+    auto over8 = [&] {
+#pragma unroll
+      for (int i = 4; i > 0; i >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, i));
+    };
+    over8();
+    const bool odd = top >= 0x7f800000u;
+    if (__any_sync(0xffffffffu, odd)) {
+      if (odd) top = qc_finite_top(raw);
+      over8();
+      if (odd && c == 0) qc_report(status, WDZ_ENAN, 2000000 + (int)blockIdx.x);
+    }
+    const float now = fmaxf(old, qc_scale(top));
+    __syncthreads();
+    if (has) {
+      float x[8];
+      raw.get(x);
+      const float inv = now > 0.0f ? __fdiv_rn(1.0f, now) : 0.0f;
+      *reinterpret_cast<uint2*>(place.q + (int64_t)run.p0 * QC_HD + 8 * c) = now > 0.0f ? qc_code8(x, odd ? -now : now, inv) : make_uint2(0, 0);
+      if (c == 0) {
+        if (!kept || now > old) place.s[b] = now;
+        if (kept && now > old) {
+          const int i = atomicAdd(&n_grown, 1);   // the order of the list does not matter
+          grown[i] = unit; olds[i] = old; news[i] = now;
+        }
+      }
+    }
+    __syncthreads();
+    const int pieces = 8 * kept;   // of 8 bytes, a unit
+    for (int i = threadIdx.x; i < n_grown * pieces; i += blockDim.x) {
+      const int k = i / pieces, g = grown[k];
+      const QcPlace to(p.c, run.slot, g >= p.c.n_heads ? g - p.c.n_heads : g, g >= p.c.n_heads);
+      uint2* at = reinterpret_cast<uint2*>(to.q + (int64_t)b * (QC_BLOCK * QC_HD)) + (i - k * pieces);
+      *at = qc_recode8(*at, olds[k], news[k]);
+    }
+  }
+}
+
+// ---- attention ---------------------------------------------------------------------------------------------------------
 struct QcAttendParams {
   QcView c;
   const void* q; int64_t ldq;
@@ -115,9 +336,9 @@ struct QcAttendParams {
   int n_rows, group;        // query heads per key head
   float scale;
   bool clear_skipped;       // rows of slots outside the cache: zeros instead of what was there
+  float* part;              // partial results [row, key head][parts], when the CTAs of a row are no cluster
 };
 
-// ---- attention -----------------------------------------------------------------------------------------------------
 // One query row per slot is a matrix-vector product, bound by the bytes of K and V.  Taking the bytes apart on the CUDA
 // cores would cost more instructions than there are issue slots at the memory's rate (about 1400 a tile of 8 KB and
 // scheduler), so both products run on the integer matrix instruction m16n8k32, which takes the cache's bytes as they lie:
@@ -144,16 +365,6 @@ constexpr float QC_ONE = 4294967040.0f;            // the weight 1 in steps: the
 __device__ __forceinline__ void qc_mma_su(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint4 qc_ld16(const int8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 qc_ld8(const int8_t* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
 }
 __device__ __forceinline__ float qc_ex2(float x) {
   float y;
@@ -192,82 +403,279 @@ __device__ __forceinline__ QcMerged qc_merge(const float* part, int step, int n,
   return r;
 }
 
-// NT: pairs of query heads of a key head.  ONE: a single query head (its scores then reach all four lanes of a group,
-// and one shuffle a word is enough).  A cluster of CTAs takes an item (row, key head); its warps take tiles in turn, and
-// the CTAs' partial results meet in the first CTA's shared memory.
-template <typename TQ, typename TO, int NT, bool ONE>
-__global__ void __launch_bounds__(QC_MAX_WARPS * 32) qcache_attend_kernel(QcAttendParams p, int cluster) {
-  constexpr int HEADS = 2 * NT, STEP = HEADS * (QC_HD + 2), MAX_CLUSTER = NT == 4 ? 8 : 16;
-  __shared__ float warp_part[QC_MAX_WARPS * STEP];
-  __shared__ float cta_part[MAX_CLUSTER * STEP];
-  pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  const int g = lane >> 2, t = lane & 3;
-  const int rank = blockIdx.x % cluster;
-  const int64_t item = blockIdx.x / cluster;
-  const int r = (int)(item / p.c.n_heads), hk = (int)(item % p.c.n_heads);
-  if (cluster > 1) qc_cluster_arrive();   // waited for below: every CTA of the cluster runs before another writes to it
-  pdl_wait();
-  const int slot = p.slots[r];
-  const bool skipped = slot < 0 || slot >= p.c.n_slots;
-  const int len = skipped ? 0 : min(max(p.lens[r], 0), p.c.n_blocks * QC_BLOCK);
-  const int64_t at = skipped ? 0 : slot;
-  const int64_t head_at = (int64_t)hk * p.c.n_blocks;
-  const int8_t* K = p.c.k + at * p.c.slot_stride + head_at * (QC_BLOCK * QC_HD);
-  const int8_t* V = p.c.v + at * p.c.slot_stride + head_at * (QC_BLOCK * QC_HD);
-  const float* ks = p.c.ks + at * p.c.scale_stride + head_at;
-  const float* vs = p.c.vs + at * p.c.scale_stride + head_at;
-  const int tiles = (len + QC_BLOCK - 1) / QC_BLOCK, stride = cluster * warps;
-  int tile = rank * warps + warp;
+// A warp's tiles pass through a ring of its own in shared memory, K and V of a tile in turn, three places of 4 KB: one is
+// worked on and two are under way (8 KB a warp).  One lane moves a piece (contiguous, 64 bytes a token, no more tokens than
+// the row has) and its scale there with asynchronous copies, so the bytes in flight cost no registers and no warp waits for
+// another.  Three places instead of four let a third more warps share an SM.  Waits are bounded.
+constexpr int QC_TILE = QC_BLOCK * QC_HD;          // bytes of a tile of K, or V
+constexpr int QC_PLACES = 3;
+constexpr int QC_PLACE = QC_TILE + 16;             // and its scale
+constexpr int QC_RING = QC_PLACES * (QC_PLACE + 8) + 8;   // places, their barriers; a multiple of 16
 
-  uint4 k[8];
-  uint2 v[16];
-  float k_mul = 0.0f, v_mul = 0.0f;
-  const int k_at = (16 * (g >> 2) + (g & 3)) * QC_HD + 16 * t, v_at = t * QC_HD + 8 * g;
-  auto load_k = [&](int tl) {
-    const int8_t* b = K + (int64_t)tl * (QC_BLOCK * QC_HD) + k_at;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) k[j] = qc_ld16(b + (32 * (j >> 2) + 4 * (j & 3)) * QC_HD);
-    k_mul = __ldg(ks + tl);
-  };
-  auto load_v = [&](int tl) {
-    const int8_t* b = V + (int64_t)tl * (QC_BLOCK * QC_HD) + v_at;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = qc_ld8(b + 4 * j * QC_HD);
-    v_mul = __ldg(vs + tl);
-  };
-  if (tile < tiles) { load_k(tile); load_v(tile); }
+// Waits for a phase of a barrier, with a limit.  The clock is read only once the wait is seen to be a long one.
+__device__ __forceinline__ bool qc_try(uint32_t bar, uint32_t phase) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(bar), "r"(phase) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool qc_wait(uint32_t bar, uint32_t phase, DevStatus* status) {
+  long long t0 = 0;
+  for (int spin = 1; !qc_try(bar, phase); ++spin) {
+    if ((spin & 63) == 0) {
+      if (t0 == 0) t0 = clock64();
+      else if (clock64() - t0 > ATT_WAIT_CYCLES) {
+        qc_report(status, WDZ_ETIMEOUT, 2000000 + (int)blockIdx.x);
+        return false;
+      }
+    }
+  }
+  return true;
+}
 
-  // The query's bytes: lane (g, t) makes column g, values 16 t .. 16 t + 15 of head g / 4 of the pair.
-  uint32_t qb[NT][4];
-  float q_mul[NT];
+struct QcRing {
+  const uint8_t* base;
+  uint32_t addr;              // of base in shared memory
+  int place = 0, phase = 0;   // of the piece that is waited for next
+
+  __device__ explicit QcRing(uint8_t* p) : base(p), addr(att_smem_u32(p)) {}
+  __device__ const uint8_t* data() const { return base + place * QC_PLACE; }
+  __device__ float scale() const { return *reinterpret_cast<const float*>(data() + QC_TILE); }
+  __device__ uint32_t bar(int at) const { return addr + QC_PLACES * QC_PLACE + 8 * at; }
+  __device__ void init() const {   // by one lane; two arrivals a piece: the bulk copy's and the scale's
+#pragma unroll
+    for (int i = 0; i < QC_PLACES; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 2;" ::"r"(bar(i)));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // by one lane: a piece of `tokens` tokens into place `at`
+  __device__ void fetch(int at, const int8_t* from, const float* scale_from, int tokens) const {
+    const uint32_t b = bar(at), dst = addr + at * QC_PLACE, bytes = (uint32_t)tokens * QC_HD;
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(from), "r"(bytes), "r"(b) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + QC_TILE), "l"(scale_from) : "memory");
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(b) : "memory");
+  }
+  __device__ void step() { if (++place == QC_PLACES) { place = 0; phase ^= 1; } }
+  // by the warp: waits for the next piece.  False: the wait ran out and the status word voids the result; the `behind`
+  // pieces that are still under way have been given a wait of their own, so that the ring may go.
+  __device__ bool wait(int behind, DevStatus* status) {
+    if (__all_sync(0xffffffffu, qc_wait(bar(place), phase, status))) return true;
+    for (int j = 0; j < behind; ++j) {
+      step();
+      qc_wait(bar(place), phase, status);
+    }
+    return false;
+  }
+};
+
+// A row's place in the cache.
+struct QcRow {
+  int r, hk, len;
+  bool skipped;
+  const int8_t *K, *V;
+  const float *ks, *vs;
+  __device__ QcRow(const QcAttendParams& p, uint32_t item) {
+    r = (int)(item / (uint32_t)p.c.n_heads); hk = (int)(item - (uint32_t)r * p.c.n_heads);
+    const int slot = p.slots[r];
+    const int n = p.lens[r];
+    skipped = slot < 0 || slot >= p.c.n_slots;
+    len = skipped ? 0 : min(max(n, 0), p.c.n_blocks * QC_BLOCK);
+    const int64_t at = skipped ? 0 : slot, head_at = (int64_t)hk * p.c.n_blocks;
+    K = p.c.k + at * p.c.slot_stride + head_at * QC_TILE;
+    V = p.c.v + at * p.c.slot_stride + head_at * QC_TILE;
+    ks = p.c.ks + at * p.c.scale_stride + head_at;
+    vs = p.c.vs + at * p.c.scale_stride + head_at;
+  }
+  __device__ int tiles() const { return (len + QC_BLOCK - 1) / QC_BLOCK; }
+  __device__ int tokens(int tile) const { return min(QC_BLOCK, len - tile * QC_BLOCK); }
+};
+
+// The query's bytes: lane (g, t) makes column g, values 16 t .. 16 t + 15 of head g / 4 of the pair.
+template <typename TQ, int NT>
+__device__ __forceinline__ void qc_query(const QcAttendParams& p, int r, int hk, int g, int t, uint32_t (&qb)[NT][4], float (&q_mul)[NT]) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int h = min(2 * nt + (g >> 2), p.group - 1);
-    float x[16], top = 0.0f;
-    bool fine = true;
+    float x[16], top = 0.0f, odd = 0.0f;
     qc_load16(reinterpret_cast<const TQ*>(p.q) + (int64_t)r * p.ldq + (hk * p.group + h) * QC_HD + 16 * t, x);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) { top = fmaxf(top, fabsf(x[i])); fine &= fabsf(x[i]) <= 3.402823466e38f; }
-    if (!fine) top = INFINITY;
+    for (int i = 0; i < 16; ++i) { top = fmaxf(top, fabsf(x[i])); odd = fmaf(x[i], 0.0f, odd); }
+    if (odd != odd) top = INFINITY;   // an infinity or a NaN among them
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const float lift = top < 1e-20f ? 18446744073709551616.0f : 1.0f;   // 2^64: keeps the quotient below finite
     const float steps = top > 0.0f ? QC_STEPS / (top * lift) * lift : 0.0f;
-    const int digit = (g & 3) ^ 1;   // columns d1, d0, d3, d2
+    const uint32_t digit = ((g & 3) ^ 1) * 0x11 + 0x40;   // columns d1, d0, d3, d2: that byte of two numbers
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       uint32_t n[4];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) n[b] = ((uint32_t)__float2int_rn(x[4 * w + b] * steps) + 0x80808080u) >> (8 * digit);
-      const uint32_t lo = __byte_perm(n[0], n[1], 0x0040), hi = __byte_perm(n[2], n[3], 0x0040);
-      qb[nt][w] = __byte_perm(lo, hi, 0x5410) ^ 0x80808080u;   // the digits are bytes less 128
+      for (int b = 0; b < 4; ++b) n[b] = (uint32_t)__float2int_rn(x[4 * w + b] * steps) + 0x80808080u;   // digits + 128
+      qb[nt][w] = __byte_perm(__byte_perm(n[0], n[1], digit), __byte_perm(n[2], n[3], digit), 0x5410) ^ 0x80808080u;
     }
     // an infinite or NaN query: infinity times zero makes the row NaN
     const float mul = (top * lift) * (1.0f / QC_STEPS) * (p.scale * 1.4426950408889634f) / lift;
     q_mul[nt] = __shfl_sync(0xffffffffu, mul, 16 * (t >> 1)) * (t & 1 ? 65536.0f : 1.0f);   // of the head whose scores this lane gets
   }
+}
 
+// One tile: scores, softmax weights, and their product with V added to acc.  release(place) is called when every lane has
+// taken its bytes out of a place, behind() says how many pieces are under way.  False: a wait ran out.
+template <int NT, bool ONE, typename Release, typename Behind>
+__device__ __forceinline__ bool qc_tile(QcRing& ring, int tokens, int g, int t, const uint32_t (&qb)[NT][4],
+                                        const float (&q_mul)[NT], float (&m)[NT], float (&l)[NT], float (&acc)[NT][8],
+                                        DevStatus* status, Release release, Behind behind) {
+  if (!ring.wait(behind(), status)) return false;
+  uint32_t pb[NT][4];      // the weights' bytes: word 2 ks + r
+  float alpha[NT];
+  const float k_now = ring.scale();
+  uint4 k[8];
+  {
+    const uint8_t* kt = ring.data() + (16 * (g >> 2) + (g & 3)) * QC_HD + 16 * t;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) k[j] = *reinterpret_cast<const uint4*>(kt + (32 * (j >> 2) + 4 * (j & 3)) * QC_HD);
+  }
+  __syncwarp();
+  release(ring.place);
+  ring.step();
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float s[8];
+    const float mul = q_mul[nt] * k_now;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      int c[4] = {0, 0, 0, 0};
+      mma_s8_16832(c, k[2 * i].x, k[2 * i + 1].x, k[2 * i].y, k[2 * i + 1].y, qb[nt][0], qb[nt][1]);
+      mma_s8_16832(c, k[2 * i].z, k[2 * i + 1].z, k[2 * i].w, k[2 * i + 1].w, qb[nt][2], qb[nt][3]);
+      s[2 * i] = (float)(c[0] * 256 + c[1]) * mul;
+      s[2 * i + 1] = (float)(c[2] * 256 + c[3]) * mul;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] += __shfl_xor_sync(0xffffffffu, s[j], 1);
+    if (tokens < QC_BLOCK) {
+      const int left = tokens - (16 * (g >> 2) + (g & 3));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) if (32 * (j >> 2) + 4 * (j & 3) >= left) s[j] = -INFINITY;
+    }
+    float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    const float m_new = fmaxf(m[nt], top);
+    alpha[nt] = qc_ex2(m[nt] - m_new);
+    m[nt] = m_new;
+    uint32_t n[8];
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float w = qc_ex2(s[j] - m_new);
+      sum += w;
+      n[j] = __float2uint_rn(w * QC_ONE);
+    }
+    l[nt] = fmaf(l[nt], alpha[nt], sum);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {   // tokens 32 h ..
+      const uint32_t x01 = __byte_perm(n[4 * h], n[4 * h + 1], 0x5140), x23 = __byte_perm(n[4 * h + 2], n[4 * h + 3], 0x5140);
+      const uint32_t y01 = __byte_perm(n[4 * h], n[4 * h + 1], 0x7362), y23 = __byte_perm(n[4 * h + 2], n[4 * h + 3], 0x7362);
+      const uint32_t d0 = __byte_perm(x01, x23, 0x5410), d1 = __byte_perm(x01, x23, 0x7632);
+      const uint32_t d2 = __byte_perm(y01, y23, 0x5410), d3 = __byte_perm(y01, y23, 0x7632);
+#pragma unroll
+      for (int rr = 0; rr < 2; ++rr) {
+        const int from = (4 * rr + t) * 4;
+        if (ONE) {
+          const uint32_t got = __shfl_sync(0xffffffffu, t & 2 ? (t & 1 ? d2 : d3) : (t & 1 ? d0 : d1), from + (g & 3));
+          pb[nt][2 * h + rr] = g < 4 ? got : 0u;
+        } else {
+          const uint32_t low = __shfl_sync(0xffffffffu, t & 1 ? d0 : d1, from + 2 * (g >> 2) + (g & 1));
+          const uint32_t high = __shfl_sync(0xffffffffu, t & 1 ? d2 : d3, from + 2 * (g >> 2) + (g & 1));
+          pb[nt][2 * h + rr] = g & 2 ? high : low;
+        }
+      }
+    }
+  }
+  if (!ring.wait(behind(), status)) return false;
+  const float v_now = ring.scale() * ((t & 1 ? 65536.0f : 1.0f) / QC_ONE);
+  const uint8_t* vt = ring.data() + t * QC_HD + 8 * g;
+  // V's bytes, four tokens of one value to a word: a[2 ks + r][value 8 g + i]
+  uint32_t a[4][8];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint2 v[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) v[b] = *reinterpret_cast<const uint2*>(vt + 4 * (4 * w + b) * QC_HD);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint32_t x0 = half ? v[0].y : v[0].x, x1 = half ? v[1].y : v[1].x;
+      const uint32_t x2 = half ? v[2].y : v[2].x, x3 = half ? v[3].y : v[3].x;
+      const uint32_t t0 = __byte_perm(x0, x1, 0x5140), t1 = __byte_perm(x2, x3, 0x5140);
+      const uint32_t t2 = __byte_perm(x0, x1, 0x7362), t3 = __byte_perm(x2, x3, 0x7362);
+      a[w][4 * half] = __byte_perm(t0, t1, 0x5410);
+      a[w][4 * half + 1] = __byte_perm(t0, t1, 0x7632);
+      a[w][4 * half + 2] = __byte_perm(t2, t3, 0x5410);
+      a[w][4 * half + 3] = __byte_perm(t2, t3, 0x7632);
+    }
+  }
+  __syncwarp();
+  release(ring.place);
+  ring.step();
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      int c[4] = {0, 0, 0, 0};
+      qc_mma_su(c, a[0][2 * i], a[0][2 * i + 1], a[1][2 * i], a[1][2 * i + 1], pb[nt][0], pb[nt][1]);
+      qc_mma_su(c, a[2][2 * i], a[2][2 * i + 1], a[3][2 * i], a[3][2 * i + 1], pb[nt][2], pb[nt][3]);
+      acc[nt][2 * i] = fmaf((float)(c[0] * 256 + c[1]), v_now, acc[nt][2 * i] * alpha[nt]);
+      acc[nt][2 * i + 1] = fmaf((float)(c[2] * 256 + c[3]), v_now, acc[nt][2 * i + 1] * alpha[nt]);
+    }
+  }
+  return true;
+}
+
+// NT: pairs of query heads of a key head.  ONE: a single query head (its scores then reach all four lanes of a group,
+// and one shuffle a word is enough).  A cluster of CTAs takes an item (row, key head); its warps take tiles in turn, and
+// the CTAs' partial results meet in the first CTA's shared memory.  Where a cluster is too small for a long row, `parts`
+// lone CTAs take it and leave their partial results to qcache_merge_kernel.
+template <typename TQ, typename TO, int NT, bool ONE>
+__global__ void __launch_bounds__(QC_MAX_WARPS * 32) qcache_attend_kernel(QcAttendParams p, int cluster, int parts, DevStatus* status) {
+  constexpr int HEADS = 2 * NT, STEP = HEADS * (QC_HD + 2);
+  extern __shared__ __align__(128) uint8_t qc_smem[];
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  QcRing ring(qc_smem + warp * QC_RING);
+  float* warp_part = reinterpret_cast<float*>(qc_smem + warps * QC_RING);
+  float* cta_part = warp_part + warps * STEP;
+  const int g = lane >> 2, t = lane & 3;
+  const int share = cluster * parts;   // CTAs of an item: a cluster, or `parts` lone ones, or one
+  const int rank = blockIdx.x % (uint32_t)share;
+  if (cluster > 1) qc_cluster_arrive();   // waited for below: every CTA of the cluster runs before another writes to it
+  if (lane == 0) ring.init();
+  __syncwarp();
+  pdl_wait();
+  const uint32_t item = blockIdx.x / (uint32_t)share;
+  const QcRow row(p, item);
+  const int tiles = row.tiles(), stride = share * warps, tile0 = rank * warps + warp;
+  const int mine = tile0 < tiles ? (tiles - tile0 + stride - 1) / stride : 0;   // tiles of this warp
+  // pieces: K and V of the warp's tiles in turn
+  int asked = 0;
+  const int8_t *k_from = row.K + (int64_t)tile0 * QC_TILE, *v_from = row.V + (int64_t)tile0 * QC_TILE;
+  const float *ks_from = row.ks + tile0, *vs_from = row.vs + tile0;
+  int left = row.len - tile0 * QC_BLOCK;   // tokens from there on
+  auto fetch = [&](int at) {
+    if (asked == 2 * mine) return;
+    const bool is_v = asked & 1;
+    if (lane == 0) ring.fetch(at, is_v ? v_from : k_from, is_v ? vs_from : ks_from, min(left, QC_BLOCK));
+    if (is_v) {
+      k_from += (int64_t)stride * QC_TILE; v_from += (int64_t)stride * QC_TILE;
+      ks_from += stride; vs_from += stride; left -= stride * QC_BLOCK;
+    }
+    ++asked;
+  };
+  for (int i = 0; i < QC_PLACES; ++i) fetch(i);
+  uint32_t qb[NT][4];
+  float q_mul[NT];
+  qc_query<TQ, NT>(p, row.r, row.hk, g, t, qb, q_mul);
   float m[NT], l[NT], acc[NT][8];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -275,97 +683,10 @@ __global__ void __launch_bounds__(QC_MAX_WARPS * 32) qcache_attend_kernel(QcAtte
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[nt][i] = 0.0f;
   }
-  for (; tile < tiles; tile += stride) {
-    const int next = tile + stride;
-    const bool more = next < tiles;
-    uint32_t pb[NT][4];      // the weights' bytes: word 2 ks + r
-    float alpha[NT];
-    const float k_now = k_mul;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float s[8];
-      const float mul = q_mul[nt] * k_now;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        int c[4] = {0, 0, 0, 0};
-        mma_s8_16832(c, k[2 * i].x, k[2 * i + 1].x, k[2 * i].y, k[2 * i + 1].y, qb[nt][0], qb[nt][1]);
-        mma_s8_16832(c, k[2 * i].z, k[2 * i + 1].z, k[2 * i].w, k[2 * i + 1].w, qb[nt][2], qb[nt][3]);
-        s[2 * i] = (float)(c[0] * 256 + c[1]) * mul;
-        s[2 * i + 1] = (float)(c[2] * 256 + c[3]) * mul;
-      }
-      if (nt == NT - 1 && more) load_k(next);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] += __shfl_xor_sync(0xffffffffu, s[j], 1);
-      if ((tile + 1) * QC_BLOCK > len) {
-        const int left = len - tile * QC_BLOCK - (16 * (g >> 2) + (g & 3));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) if (32 * (j >> 2) + 4 * (j & 3) >= left) s[j] = -INFINITY;
-      }
-      float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-      const float m_new = fmaxf(m[nt], top);
-      alpha[nt] = qc_ex2(m[nt] - m_new);
-      m[nt] = m_new;
-      uint32_t n[8];
-      float sum = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float w = qc_ex2(s[j] - m_new);
-        sum += w;
-        n[j] = __float2uint_rn(w * QC_ONE);
-      }
-      l[nt] = fmaf(l[nt], alpha[nt], sum);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {   // tokens 32 h ..
-        const uint32_t x01 = __byte_perm(n[4 * h], n[4 * h + 1], 0x5140), x23 = __byte_perm(n[4 * h + 2], n[4 * h + 3], 0x5140);
-        const uint32_t y01 = __byte_perm(n[4 * h], n[4 * h + 1], 0x7362), y23 = __byte_perm(n[4 * h + 2], n[4 * h + 3], 0x7362);
-        const uint32_t d0 = __byte_perm(x01, x23, 0x5410), d1 = __byte_perm(x01, x23, 0x7632);
-        const uint32_t d2 = __byte_perm(y01, y23, 0x5410), d3 = __byte_perm(y01, y23, 0x7632);
-#pragma unroll
-        for (int rr = 0; rr < 2; ++rr) {
-          const int from = (4 * rr + t) * 4;
-          if (ONE) {
-            const uint32_t got = __shfl_sync(0xffffffffu, t & 2 ? (t & 1 ? d2 : d3) : (t & 1 ? d0 : d1), from + (g & 3));
-            pb[nt][2 * h + rr] = g < 4 ? got : 0u;
-          } else {
-            const uint32_t low = __shfl_sync(0xffffffffu, t & 1 ? d0 : d1, from + 2 * (g >> 2) + (g & 1));
-            const uint32_t high = __shfl_sync(0xffffffffu, t & 1 ? d2 : d3, from + 2 * (g >> 2) + (g & 1));
-            pb[nt][2 * h + rr] = g & 2 ? high : low;
-          }
-        }
-      }
-    }
-    // V's bytes, four tokens of one value to a word: a[2 ks + r][value 8 g + i]
-    uint32_t a[4][8];
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t x0 = half ? v[4 * w].y : v[4 * w].x, x1 = half ? v[4 * w + 1].y : v[4 * w + 1].x;
-        const uint32_t x2 = half ? v[4 * w + 2].y : v[4 * w + 2].x, x3 = half ? v[4 * w + 3].y : v[4 * w + 3].x;
-        const uint32_t t0 = __byte_perm(x0, x1, 0x5140), t1 = __byte_perm(x2, x3, 0x5140);
-        const uint32_t t2 = __byte_perm(x0, x1, 0x7362), t3 = __byte_perm(x2, x3, 0x7362);
-        a[w][4 * half] = __byte_perm(t0, t1, 0x5410);
-        a[w][4 * half + 1] = __byte_perm(t0, t1, 0x7632);
-        a[w][4 * half + 2] = __byte_perm(t2, t3, 0x5410);
-        a[w][4 * half + 3] = __byte_perm(t2, t3, 0x7632);
-      }
-    }
-    const float v_now = v_mul * ((t & 1 ? 65536.0f : 1.0f) / QC_ONE);
-    if (more) load_v(next);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        int c[4] = {0, 0, 0, 0};
-        qc_mma_su(c, a[0][2 * i], a[0][2 * i + 1], a[1][2 * i], a[1][2 * i + 1], pb[nt][0], pb[nt][1]);
-        qc_mma_su(c, a[2][2 * i], a[2][2 * i + 1], a[3][2 * i], a[3][2 * i + 1], pb[nt][2], pb[nt][3]);
-        acc[nt][2 * i] = fmaf((float)(c[0] * 256 + c[1]), v_now, acc[nt][2 * i] * alpha[nt]);
-        acc[nt][2 * i + 1] = fmaf((float)(c[2] * 256 + c[3]), v_now, acc[nt][2 * i + 1] * alpha[nt]);
-      }
-    }
+  int taken = 0;
+  for (int i = 0; i < mine; ++i) {
+    if (!qc_tile<NT, ONE>(ring, row.tokens(tile0 + i * stride), g, t, qb, q_mul, m, l, acc, status, fetch,
+                          [&] { return asked - ++taken; })) break;
   }
 
   // the warp's partial results
@@ -383,11 +704,21 @@ __global__ void __launch_bounds__(QC_MAX_WARPS * 32) qcache_attend_kernel(QcAtte
     if (g == 0 && !(t & 1)) { dst[QC_HD] = m[nt]; dst[QC_HD + 1] = l[nt]; }
   }
   __syncthreads();
-  const bool write = !skipped || p.clear_skipped;
+  const bool write = !row.skipped || p.clear_skipped;
   auto store = [&](int h, int c, const QcMerged& x) {
-    if (write) reinterpret_cast<TO*>(p.out)[(int64_t)r * p.ldo + (hk * p.group + h) * QC_HD + c] =
-        from_f<TO>(len > 0 ? x.o / x.l : 0.0f);
+    if (write) reinterpret_cast<TO*>(p.out)[(int64_t)row.r * p.ldo + (row.hk * p.group + h) * QC_HD + c] =
+        from_f<TO>(row.len > 0 ? x.o / x.l : 0.0f);
   };
+  if (parts > 1) {
+    float* dst = p.part + ((int64_t)item * parts + rank) * STEP;
+    for (int i = threadIdx.x; i < p.group * QC_HD; i += blockDim.x) {
+      const int h = i >> 6, c = i & 63;
+      const QcMerged x = qc_merge(warp_part + h * (QC_HD + 2), STEP, warps, c);
+      dst[h * (QC_HD + 2) + c] = x.o;
+      if (c < 2) dst[h * (QC_HD + 2) + QC_HD + c] = c ? x.l : x.m;
+    }
+    return;
+  }
   if (cluster == 1) {
     for (int i = threadIdx.x; i < p.group * QC_HD; i += blockDim.x)
       store(i >> 6, i & 63, qc_merge(warp_part + (i >> 6) * (QC_HD + 2), STEP, warps, i & 63));
@@ -408,6 +739,53 @@ __global__ void __launch_bounds__(QC_MAX_WARPS * 32) qcache_attend_kernel(QcAtte
   if (rank == 0)
     for (int i = threadIdx.x; i < p.group * QC_HD; i += blockDim.x)
       store(i >> 6, i & 63, qc_merge(cta_part + (i >> 6) * (QC_HD + 2), STEP, cluster, i & 63));
+}
+
+// The partial results of a row's parts (qcache_attend_kernel with parts > 1), merged.  Block = 256 threads: a thread per
+// part for the weights, then four groups of 64 that take every fourth part; grid = (row, key head) x its query heads.
+constexpr int QC_MAX_PARTS = 256;
+template <typename TO>
+__global__ void __launch_bounds__(256) qcache_merge_kernel(QcAttendParams p, int parts, int step) {
+  __shared__ float weight[QC_MAX_PARTS], top[8], total[8], sums[4][QC_HD];
+  pdl_trigger();
+  const uint32_t item = blockIdx.x / (uint32_t)p.group;
+  const int h = blockIdx.x % (uint32_t)p.group, tid = threadIdx.x, sub = tid >> 6, c = tid & 63;
+  const int r = (int)(item / (uint32_t)p.c.n_heads), hk = (int)(item - (uint32_t)r * p.c.n_heads);
+  pdl_wait();
+  const int slot = p.slots[r];
+  if ((slot < 0 || slot >= p.c.n_slots) && !p.clear_skipped) return;
+  const float* part = p.part + (int64_t)item * parts * step + h * (QC_HD + 2);
+  float m = -INFINITY, l = 0.0f;
+  if (tid < parts) { m = part[tid * step + QC_HD]; l = part[tid * step + QC_HD + 1]; }
+  float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  float t = warp_max(m);
+  if ((tid & 31) == 0) top[tid >> 5] = t;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t = fmaxf(t, top[i]);
+  const float w = l == 0.0f ? 0.0f : qc_ex2(m - t);   // l = 0: no tokens; NaN goes through
+  weight[tid] = w;
+  const float s = warp_sum(l * w);
+  if ((tid & 31) == 0) total[tid >> 5] = s;
+  __syncthreads();
+  int i = sub;
+  for (; i + 28 < parts; i += 32) {   // eight parts' loads at a time
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = part[(i + 4 * j) * step + c];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j & 3] = fmaf(x[j], weight[i + 4 * j], o[j & 3]);
+  }
+  for (; i < parts; i += 4) o[0] = fmaf(part[i * step + c], weight[i], o[0]);
+  sums[sub][c] = (o[0] + o[1]) + (o[2] + o[3]);
+  __syncthreads();
+  if (sub) return;
+  float all = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) all += total[j];
+  const float v = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+  // no tokens at all: the sum is 0
+  reinterpret_cast<TO*>(p.out)[(int64_t)r * p.ldo + (hk * p.group + h) * QC_HD + c] = from_f<TO>(all == 0.0f ? 0.0f : v / all);
 }
 
 }  // namespace wdz

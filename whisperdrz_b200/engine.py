@@ -436,30 +436,34 @@ class Engine:
         return QCache.empty(n_slots or self.n_slots, n_tokens or self.dims.n_audio_ctx, n_heads or self.dims.n_text_head,
                             self.device)
 
+    # The calls below take a few microseconds on the device, so their checks are written to cost little on the host.
+    def _raw_stream(self) -> int:
+        """The current stream's handle, without the object around it."""
+        return torch._C._cuda_getCurrentRawStream(self._ordinal)
+
+    def _here(self, name: str, ordinal: int) -> None:
+        if ordinal != self._ordinal:
+            raise ValueError(f"{name} does not lie on the engine's device")
+
     def _rows(self, name: str, t: torch.Tensor, width: int) -> torch.Tensor:
         """``t`` as rows [n, width] in a type and at places that the kernels take: no copy where it has them already."""
-        if t.dtype not in _TORCH_DTYPE:
-            raise ValueError(f"{name} must be float32 or bfloat16, got {t.dtype}")
         if t.dim() == 3:
             t = t.flatten(1)
-        if t.dim() != 2 or t.shape[1] != width:
-            raise ValueError(f"{name} must be [rows, {width}], got {tuple(t.shape)}")
-        self._on_device(name, t.device)
-        if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width) or t.stride(0) * t.element_size() % 16 or t.data_ptr() % 16:
+        if t.dtype not in _TORCH_DTYPE or t.dim() != 2 or t.shape[1] != width:
+            raise ValueError(f"{name} must be [rows, {width}] in float32 or bfloat16, got {t.dtype} {tuple(t.shape)}")
+        self._here(name, t.get_device())
+        step, one = t.stride()
+        if one != 1 or (step < width and t.shape[0] > 1) or step * t.element_size() % 16 or t.data_ptr() % 16:
             t = t.clone(memory_format=torch.contiguous_format)
         return t
 
     def _index(self, name: str, x, n: int) -> torch.Tensor:
         """An int32 index tensor of ``n`` entries on the device; host sequences are uploaded."""
-        t = x if isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.is_cuda and x.is_contiguous() else self._i32(x)
-        self._on_device(name, t.device)
-        if t.dim() != 1 or t.shape[0] != n:
-            raise ValueError(f"{name} must have {n} entries, got {tuple(t.shape)}")
-        return t
-
-    def _on_device(self, name: str, device) -> None:
-        if device != self.device and (device.type, device.index) != (self.device.type, self._ordinal):
-            raise ValueError(f"{name} lies on {device}, the engine on {self.device}")
+        if not isinstance(x, torch.Tensor) or x.dtype != torch.int32 or x.get_device() != self._ordinal or not x.is_contiguous():
+            x = self._i32(x)
+        if x.dim() != 1 or x.shape[0] != n:
+            raise ValueError(f"{name} must have {n} entries, got {tuple(x.shape)}")
+        return x
 
     def qcache_store(self, cache: QCache, k: torch.Tensor, v: torch.Tensor, slots, positions, row_begin=None,
                      max_run: int | None = None) -> None:
@@ -474,7 +478,7 @@ class Engine:
         rows).  Non-finite values, places outside the cache and slots named twice are told by ``device_status()``;
         slots outside the cache are skipped."""
         width = cache.n_heads * HEAD_DIM
-        self._on_device("the cache", cache.device)
+        self._here("the cache", cache.ordinal)
         k, v = self._rows("k", k, width), self._rows("v", v, width)
         if k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError("k and v must have the same shape and type")
@@ -495,15 +499,17 @@ class Engine:
             rb = self._index("row_begin", row_begin, n_runs + 1)
             most = n if max_run is None else int(max_run)
         if not isinstance(slots, torch.Tensor):
-            named = [int(x) for x in slots]
-            if len(set(named)) != len(named):
+            slots = [int(x) for x in slots]
+            if len(set(slots)) != len(slots):
                 raise ValueError("qcache_store: a slot is named twice")
+        sl, ps = self._index("slots", slots, n_runs), self._index("positions", positions, n_runs)
         if n == 0 or n_runs == 0:
             return
-        sl, ps = self._index("slots", slots, n_runs), self._index("positions", positions, n_runs)
-        self._check(self.lib.wdz_qcache_store(
+        rc = self.lib.wdz_qcache_store(
             self.h, cache.ref, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), _TORCH_DTYPE[k.dtype], n,
-            None if rb is None else rb.data_ptr(), sl.data_ptr(), ps.data_ptr(), n_runs, most, self._stream()))
+            None if rb is None else rb.data_ptr(), sl.data_ptr(), ps.data_ptr(), n_runs, most, self._raw_stream())
+        if rc:
+            self._check(rc)
 
     def qcache_attention(self, q: torch.Tensor, cache: QCache, slots, lens, scale: float = HEAD_DIM ** -0.5,
                          out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -514,55 +520,66 @@ class Engine:
         to 8, consecutive query heads sharing a key head.  Returns [n, q_heads * 64] in ``out_dtype`` (default: the
         engine's type), or fills ``out``.  Length 0 gives zeros; a row whose slot lies outside the cache is left as it
         was (zeros when ``out`` is not given)."""
-        self._on_device("the cache", cache.device)
         width = q.shape[1] if q.dim() == 2 else q.shape[1:].numel()
-        if width == 0 or width % (cache.n_heads * HEAD_DIM) or width // (cache.n_heads * HEAD_DIM) > 8:
+        shared, rest = divmod(width, cache.n_heads * HEAD_DIM)
+        if rest or not 1 <= shared <= 8:
             raise ValueError(f"q must have 1 to 8 times the cache's {cache.n_heads} heads of {HEAD_DIM}, got {tuple(q.shape)}")
+        self._here("the cache", cache.ordinal)
         q = self._rows("q", q, width)
         n = q.shape[0]
-        if out_dtype is not None and out_dtype not in _TORCH_DTYPE:
-            raise ValueError("out_dtype must be float32 or bfloat16")
-        clear = out is None
-        if clear:
-            out = torch.empty(n, width, dtype=out_dtype or self.dtype, device=self.device)
-        elif (out.dtype not in _TORCH_DTYPE or out_dtype not in (None, out.dtype) or tuple(out.shape) != (n, width)
-              or out.stride(1) != 1 or (n > 1 and out.stride(0) < width)
-              or out.stride(0) * out.element_size() % 16 or out.data_ptr() % 16):
-            raise ValueError(f"out must be [{n}, {width}] rows in float32 or bfloat16 that start on 16 bytes")
-        self._on_device("out", out.device)
+        if out is None:
+            to = out_dtype or self.dtype
+            if to not in _TORCH_DTYPE:
+                raise ValueError("out_dtype must be float32 or bfloat16")
+            given, out = False, q.new_empty((n, width), dtype=to)
+        else:
+            given, to = True, out.dtype
+            if (to not in _TORCH_DTYPE or out_dtype not in (None, to) or tuple(out.shape) != (n, width) or out.stride(1) != 1
+                    or (n > 1 and out.stride(0) < width) or out.stride(0) * out.element_size() % 16 or out.data_ptr() % 16):
+                raise ValueError(f"out must be [{n}, {width}] rows in float32 or bfloat16 that start on 16 bytes")
+            self._here("out", out.get_device())
+        sl, ln = self._index("slots", slots, n), self._index("lens", lens, n)
         if n == 0:
             return out
-        sl, ln = self._index("slots", slots, n), self._index("lens", lens, n)
-        self._check(self.lib.wdz_qcache_attention(
+        need = cache.scratch.get((n, shared))
+        if need is None:
+            need = self.lib.wdz_qcache_attention_scratch(self.h, cache.ref, width // HEAD_DIM, n)
+            cache.scratch[(n, shared)] = need
+        scratch = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
+        rc = self.lib.wdz_qcache_attention(
             self.h, cache.ref, q.data_ptr(), q.stride(0), _TORCH_DTYPE[q.dtype], width // HEAD_DIM, sl.data_ptr(),
-            ln.data_ptr(), n, scale, out.data_ptr(), out.stride(0), _TORCH_DTYPE[out.dtype], int(clear),
-            self._stream()))
+            ln.data_ptr(), n, scale, out.data_ptr(), out.stride(0), _TORCH_DTYPE[to], not given,
+            None if scratch is None else scratch.data_ptr(), need if need > 0 else 0, self._raw_stream())
+        if rc:
+            self._check(rc)
         return out
 
     def linear_rows_packed(self, x: torch.Tensor, w: PackedLinear, residual: torch.Tensor | None = None,
                            out: torch.Tensor | None = None) -> torch.Tensor:
         """``linear_rows`` with 4-bit weights (``lowbit.pack_linear``): x f32 or bf16 [M, K] @ W[N, K].T (+ bias)
         (+ residual f32 [M, N]) -> f32 [M, N].  ``residual`` and ``out`` may be the same tensor."""
-        self._on_device("the weights", w.device)
+        self._here("the weights", w.ordinal)
         if x.dtype not in _TORCH_DTYPE or x.dim() != 2 or x.shape[1] != w.in_features:
             raise ValueError(f"x must be [rows, {w.in_features}] in float32 or bfloat16, got {x.dtype} {tuple(x.shape)}")
-        self._on_device("x", x.device)
+        self._here("x", x.get_device())
         if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
             x = x.contiguous()
         M, N = x.shape[0], w.out_features
         for name, t in (("residual", residual), ("out", out)):
-            if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (M, N) or not t.is_contiguous()):
-                raise ValueError(f"{name} must be a contiguous float32 [{M}, {N}]")
             if t is not None:
-                self._on_device(name, t.device)
-        y = out if out is not None else torch.empty(M, N, dtype=torch.float32, device=self.device)
+                if t.dtype != torch.float32 or tuple(t.shape) != (M, N) or not t.is_contiguous():
+                    raise ValueError(f"{name} must be a contiguous float32 [{M}, {N}]")
+                self._here(name, t.get_device())
+        y = out if out is not None else x.new_empty((M, N), dtype=torch.float32)
         b = w.bias
         if b is not None and b.dtype != x.dtype:
             b = b.to(x.dtype)
-        self._check(self.lib.wdz_linear_rows_packed(
+        rc = self.lib.wdz_linear_rows_packed(
             self.h, x.data_ptr(), x.stride(0), _TORCH_DTYPE[x.dtype], M, w.in_features, w.weight.data_ptr(),
             w.scale.data_ptr(), w.group, None if b is None else b.data_ptr(),
-            None if residual is None else residual.data_ptr(), N, y.data_ptr(), self._stream()))
+            None if residual is None else residual.data_ptr(), N, y.data_ptr(), self._raw_stream())
+        if rc:
+            self._check(rc)
         return y
 
     # ------------------------------------------------------- word-timing alignment

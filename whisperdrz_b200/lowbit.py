@@ -45,10 +45,11 @@ class QCache:
         if step % 16 or k.data_ptr() % 16 or v.data_ptr() % 16:
             raise ValueError("QCache: values must start on 16 bytes")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.n_slots, self.n_heads, self.n_tokens, self.device = n_slots, n_heads, n_tokens, k.device
+        self.n_slots, self.n_heads, self.n_tokens, self.device, self.ordinal = n_slots, n_heads, n_tokens, k.device, k.get_device()
         self.desc = capi.QCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), step, scale_step,
                                     n_slots, n_heads, n_tokens // BLOCK)
         self.ref = C.byref(self.desc)
+        self.scratch: dict = {}   # bytes of scratch by call shape, as the library told them
 
     @classmethod
     def empty(cls, n_slots: int, n_tokens: int, n_heads: int, device) -> "QCache":
@@ -79,7 +80,7 @@ class PackedLinear:
         if not weight.is_contiguous() or not scale.is_contiguous() or weight.data_ptr() % 16 or scale.data_ptr() % 8:
             raise ValueError("PackedLinear: contiguous tensors, the weights on 16 bytes and the scales on 8")
         self.weight, self.scale, self.in_features, self.group = weight, scale, int(in_features), int(group)
-        self.out_features, self.device = weight.shape[0], weight.device
+        self.out_features, self.device, self.ordinal = weight.shape[0], weight.device, weight.get_device()
         self.bias = None if bias is None else bias.contiguous()
 
 
