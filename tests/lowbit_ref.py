@@ -2,7 +2,7 @@
 import numpy as np
 
 BLOCK, HEAD = 64, 64
-TINY = 2.0 ** -119
+TINY = 2.0 ** -117
 
 
 def dequant(values, scale):

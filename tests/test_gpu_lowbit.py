@@ -119,7 +119,7 @@ def test_store_extreme_values(eng, dtype, start):
     rows[:] = torch.randn(70, 128, generator=g)
     rows[5], rows[6, ::2], rows[7, ::3] = 0.0, 127.0, 63.5
     rows[64:, :64] = 0.0                 # a block of zeros in head 0
-    rows[64:, 64:] *= 1e-38              # and of numbers below 2^-119 in head 1
+    rows[64:, 64:] *= 1e-38              # and of numbers below 2^-117 in head 1
     k, v = rows.to(dtype), (rows * 2.5e36).to(dtype)
     parts = _filled(1, 2, 2)
     _check_store(eng, parts, k, v, [0], [start], [0, 70])

@@ -162,30 +162,39 @@ def test_abi_refuses_bad_arguments_before_it_looks_at_the_engine(lib, handle):
 
 # --------------------------------------------------- the store's arithmetic
 def test_store_rounding_as_the_kernel_computes_it():
-    """rint(x / s) from a rounded product and one exact remainder, in float32, against fractions: at every half step, one
-    float to either side of it, and at random places, for scales of every mantissa size."""
+    """rint(x / s) from the products with the floats above and below 1 / s, and the sign of x - h s where they differ, in
+    float32, against fractions: at every half step, one float to either side of it, and at random places, for scales of
+    every mantissa size and rows in bf16."""
     rng = np.random.default_rng(0)
     f = np.float32
-    for trial in range(400):
-        top = f(rng.uniform(1, 2) * 2.0 ** int(rng.integers(-100, 100)))
-        if trial % 4 == 0:
+    magic = 12582912.0
+    differed = 0
+    for trial in range(80):
+        top = f(rng.uniform(1, 2) * 2.0 ** int(rng.integers(-116, 100)))
+        if trial % 2:
             top = torch.tensor(top).bfloat16().float().numpy()[()]
         s = f(top / f(127))
         inv = f(1) / s
         half_steps = (np.arange(-127, 127) + 0.5).astype(np.float64) * np.float64(s)
         x = half_steps.astype(f)
-        x = np.concatenate([x, np.nextafter(x, f(np.inf)), np.nextafter(x, f(-np.inf)), (rng.uniform(-1, 1, 64) * top).astype(f)])
+        x = np.concatenate([x, np.nextafter(x, f(np.inf)), np.nextafter(x, f(-np.inf)), (rng.uniform(-1, 1, 64) * top).astype(f), [top]])
+        if trial % 4 == 1:
+            x = torch.tensor(x).bfloat16().float().numpy()
         x = x[np.abs(x) <= top]
-        q = np.rint(np.clip((x * inv).astype(f), f(-127), f(127)))
-        # the fused multiply-add: q s has at most 31 bits, so the difference in 64 bits is exact and is rounded once
-        d = (x.astype(np.float64) - q.astype(np.float64) * np.float64(s)).astype(f)
-        half, odd = f(0.5) * s, q.astype(np.int64) % 2 == 1
-        up = (d > half) | ((d == half) & odd)
-        down = (d < -half) | ((d == -half) & odd)
-        q = np.clip(q + up - down, -127, 127)
-        fs = Fraction(float(s))
-        want = np.array([round(Fraction(float(v)) / fs) for v in x])   # half to even
-        assert (q == np.clip(want, -127, 127)).all()
+
+        def whole(m):   # a fused multiply-add with 1.5 2^23: the product has 48 bits, so 64 bits hold the sum before it is rounded
+            return (x.astype(np.float64) * np.float64(m) + magic).astype(f).astype(np.float64) - magic
+
+        a, b = whole(np.nextafter(inv, f(np.inf))), whole(np.nextafter(inv, f(0)))
+        half = 0.5 * (a + b)
+        sign = np.array([(Fraction(float(v)) > Fraction(float(h)) * Fraction(float(s))) - (Fraction(float(v)) < Fraction(float(h)) * Fraction(float(s)))
+                         for v, h in zip(x, half)])
+        even = np.where(a % 2 == 0, a, b)
+        q = np.where(a == b, a, np.where(sign > 0, np.maximum(a, b), np.where(sign < 0, np.minimum(a, b), even)))
+        differed += int((a != b).sum())
+        want = np.array([round(Fraction(float(v)) / Fraction(float(s))) for v in x])   # half to even
+        assert (q == want).all() and np.abs(q).max() <= 127
+    assert differed > 200
 
 
 def test_reference_store_continues_a_block():

@@ -15,7 +15,7 @@ namespace wdz {
 
 constexpr int QC_BLOCK = WDZ_QCACHE_BLOCK;   // tokens that share a scale
 constexpr int QC_HD = 64;
-constexpr float QC_TINY = 1.5046328e-36f;    // 2^-119: below it x / 127 would leave the normal range; such a block is zero
+constexpr float QC_TINY = 6.0185310762e-36f;   // 2^-117: below it the store's remainders would underflow; such a block is zero
 
 struct QcView {
   int8_t *k, *v;
@@ -34,13 +34,15 @@ struct QcStoreParams {
 
 // ---- store ---------------------------------------------------------------------------------------------------------
 // Bound by the rows' bytes (2 or 4 a value) and the cache's (1).  rint(x / s) has to be exact, a value next to a half step
-// included, at a few instructions a value: x (1 / s) is rounded to a whole number q by one fused multiply-add with
-// 1.5 2^23; 1 / s is off by 2^-24, so q is at most one off and only near a half step.  The remainder d = x - q s has so few
-// bits that one more fused multiply-add gives it without rounding wherever it decides (q s is a multiple of s's last bit,
-// x of s's last bit / 2 or less, and |d| <= s / 2 needs 24 of those); |d| < s / 2 everywhere proves q right, and where a
-// lane sees anything else (ties, NaN) its values are settled one by one by qc_code.
+// included, at a few instructions a value: x is multiplied by the two floats next to 1 / s, above and below, and each product
+// is rounded to a whole number by the same fused multiply-add with 1.5 2^23.  x / s lies strictly between the products and
+// rounding is monotonic, so where the two agree that is the result.  Where they differ (near a half step: 1 value in 1000 of
+// bf16 rows, whose quotients by a bf16 maximum often are nearly halves) the sign of x - h s, h the half between them, tells:
+// h s has at most 32 bits and a fused multiply-add rounds only the difference, which keeps its sign.
 
-// rint(x / s), half to even, settled by the remainder.
+// rint(x / s), half to even, for values that need not be finite, settled by the remainder x - q s: it has so few bits that a
+// fused multiply-add gives it without rounding wherever it decides (q s is a multiple of s's last bit, x of s's last bit / 2
+// or less, and |x - q s| <= s / 2 needs 24 of those).
 __device__ __forceinline__ int qc_code(float x, float s, float inv) {
   const float lim = fminf(fmaxf(x * inv, -127.0f), 127.0f);   // infinities saturate; NaN becomes a bound and is set aside below
   float q = rintf(lim);
@@ -49,27 +51,50 @@ __device__ __forceinline__ int qc_code(float x, float s, float inv) {
   if (d > half || (d == half && odd)) q += 1.0f;
   if (d < -half || (d == -half && odd)) q -= 1.0f;
   q = fminf(fmaxf(q, -127.0f), 127.0f);
-  return x == x ? (int)q : 0;
+  return x == x && s > 0.0f ? (int)q : 0;
 }
 
-// Eight values -> eight bytes.
-__device__ __forceinline__ uint2 qc_code8(const float (&x)[8], float s, float inv) {
-  constexpr float MAGIC = 12582912.0f;   // 1.5 2^23
-  uint32_t n[8];
-  float worst = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float t = fmaf(x[i], inv, MAGIC);
-    n[i] = __float_as_uint(t);
-    worst = fmaxf(worst, fabsf(fmaf(MAGIC - t, s, x[i])));
+// What a block's values are divided by: the scale, 1 / scale rounded, and the floats next to that.  Scale 0 makes zeros.
+struct QcDivisor {
+  float s, inv, above, below;
+  __device__ explicit QcDivisor(float scale) : s(scale) {
+    inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+    above = scale > 0.0f ? __uint_as_float(__float_as_uint(inv) + 1) : 0.0f;
+    below = scale > 0.0f ? __uint_as_float(__float_as_uint(inv) - 1) : 0.0f;
   }
-  if (!(worst < 0.5f * s)) {   // a NaN is lost in the maximum: rows that hold one come here with s negated
-#pragma unroll
-    for (int i = 0; i < 8; ++i) n[i] = (uint32_t)qc_code(x[i], fabsf(s), inv);
-  }
+};
+
+__device__ __forceinline__ uint2 qc_bytes(const uint32_t (&n)[8]) {
   const uint32_t a = __byte_perm(n[0], n[1], 0x0040), b = __byte_perm(n[2], n[3], 0x0040);
   const uint32_t c = __byte_perm(n[4], n[5], 0x0040), d = __byte_perm(n[6], n[7], 0x0040);
   return make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410));
+}
+// Eight finite values -> eight bytes.
+__device__ __forceinline__ uint2 qc_code8(const float (&x)[8], const QcDivisor& by) {
+  constexpr float MAGIC = 12582912.0f;   // 1.5 2^23: the sums' bits are its bits plus the whole number
+  uint32_t n[8], other[8], differ = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    n[i] = __float_as_uint(fmaf(x[i], by.above, MAGIC));
+    other[i] = __float_as_uint(fmaf(x[i], by.below, MAGIC));
+    differ |= n[i] ^ other[i];
+  }
+  if (differ) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float half = 0.5f * ((__uint_as_float(n[i]) - MAGIC) + (__uint_as_float(other[i]) - MAGIC));
+      const float d = fmaf(-half, by.s, x[i]);
+      const uint32_t even = n[i] & 1 ? other[i] : n[i];
+      n[i] = d > 0.0f ? max(n[i], other[i]) : d < 0.0f ? min(n[i], other[i]) : even;
+    }
+  }
+  return qc_bytes(n);
+}
+__device__ __forceinline__ uint2 qc_settle8(const float (&x)[8], const QcDivisor& by) {
+  uint32_t n[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) n[i] = (uint32_t)qc_code(x[i], by.s, by.inv);
+  return qc_bytes(n);
 }
 
 // rint(q s_old / s_new), half to even, of eight bytes.  The rounded quotient is at most one off; both products are exact
@@ -100,49 +125,57 @@ __device__ __forceinline__ void qc_report(DevStatus* st, int code, int detail) {
   if (atomicCAS(&st->code, 0, code) == 0) st->detail = detail;
 }
 
+// The larger of two magnitudes, NaN if one is.
+__device__ __forceinline__ float qc_max(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+// Magnitudes in their bits' order: numbers, infinity, NaN.
+__device__ __forceinline__ uint32_t qc_bits(float magnitude) { return __float_as_uint(magnitude) & 0x7fffffffu; }
+
 // Eight neighbouring values of a row, as they lie.
 template <typename T> struct QcRaw;
 template <> struct QcRaw<bf16> {
-  uint4 v;
+  uint4 v = make_uint4(0, 0, 0, 0);
+  __device__ QcRaw() {}
+  __device__ explicit QcRaw(const uint8_t* staged) : v(*reinterpret_cast<const uint4*>(staged)) {}   // as the store kernel lays it
   __device__ void load(const void* p) { v = *reinterpret_cast<const uint4*>(p); }
-  __device__ void clear() { v = make_uint4(0, 0, 0, 0); }
   __device__ void get(float (&x)[8]) const {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
   }
-  // the largest magnitude's bits as fp32's, infinities and NaN above all numbers
-  __device__ uint32_t top() const {
-    const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
-    return max(m << 16, m & 0xffff0000u);
+  // the largest magnitude so far and these; NaN stays
+  __device__ float top(float m) const {
+    __nv_bfloat162 x[4];
+    memcpy(x, &v, 16);
+    const __nv_bfloat162 y = __hmax2_nan(__hmax2_nan(__habs2(x[0]), __habs2(x[1])), __hmax2_nan(__habs2(x[2]), __habs2(x[3])));
+    return qc_max(m, __bfloat162float(__hmax_nan(__low2bfloat16(y), __high2bfloat16(y))));
   }
 };
 template <> struct QcRaw<float> {
-  float4 a, b;
+  float4 a = make_float4(0, 0, 0, 0), b = a;
+  __device__ QcRaw() {}
+  __device__ explicit QcRaw(const uint8_t* staged) : a(*reinterpret_cast<const float4*>(staged)), b(*reinterpret_cast<const float4*>(staged + 512)) {}
   __device__ void load(const void* p) { a = reinterpret_cast<const float4*>(p)[0]; b = reinterpret_cast<const float4*>(p)[1]; }
-  __device__ void clear() { a = b = make_float4(0, 0, 0, 0); }
   __device__ void get(float (&x)[8]) const {
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
   }
-  __device__ uint32_t top() const {
+  __device__ float top(float m) const {
     float x[8];
     get(x);
-    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    for (int i = 0; i < 8; ++i) m = qc_max(m, fabsf(x[i]));
     return m;
   }
 };
 template <typename T>
-__device__ __forceinline__ uint32_t qc_finite_top(const QcRaw<T>& r) {   // the same without infinities and NaN
+__device__ __forceinline__ float qc_finite_top(const QcRaw<T>& r, float m) {   // the same without infinities and NaN
   float x[8];
   r.get(x);
-  uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
-    if (u < 0x7f800000u) m = max(m, u);
-  }
+  for (int i = 0; i < 8; ++i) m = fabsf(x[i]) <= 3.402823466e38f ? fmaxf(m, fabsf(x[i])) : m;
   return m;
 }
 
@@ -182,83 +215,97 @@ __device__ __forceinline__ float qc_scale(uint32_t top_bits) {
   return top >= QC_TINY ? __fdiv_rn(top, 127.0f) : 0.0f;
 }
 
-// Runs of any length.  A unit is a block of 64 tokens of one head, K or V: SHARE warps hold it in registers between the
-// maximum and the rounding, so the rows are read once; a lane has 8 neighbouring values of a token, four tokens at a time.
-// Block = 4 warps; grid = (blocks of the longest run, groups of 4 / SHARE units of heads and K / V, run).
+// Runs of any length.  A unit is a block of 64 tokens of one head, K or V, and belongs to one warp, which keeps it in shared
+// memory between the maximum and the rounding, so the rows are read once.  A lane has 8 neighbouring values of a token, four
+// tokens at a time, and reads back only what it brought itself (asynchronous copies): no barrier, and few registers, so that
+// the many warps of an SM hide one another's copies.  With few units (SHARE = 4) four warps take a unit's tokens in turn and
+// exchange the maximum: then the time is one unit's way through, not the SMs' rate.
+// Block = 2 units of a warp, or 1 of four; grid = (blocks of the longest run, groups of units, run).
+template <typename T> constexpr int QC_UNIT = QC_BLOCK * QC_HD * (int)sizeof(T);   // bytes of a unit's rows
+
 template <typename T, int SHARE>
-__global__ void __launch_bounds__(128) qcache_store_kernel(QcStoreParams p, DevStatus* status) {
-  constexpr int TOKENS = QC_BLOCK / SHARE, STEPS = TOKENS / 4;
-  __shared__ uint32_t tops[4];
+__global__ void __launch_bounds__((SHARE == 1 ? 2 : SHARE) * 32) qcache_store_kernel(QcStoreParams p, DevStatus* status) {
+  constexpr int PIECE = 8 * sizeof(T), STEP = 32 * PIECE;   // bytes of a lane's piece, of all lanes'
+  extern __shared__ __align__(16) uint8_t qc_rows[];
+  __shared__ uint32_t tops[2][4];
   pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % SHARE;
-  const int unit = blockIdx.y * (4 / SHARE) + warp / SHARE;
-  const bool has = unit < 2 * p.c.n_heads;
-  const bool is_v = has && unit >= p.c.n_heads;
-  const int head = has ? (is_v ? unit - p.c.n_heads : unit) : 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = SHARE > 1 ? warp : 0;
+  const int unit = SHARE > 1 ? blockIdx.y : blockIdx.y * 2 + warp;
+  uint8_t* mine = qc_rows + (SHARE > 1 ? 0 : warp) * QC_UNIT<T> + lane * 16;   // 16 bytes of each lane side by side
   pdl_wait();
   const QcRun run(p, blockIdx.z, blockIdx.x == 0 && blockIdx.y == 0, status);
-  if (!run.ok) return;
+  if (!run.ok || unit >= 2 * p.c.n_heads) return;
+  const bool is_v = unit >= p.c.n_heads;
+  const int head = is_v ? unit - p.c.n_heads : unit;
   const QcPlace place(p.c, run.slot, head, is_v);
   const int64_t ld = (is_v ? p.ldv : p.ldk) * (int64_t)sizeof(T);
-  const char* src = reinterpret_cast<const char*>(is_v ? p.v : p.k) + (int64_t)(head * QC_HD + 8 * (lane & 7)) * sizeof(T);
+  const char* src = reinterpret_cast<const char*>(is_v ? p.v : p.k) + (int64_t)head * (QC_HD * sizeof(T)) + PIECE * (lane & 7);
+  auto over_unit = [&](float top, int round) {
+    uint32_t bits = __reduce_max_sync(0xffffffffu, qc_bits(top));
+    if (SHARE > 1) {   // the CTA is the unit; each round has words of its own, so one barrier is enough
+      if (lane == 0) tops[round][warp] = bits;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < SHARE; ++i) bits = max(bits, tops[round][i]);
+    }
+    return bits;
+  };
   for (int b = run.p0 / QC_BLOCK + blockIdx.x; b * QC_BLOCK < run.p1; b += gridDim.x) {
-    const int lo = max(run.p0, b * QC_BLOCK), hi = min(run.p1, (b + 1) * QC_BLOCK);
-    const int t0 = b * QC_BLOCK + part * TOKENS + (lane >> 3);   // this lane's tokens: t0, t0 + 4, ..
-    QcRaw<T> raw[STEPS];
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-      const int t = t0 + 4 * i;
-      raw[i].clear();
-      if (has && t >= lo && t < hi) raw[i].load(src + (int64_t)(run.r0 + t - run.p0) * ld);
+    const int lo = max(run.p0, b * QC_BLOCK), hi = min(run.p1, (b + 1) * QC_BLOCK), t0 = b * QC_BLOCK + (lane >> 3);
+    const int i0 = (lo - b * QC_BLOCK) >> 2, i1 = (hi - b * QC_BLOCK + 3) >> 2;   // steps of four tokens that the run reaches
+    const int is = i0 + part;   // this warp's: is, is + SHARE, ..
+    const char* from = src + (int64_t)(run.r0 + t0 + 4 * is - run.p0) * ld;   // followed only where the token is the run's
+    const uint32_t to_smem = att_smem_u32(mine);
+#pragma unroll 4
+    for (int i = is; i < i1; i += SHARE, from += 4 * SHARE * ld) {
+      const uint32_t bytes = t0 + 4 * i >= lo && t0 + 4 * i < hi ? 16 : 0;   // 0: zeros
+      const char* at = bytes ? from : src;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to_smem + i * STEP), "l"(at), "r"(bytes) : "memory");
+      if (PIECE == 32)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to_smem + i * STEP + 512), "l"(at + 16), "r"(bytes) : "memory");
     }
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i) top = max(top, raw[i].top());
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (SHARE > 1) {
-      __syncthreads();
-      if (lane == 0) tops[warp] = top;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < SHARE; ++i) top = max(top, tops[warp - part + i]);
-    }
-    const bool odd = top >= 0x7f800000u;
-    if (odd) {   // an infinity or a NaN: the scale goes by the rest
-      top = 0;
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) top = max(top, qc_finite_top(raw[i]));
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) qc_report(status, WDZ_ENAN, 2000000 + (int)blockIdx.z);
-    }
-    if (SHARE > 1) {
-      if (__syncthreads_or(odd)) {
-        if (lane == 0) tops[warp] = top;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < SHARE; ++i) top = max(top, tops[warp - part + i]);
-      }
-    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
     const bool entered = lo > b * QC_BLOCK;   // behind the block's first token: what it holds stays
-    const float old = has && entered ? place.s[b] : 0.0f, now = fmaxf(old, qc_scale(top));
-    if (has) {
-      if (now > old && entered)
-        for (int t = b * QC_BLOCK + part * 4 + (lane >> 3); t < lo; t += 4 * SHARE) {
-          uint2* at = reinterpret_cast<uint2*>(place.q + (int64_t)t * QC_HD + 8 * (lane & 7));
-          *at = qc_recode8(*at, old, now);
-        }
-      const float inv = now > 0.0f ? __fdiv_rn(1.0f, now) : 0.0f, sign = odd ? -now : now;
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int t = t0 + 4 * i;
-        if (t >= lo && t < hi) {
-          float x[8];
-          raw[i].get(x);
-          *reinterpret_cast<uint2*>(place.q + (int64_t)t * QC_HD + 8 * (lane & 7)) = now > 0.0f ? qc_code8(x, sign, inv) : make_uint2(0, 0);
-        }
+    const float old = entered ? place.s[b] : 0.0f;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    float top = 0.0f;
+#pragma unroll 8
+    for (int i = is; i < i1; i += SHARE) top = QcRaw<T>(mine + i * STEP).top(top);
+    uint32_t bits = over_unit(top, 0);
+    const bool odd = bits >= 0x7f800000u;
+    if (odd) {   // an infinity or a NaN: the scale goes by the rest
+      top = 0.0f;
+#pragma unroll 1
+      for (int i = is; i < i1; i += SHARE) top = qc_finite_top(QcRaw<T>(mine + i * STEP), top);
+      bits = over_unit(top, 1);
+      if (part == 0 && lane == 0) qc_report(status, WDZ_ENAN, 2000000 + (int)blockIdx.z);
+    }
+    const float now = fmaxf(old, qc_scale(bits));
+    if (part == 0 && lane == 0) place.s[b] = now;   // every lane has read the old one
+    int8_t* to = place.q + (int64_t)(b * QC_BLOCK + (lane >> 3)) * QC_HD + 8 * (lane & 7);
+    if (now > old && entered)
+      for (int t = b * QC_BLOCK + (lane >> 3) + 4 * part; t < lo; t += 4 * SHARE) {
+        uint2* at = reinterpret_cast<uint2*>(place.q + (int64_t)t * QC_HD + 8 * (lane & 7));
+        *at = qc_recode8(*at, old, now);
+      }
+    const QcDivisor by(now);
+    if (odd) {
+#pragma unroll 1
+      for (int i = is; i < i1; i += SHARE) {
+        float x[8];
+        QcRaw<T>(mine + i * STEP).get(x);
+        if (t0 + 4 * i >= lo && t0 + 4 * i < hi) *reinterpret_cast<uint2*>(to + 4 * i * QC_HD) = qc_settle8(x, by);
+      }
+    } else {
+#pragma unroll 4
+      for (int i = is; i < i1; i += SHARE) {
+        float x[8];
+        QcRaw<T>(mine + i * STEP).get(x);
+        const uint2 w = qc_code8(x, by);
+        if (t0 + 4 * i >= lo && t0 + 4 * i < hi) *reinterpret_cast<uint2*>(to + 4 * i * QC_HD) = w;
       }
     }
-    if (SHARE > 1) __syncthreads(); else __syncwarp();   // every part has read the old scale
-    if (has && part == 0 && lane == 0) place.s[b] = now;
+    if (SHARE > 1) __syncthreads();   // before the next block writes its words
   }
 }
 
@@ -283,13 +330,12 @@ __global__ void __launch_bounds__(320) qcache_step_kernel(QcStoreParams p, DevSt
     __syncthreads();
     if (threadIdx.x == 0) n_grown = 0;
     QcRaw<T> raw;
-    raw.clear();
     float old = 0.0f;
     if (has) {
       raw.load(reinterpret_cast<const T*>(is_v ? p.v : p.k) + (int64_t)run.r0 * (is_v ? p.ldv : p.ldk) + head * QC_HD + 8 * c);
       if (kept) old = place.s[b];
     }
-    uint32_t top = raw.top();
+    uint32_t top = qc_bits(raw.top(0.0f));
     auto over8 = [&] {
 #pragma unroll
       for (int i = 4; i > 0; i >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, i));
@@ -297,7 +343,7 @@ __global__ void __launch_bounds__(320) qcache_step_kernel(QcStoreParams p, DevSt
     over8();
     const bool odd = top >= 0x7f800000u;
     if (__any_sync(0xffffffffu, odd)) {
-      if (odd) top = qc_finite_top(raw);
+      if (odd) top = qc_bits(qc_finite_top(raw, 0.0f));
       over8();
       if (odd && c == 0) qc_report(status, WDZ_ENAN, 2000000 + (int)blockIdx.x);
     }
@@ -306,8 +352,8 @@ __global__ void __launch_bounds__(320) qcache_step_kernel(QcStoreParams p, DevSt
     if (has) {
       float x[8];
       raw.get(x);
-      const float inv = now > 0.0f ? __fdiv_rn(1.0f, now) : 0.0f;
-      *reinterpret_cast<uint2*>(place.q + (int64_t)run.p0 * QC_HD + 8 * c) = now > 0.0f ? qc_code8(x, odd ? -now : now, inv) : make_uint2(0, 0);
+      const QcDivisor by(now);
+      *reinterpret_cast<uint2*>(place.q + (int64_t)run.p0 * QC_HD + 8 * c) = odd ? qc_settle8(x, by) : qc_code8(x, by);
       if (c == 0) {
         if (!kept || now > old) place.s[b] = now;
         if (kept && now > old) {
