@@ -2069,7 +2069,7 @@ int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_
   const int sp = e->span_begin(WDZ_PROF_DEC_GEMM, (double)N * p.Kp * (0.5 + 2.0 / group), (cudaStream_t)s);
   const int tiles = (N + 15) / 16, segs = p.Kp / 128;
   p.split = 1;
-  while (p.split < GP_WARPS && p.split < segs && (int64_t)tiles * p.split < 8ll * e->sm_count) p.split *= 2;
+  while (p.split < GP_WARPS && p.split < segs && (int64_t)tiles * p.split < 8ll * e->sm_count) p.split *= 2, ++p.split_log;
   const int64_t esz = x_dtype == WDZ_BF16 ? 2 : 4;
   p.vec = K % 8 == 0 && aligned16(x_dev, M > 1 ? ldx * esz : 0);
   auto go = [&](auto kern, int rows_per_cta, size_t smem) {

@@ -33,12 +33,12 @@ struct GemvPackedParams {
   const float* residual;   // f32 [M, N], or nullptr; may be y
   float* y;
   int M, N, K, Kp, group;
-  int split;               // warps that share a tile of 16 features
+  int split, split_log;    // warps that share a tile of 16 features: 1, 2, 4 or 8
   bool vec;                // rows of x can be read in pieces of eight
 };
 
 constexpr int GP_WARPS = 8;
-constexpr int GP_AHEAD = 4;   // segments of 128 weights that a warp of the byte kernel has under way
+constexpr int GP_AHEAD = 2;   // segments of 128 weights that a warp of the byte kernel has under way
 
 __device__ __forceinline__ void mma_s8_16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -111,22 +111,29 @@ template <> struct GpScale<4> {
 // The 16 features' sums of `split` warps, plus bias and residual, for rows m0 .. m0 + rows.
 template <typename T, int ROWS>
 __device__ __forceinline__ void gp_finish(const GemvPackedParams& p, const float (&red)[GP_WARPS][ROWS][17], int m0) {
-  const int rows = min(ROWS, p.M - m0), cols = 16 * (GP_WARPS / p.split), n_first = blockIdx.x * cols;
-  for (int i = threadIdx.x; i < rows * cols; i += GP_WARPS * 32) {
-    const int row = i / cols, col = i % cols, n = n_first + col;
+  const int rows = min(ROWS, p.M - m0), shift = 7 - p.split_log, cols = 1 << shift, n_first = blockIdx.x << shift;
+  for (int i = threadIdx.x; i < rows << shift; i += GP_WARPS * 32) {
+    const int row = i >> shift, col = i & (cols - 1), n = n_first + col;
     if (n >= p.N) continue;
-    float v = 0.0f;
-    for (int w = 0; w < p.split; ++w) v += red[(col >> 4) * p.split + w][row][col & 15];
-    if (p.bias) v += to_f(reinterpret_cast<const T*>(p.bias)[n]);
     const int64_t at = (int64_t)(m0 + row) * p.N + n;
-    if (p.residual) v += p.residual[at];
-    p.y[at] = v;
+    float v = p.residual ? p.residual[at] : 0.0f;
+    if (p.bias) v += to_f(reinterpret_cast<const T*>(p.bias)[n]);
+    float sum = 0.0f;
+    for (int w = 0; w < p.split; ++w) sum += red[((col >> 4) << p.split_log) + w][row][col & 15];
+    p.y[at] = v + sum;
   }
 }
 
 constexpr float GP_S8_STEPS = 127.0f * 16777216.0f;   // a row's largest value in steps: rounding up leaves its top byte a byte
 constexpr int GP_S8_ROWS = 2, GP_S8_CHUNK = 64;       // rows of a CTA, segments of x that one pass keeps in shared memory (64 KB)
 template <int PAIRS> constexpr int GP_F32_CHUNK = PAIRS == 1 ? 40 : 10;   // the same (80 KB)
+
+// The upper nibbles u of four bytes as 16 (u - 8): one instruction with both masks in registers.
+__device__ __forceinline__ uint32_t gp_signed16(uint32_t w, uint32_t flip, uint32_t keep) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0x28;" : "=r"(r) : "r"(w), "r"(flip), "r"(keep));   // (w ^ flip) & keep
+  return r;
+}
 
 // Block = 8 warps; grid = (tiles of 16 features x split / 8, rows / 2).  GS: scales of a segment of 128 weights.
 template <int GS>
@@ -136,7 +143,7 @@ __global__ void __launch_bounds__(GP_WARPS * 32, 3) gemv_packed_s8_kernel(GemvPa
   __shared__ float tops[GP_WARPS][GP_S8_ROWS];
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int part = warp % p.split, tile = blockIdx.x * (GP_WARPS / p.split) + warp / p.split;
+  const int part = warp & (p.split - 1), tile = blockIdx.x * (GP_WARPS >> p.split_log) + (warp >> p.split_log);
   const int m0 = blockIdx.y * GP_S8_ROWS, segs = p.Kp >> 7, rows = min(GP_S8_ROWS, p.M - m0);
   const int na = min(tile * 16 + g, p.N - 1), nb = min(tile * 16 + g + 8, p.N - 1);
   const uint4* wa = reinterpret_cast<const uint4*>(p.W + (int64_t)na * (p.Kp >> 3)) + t;   // a segment is four uint4
@@ -147,20 +154,22 @@ __global__ void __launch_bounds__(GP_WARPS * 32, 3) gemv_packed_s8_kernel(GemvPa
   pdl_wait();
 
   float sum[2] = {0.0f, 0.0f};
+  const uint32_t xs_at = (uint32_t)__cvta_generic_to_shared(xs);
+  const uint32_t xs_mine = xs_at + 8 * ((rows == 1 ? lane & 15 : lane));   // a lone row's columns twice: no column is empty
   for (int first = 0; first < segs; first += GP_S8_CHUNK) {
-    const int here = min(GP_S8_CHUNK, segs - first), last = first + here;
+    const int here = min(GP_S8_CHUNK, segs - first);
+    const int n = part < here ? (here - part + p.split - 1) >> p.split_log : 0;   // segments of this warp
     uint4 a[GP_AHEAD], b[GP_AHEAD];
     GpScale<GS> fa[GP_AHEAD], fb[GP_AHEAD];
-    auto fetch = [&](int u, int sg) {
-      if (sg < last) {
-        a[u] = __ldg(wa + 4 * sg);
-        b[u] = __ldg(wb + 4 * sg);
-        fa[u].load(sa + sg * GS);
-        fb[u].load(sb + sg * GS);
-      }
+    auto fetch = [&](int u, int j) {
+      const int sg = first + part + (j << p.split_log);
+      a[u] = __ldg(wa + 4 * sg);
+      b[u] = __ldg(wb + 4 * sg);
+      fa[u].load(sa + sg * GS);
+      fb[u].load(sb + sg * GS);
     };
 #pragma unroll
-    for (int u = 0; u < GP_AHEAD; ++u) fetch(u, first + part + u * p.split);   // under way while x is taken apart
+    for (int u = 0; u < GP_AHEAD; ++u) if (u < n) fetch(u, u);   // under way while x is taken apart
 
     // largest value of each row, 8 values a thread and step
     const int units = here * 16;
@@ -217,36 +226,42 @@ __global__ void __launch_bounds__(GP_WARPS * 32, 3) gemv_packed_s8_kernel(GemvPa
     __syncthreads();
 
     float acc[2] = {0.0f, 0.0f};
-    const bool mine = (g >> 2) < rows;
-    for (int base = first + part; base < last; base += GP_AHEAD * p.split) {
+    uint32_t flip = 0x80808080u, keep = 0xf0f0f0f0u;
+    asm volatile("" : "+r"(flip), "+r"(keep));   // known to nobody: they stay in registers
+    for (int j = 0; j < n; j += GP_AHEAD) {
 #pragma unroll
       for (int u = 0; u < GP_AHEAD; ++u) {
-        const int sg = base + u * p.split;
-        if (sg < last) {
-          const uint4 a_now = a[u], b_now = b[u];
-          const GpScale<GS> fa_now = fa[u], fb_now = fb[u];
-          fetch(u, sg + GP_AHEAD * p.split);
-          const uint32_t* aw = reinterpret_cast<const uint32_t*>(&a_now);
-          const uint32_t* bw = reinterpret_cast<const uint32_t*>(&b_now);
-          const uint2* xq = xs + (sg - first) * 128 + lane;
-          int c[4] = {0, 0, 0, 0};
+        if (j + u >= n) break;
+        uint32_t op[4][4];
+        const uint32_t aw[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, bw[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint2 xb = make_uint2(0, 0);
-            if (mine) xb = xq[32 * i];
-            mma_s8_16832(c, ((aw[i] << 4) ^ 0x80808080u) & 0xf0f0f0f0u, ((bw[i] << 4) ^ 0x80808080u) & 0xf0f0f0f0u,
-                         (aw[i] ^ 0x80808080u) & 0xf0f0f0f0u, (bw[i] ^ 0x80808080u) & 0xf0f0f0f0u, xb.x, xb.y);
-            if ((i + 1) % (4 / GS) == 0) {   // the end of a group: columns (d1, d0) or (d3, d2) fold into one number
-              acc[0] = fmaf((float)(c[0] * 256 + c[1]), fa_now.get(i / (4 / GS)), acc[0]);
-              acc[1] = fmaf((float)(c[2] * 256 + c[3]), fb_now.get(i / (4 / GS)), acc[1]);
-              c[0] = c[1] = c[2] = c[3] = 0;
-            }
+        for (int i = 0; i < 4; ++i) {
+          op[i][0] = gp_signed16(aw[i] << 4, flip, keep);
+          op[i][1] = gp_signed16(bw[i] << 4, flip, keep);
+          op[i][2] = gp_signed16(aw[i], flip, keep);
+          op[i][3] = gp_signed16(bw[i], flip, keep);
+        }
+        float sa_g[GS], sb_g[GS];
+#pragma unroll
+        for (int i = 0; i < GS; ++i) { sa_g[i] = fa[u].get(i); sb_g[i] = fb[u].get(i); }
+        if (j + u + GP_AHEAD < n) fetch(u, j + u + GP_AHEAD);
+        const uint32_t xq = xs_mine + ((part + ((j + u) << p.split_log)) << 10);
+        int c[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint2 xb;
+          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(xb.x), "=r"(xb.y) : "r"(xq + 256 * i));
+          mma_s8_16832(c, op[i][0], op[i][1], op[i][2], op[i][3], xb.x, xb.y);
+          if ((i + 1) % (4 / GS) == 0) {   // the end of a group: columns (d1, d0) or (d3, d2) fold into one number
+            acc[0] = fmaf((float)(c[0] * 256 + c[1]), sa_g[i / (4 / GS)], acc[0]);
+            acc[1] = fmaf((float)(c[2] * 256 + c[3]), sb_g[i / (4 / GS)], acc[1]);
+            c[0] = c[1] = c[2] = c[3] = 0;
           }
         }
       }
     }
     // a step of the row, / 16 for the shifted nibble; an infinite or NaN row: infinity times zero is NaN
-    const float step = (t >> 1 ? top[1] : top[0]) * (1.0f / (16.0f * GP_S8_STEPS)) * (t & 1 ? 65536.0f : 1.0f);
+    const float step = (t >> 1 && rows > 1 ? top[1] : top[0]) * (1.0f / (16.0f * GP_S8_STEPS)) * (t & 1 ? 65536.0f : 1.0f);
     sum[0] = fmaf(acc[0], step, sum[0]);
     sum[1] = fmaf(acc[1], step, sum[1]);
   }
@@ -266,7 +281,7 @@ __global__ void __launch_bounds__(GP_WARPS * 32) gemv_packed_f32_kernel(GemvPack
   __shared__ float red[GP_WARPS][2 * PAIRS][17];
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int part = warp % p.split, tile = blockIdx.x * (GP_WARPS / p.split) + warp / p.split;
+  const int part = warp & (p.split - 1), tile = blockIdx.x * (GP_WARPS >> p.split_log) + (warp >> p.split_log);
   const int m0 = blockIdx.y * 2 * PAIRS, segs = p.Kp >> 7, rows = min(2 * PAIRS, p.M - m0);
   const int na = min(tile * 16 + g, p.N - 1), nb = min(tile * 16 + g + 8, p.N - 1);
   const uint4* wa = reinterpret_cast<const uint4*>(p.W + (int64_t)na * (p.Kp >> 3)) + t;
@@ -363,7 +378,7 @@ __global__ void __launch_bounds__(GP_WARPS * 32) gemv_packed_bf16_kernel(GemvPac
   __shared__ float red[GP_WARPS][8 * NT][17];
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int part = warp % p.split, tile = blockIdx.x * (GP_WARPS / p.split) + warp / p.split;
+  const int part = warp & (p.split - 1), tile = blockIdx.x * (GP_WARPS >> p.split_log) + (warp >> p.split_log);
   const int m0 = blockIdx.y * 8 * NT, segs = p.Kp >> 7;
   const int na = min(tile * 16 + g, p.N - 1), nb = min(tile * 16 + g + 8, p.N - 1);
   const uint4* wa = reinterpret_cast<const uint4*>(p.W + (int64_t)na * (p.Kp >> 3)) + t;   // a segment is four uint4

@@ -459,9 +459,10 @@ class Engine:
 
     def _index(self, name: str, x, n: int) -> torch.Tensor:
         """An int32 index tensor of ``n`` entries on the device; host sequences are uploaded."""
-        if not isinstance(x, torch.Tensor) or x.dtype != torch.int32 or x.get_device() != self._ordinal or not x.is_contiguous():
-            x = self._i32(x)
-        if x.dim() != 1 or x.shape[0] != n:
+        if isinstance(x, torch.Tensor) and x.dtype is torch.int32 and x.numel() == n and x.is_contiguous() and x.get_device() == self._ordinal:
+            return x
+        x = self._i32(x)
+        if x.numel() != n:
             raise ValueError(f"{name} must have {n} entries, got {tuple(x.shape)}")
         return x
 
@@ -520,36 +521,47 @@ class Engine:
         to 8, consecutive query heads sharing a key head.  Returns [n, q_heads * 64] in ``out_dtype`` (default: the
         engine's type), or fills ``out``.  Length 0 gives zeros; a row whose slot lies outside the cache is left as it
         was (zeros when ``out`` is not given)."""
-        width = q.shape[1] if q.dim() == 2 else q.shape[1:].numel()
+        if q.dim() == 3:
+            q = q.flatten(1)
+        elif q.dim() != 2:
+            raise ValueError(f"q must be [rows, q_heads * {HEAD_DIM}], got {tuple(q.shape)}")
+        n, width = q.shape
         shared, rest = divmod(width, cache.n_heads * HEAD_DIM)
         if rest or not 1 <= shared <= 8:
             raise ValueError(f"q must have 1 to 8 times the cache's {cache.n_heads} heads of {HEAD_DIM}, got {tuple(q.shape)}")
-        self._here("the cache", cache.ordinal)
-        q = self._rows("q", q, width)
-        n = q.shape[0]
+        ordinal = self._ordinal
+        if cache.ordinal != ordinal or q.get_device() != ordinal:
+            raise ValueError("q and the cache must lie on the engine's device")
+        code = _TORCH_DTYPE.get(q.dtype)
+        if code is None:
+            raise ValueError(f"q must be float32 or bfloat16, got {q.dtype}")
+        step, one = q.stride()
+        at = q.data_ptr()
+        if one != 1 or (step < width and n > 1) or step % (8 if code else 4) or at % 16:
+            q = q.clone(memory_format=torch.contiguous_format)
+            step, at = width, q.data_ptr()
         if out is None:
-            to = out_dtype or self.dtype
-            if to not in _TORCH_DTYPE:
+            to = _TORCH_DTYPE.get(out_dtype or self.dtype)
+            if to is None:
                 raise ValueError("out_dtype must be float32 or bfloat16")
-            given, out = False, q.new_empty((n, width), dtype=to)
+            clear, out, out_step = 1, q.new_empty((n, width), dtype=out_dtype or self.dtype), width
         else:
-            given, to = True, out.dtype
-            if (to not in _TORCH_DTYPE or out_dtype not in (None, to) or tuple(out.shape) != (n, width) or out.stride(1) != 1
-                    or (n > 1 and out.stride(0) < width) or out.stride(0) * out.element_size() % 16 or out.data_ptr() % 16):
+            to, clear = _TORCH_DTYPE.get(out.dtype), 0
+            if (to is None or out_dtype not in (None, out.dtype) or tuple(out.shape) != (n, width) or out.stride(1) != 1
+                    or (n > 1 and out.stride(0) < width) or out.stride(0) % (8 if to else 4) or out.data_ptr() % 16):
                 raise ValueError(f"out must be [{n}, {width}] rows in float32 or bfloat16 that start on 16 bytes")
             self._here("out", out.get_device())
-        sl, ln = self._index("slots", slots, n), self._index("lens", lens, n)
+            out_step = out.stride(0)
+        slots, lens = self._index("slots", slots, n), self._index("lens", lens, n)
         if n == 0:
             return out
         need = cache.scratch.get((n, shared))
         if need is None:
-            need = self.lib.wdz_qcache_attention_scratch(self.h, cache.ref, width // HEAD_DIM, n)
-            cache.scratch[(n, shared)] = need
-        scratch = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
+            need = cache.scratch[(n, shared)] = max(0, self.lib.wdz_qcache_attention_scratch(self.h, cache.ref, width // HEAD_DIM, n))
+        scratch = q.new_empty(need, dtype=torch.uint8) if need else None
         rc = self.lib.wdz_qcache_attention(
-            self.h, cache.ref, q.data_ptr(), q.stride(0), _TORCH_DTYPE[q.dtype], width // HEAD_DIM, sl.data_ptr(),
-            ln.data_ptr(), n, scale, out.data_ptr(), out.stride(0), _TORCH_DTYPE[to], not given,
-            None if scratch is None else scratch.data_ptr(), need if need > 0 else 0, self._raw_stream())
+            self.h, cache.ref, at, step, code, width // HEAD_DIM, slots.data_ptr(), lens.data_ptr(), n, scale, out.data_ptr(),
+            out_step, to, clear, scratch.data_ptr() if need else None, need, torch._C._cuda_getCurrentRawStream(ordinal))
         if rc:
             self._check(rc)
         return out
@@ -558,29 +570,41 @@ class Engine:
                            out: torch.Tensor | None = None) -> torch.Tensor:
         """``linear_rows`` with 4-bit weights (``lowbit.pack_linear``): x f32 or bf16 [M, K] @ W[N, K].T (+ bias)
         (+ residual f32 [M, N]) -> f32 [M, N].  ``residual`` and ``out`` may be the same tensor."""
-        self._here("the weights", w.ordinal)
-        if x.dtype not in _TORCH_DTYPE or x.dim() != 2 or x.shape[1] != w.in_features:
+        code, ordinal = _TORCH_DTYPE.get(x.dtype), self._ordinal
+        if code is None or x.dim() != 2:
             raise ValueError(f"x must be [rows, {w.in_features}] in float32 or bfloat16, got {x.dtype} {tuple(x.shape)}")
-        self._here("x", x.get_device())
-        if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
-            x = x.contiguous()
-        M, N = x.shape[0], w.out_features
-        for name, t in (("residual", residual), ("out", out)):
-            if t is not None:
-                if t.dtype != torch.float32 or tuple(t.shape) != (M, N) or not t.is_contiguous():
-                    raise ValueError(f"{name} must be a contiguous float32 [{M}, {N}]")
-                self._here(name, t.get_device())
-        y = out if out is not None else x.new_empty((M, N), dtype=torch.float32)
+        M, K = x.shape
+        if K != w.in_features:
+            raise ValueError(f"x must be [rows, {w.in_features}], got {tuple(x.shape)}")
+        if w.ordinal != ordinal or x.get_device() != ordinal:
+            raise ValueError("x and the weights must lie on the engine's device")
+        step, one = x.stride()
+        if one != 1 or (step < K and M > 1):
+            x = x.clone(memory_format=torch.contiguous_format)
+            step = K
+        N = w.out_features
+        add = None
+        if residual is not None:
+            add = self._f32_rows("residual", residual, M, N).data_ptr()
+        if out is None:
+            out = x.new_empty((M, N), dtype=torch.float32)
+        else:
+            self._f32_rows("out", out, M, N)
         b = w.bias
-        if b is not None and b.dtype != x.dtype:
+        if b is not None and b.dtype is not x.dtype:
             b = b.to(x.dtype)
         rc = self.lib.wdz_linear_rows_packed(
-            self.h, x.data_ptr(), x.stride(0), _TORCH_DTYPE[x.dtype], M, w.in_features, w.weight.data_ptr(),
-            w.scale.data_ptr(), w.group, None if b is None else b.data_ptr(),
-            None if residual is None else residual.data_ptr(), N, y.data_ptr(), self._raw_stream())
+            self.h, x.data_ptr(), step, code, M, K, w.at, w.scale_at, w.group, None if b is None else b.data_ptr(), add, N,
+            out.data_ptr(), torch._C._cuda_getCurrentRawStream(ordinal))
         if rc:
             self._check(rc)
-        return y
+        return out
+
+    def _f32_rows(self, name: str, t: torch.Tensor, M: int, N: int) -> torch.Tensor:
+        if t.dtype is not torch.float32 or tuple(t.shape) != (M, N) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous float32 [{M}, {N}]")
+        self._here(name, t.get_device())
+        return t
 
     # ------------------------------------------------------- word-timing alignment
     def align_configure(self, heads) -> None:

@@ -82,6 +82,7 @@ class PackedLinear:
         self.weight, self.scale, self.in_features, self.group = weight, scale, int(in_features), int(group)
         self.out_features, self.device, self.ordinal = weight.shape[0], weight.device, weight.get_device()
         self.bias = None if bias is None else bias.contiguous()
+        self.at, self.scale_at = weight.data_ptr(), scale.data_ptr()
 
 
 def pack_linear(weight: torch.Tensor, group: int = 64, bias: torch.Tensor | None = None) -> PackedLinear:
