@@ -96,6 +96,20 @@ def test_store_steps(eng, rows, dtype):
     eng.device_status()
 
 
+@pytest.mark.parametrize("heads", [1, 21, 45])
+def test_store_steps_of_any_head_count(eng, heads):
+    """More heads than a block takes at a time, K and V at different distances, scales that grow in some heads only."""
+    g = torch.Generator().manual_seed(heads)
+    d = heads * 64
+    k = torch.randn(3, d + 64, generator=g)[:, :d]
+    v = torch.randn(3, 2 * d, generator=g)[:, d:]
+    k[0] *= 30
+    v[1, ::2] *= 30
+    _check_store(eng, _filled(4, heads, 2, seed=heads), k, v, [3, 0, 2], [63, 100, 64])
+    _check_store(eng, _filled(4, heads, 2, seed=heads), k, v, [3, 0, 2], [63, 100, 64], [0, 1, 2, 3])   # as runs
+    eng.device_status()
+
+
 def test_store_token_by_token_fills_a_slot_like_the_definition(eng):
     parts = [t * 0 for t in _filled(2, 2, 3)]
     want = [t.clone().numpy() for t in parts]
@@ -372,7 +386,8 @@ def _check_linear(eng, x, packed, w, b, residual=None, out=None):
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("m,n,k", [(1, 1280, 1280), (1, 17, 130), (2, 64, 64), (3, 100, 1), (5, 33, 1237), (8, 256, 5120), (9, 31, 640),
-                                   (16, 160, 256), (17, 48, 384), (33, 16, 136), (70, 15, 127)])
+                                   (16, 160, 256), (17, 48, 384), (33, 16, 136), (70, 15, 127), (2, 40, 9000), (1, 16, 20000),
+                                   (4, 24, 8192)])
 def test_linear_shapes(eng, m, n, k, group, dtype):
     packed, w, b = _packed(n, k, group, seed=m + n, bias=dtype if m % 2 else None)
     x = torch.randn(m, k, generator=torch.Generator().manual_seed(k)).to(dtype)
@@ -477,6 +492,58 @@ def test_decode_steps_run_together(eng):
         # the attention's bf16 rounding, 2^-8 of each value, through the product; all else is fp32
         tol = 1.01 * 2.0 ** -8 * (np.abs(a) @ np.abs(wo).T) + 1e-4 * np.abs(want).max()
         assert (np.abs(y.double().cpu().numpy() - want) <= tol).all()
+
+
+@pytest.mark.parametrize("rows,heads,group,tokens", [(1, 20, 1, 1500), (2, 4, 4, 20000), (40, 20, 1, 448)])
+def test_attention_captured(eng, rows, heads, group, tokens):
+    """Each way that a launch is cut (clusters, parts with scratch of the graph's own, a CTA a row), replayed with other
+    lengths and other queries while an eager call runs beside it."""
+    cache = _cuda_cache(_filled(rows, heads, (tokens + 63) // 64, seed=1))
+    g = torch.Generator().manual_seed(2)
+    q = torch.randn(rows, heads * group * 64, generator=g).cuda()
+    slots = torch.arange(rows, dtype=torch.int32).cuda()
+    lens = torch.full((rows,), tokens, dtype=torch.int32).cuda()
+    eng.qcache_attention(q, cache, slots, lens, out_dtype=F32)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = eng.qcache_attention(q, cache, slots, lens, out_dtype=F32)
+    for n in (tokens, 1, tokens // 2, 0, tokens - 1):
+        lens.fill_(n)
+        q.copy_(torch.randn(q.shape, generator=g))
+        want = eng.qcache_attention(q, cache, slots, lens, out_dtype=F32).clone()
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            graph.replay()
+        beside = eng.qcache_attention(q, cache, slots, lens, out_dtype=F32)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(beside, want)
+        if n == 0:
+            assert (out == 0).all()
+    eng.device_status()
+
+
+def test_attention_in_place_of_its_queries(eng):
+    parts = _filled(3, 4, 3, seed=1)
+    q = torch.randn(3, 256, generator=torch.Generator().manual_seed(3))
+    c = _cuda_cache(parts)
+    want = eng.qcache_attention(q.cuda(), c, [2, 0, 1], [190, 64, 0], out_dtype=F32)
+    both = q.cuda()
+    assert eng.qcache_attention(both, c, [2, 0, 1], [190, 64, 0], out=both) is both
+    assert torch.equal(both, want)
+
+
+def test_calls_refuse_tensors_elsewhere(eng):
+    c = _cuda_cache(_filled(2, 2, 1))
+    q, i = torch.zeros(2, 128), torch.zeros(2, dtype=torch.int32)
+    host = QCache(*_filled(2, 2, 1))
+    for call in (lambda: eng.qcache_attention(q, c, i, i), lambda: eng.qcache_attention(q.cuda(), host, i, i),
+                 lambda: eng.qcache_attention(q.cuda(), c, i, i, out=torch.zeros(2, 128)),
+                 lambda: eng.qcache_store(c, q, q, [0, 1], [0, 0]), lambda: eng.qcache_store(host, q.cuda(), q.cuda(), [0, 1], [0, 0]),
+                 lambda: eng.linear_rows_packed(torch.zeros(1, 128), _packed(4, 128, 32, 0)[0]),
+                 lambda: eng.linear_rows_packed(torch.zeros(1, 128).cuda(), pack_linear(torch.zeros(4, 128)))):
+        with pytest.raises(ValueError):
+            call()
 
 
 def test_steps_in_captured_graphs_and_on_side_streams(eng):

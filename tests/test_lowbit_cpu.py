@@ -142,7 +142,8 @@ def test_abi_refuses_bad_arguments_before_it_looks_at_the_engine(lib, handle):
     not_ready = -4
     assert store() == not_ready and attend() == not_ready and linear() == not_ready
     caches = [_desc(k=None), _desc(v_scale=None), _desc(k=257), _desc(slot_stride=2 * 2 * 4096 - 16), _desc(slot_stride=2 * 2 * 4096 + 8),
-              _desc(scale_slot_stride=3), _desc(n_slots=0), _desc(n_heads=0), _desc(n_blocks=0), _desc(n_blocks=2 ** 30)]
+              _desc(scale_slot_stride=3), _desc(n_slots=0), _desc(n_heads=0), _desc(n_blocks=0), _desc(n_blocks=2 ** 30),
+              _desc(v_scale=2050)]
     for c in caches:
         assert store(cache=c) == -1 and attend(cache=c) == -1
     for bad in (dict(k=None), dict(v=None), dict(sl=None), dict(ps=None), dict(dtype=2), dict(n=-1), dict(runs=-1), dict(most=-1),
@@ -155,8 +156,12 @@ def test_abi_refuses_bad_arguments_before_it_looks_at_the_engine(lib, handle):
                 dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=-1.0)):
         assert attend(**bad) == -1, bad
     for bad in (dict(x=None), dict(w=None), dict(sc=None), dict(y=None), dict(xt=9), dict(M=-1), dict(N=0), dict(K=0), dict(g=16), dict(g=0),
-                dict(ldx=129), dict(w=4104), dict(sc=4100), dict(K=2 ** 31 - 100)):
+                dict(ldx=129), dict(w=4104), dict(sc=4100), dict(K=2 ** 31 - 100), dict(x=4098), dict(b=4098), dict(r=4098), dict(y=4097)):
         assert linear(**bad) == -1, bad
+    assert linear(M=8 * 65535 + 1) == -5
+    assert lib.wdz_qcache_attention_scratch(handle, C.byref(_desc()), 2, -1) == -1
+    assert lib.wdz_qcache_attention_scratch(handle, C.byref(_desc()), 2, 3) == 0
+    assert lib.wdz_qcache_attention_scratch(handle, C.byref(_desc(n_blocks=512, slot_stride=2 ** 26, scale_slot_stride=2 ** 12)), 4, 1) > 0
     assert lib.wdz_qcache_store(None, C.byref(_desc()), 1, 1, 1, 1, 0, 1, None, 1, 1, 1, 1, None) == -1
 
 

@@ -1888,6 +1888,7 @@ int qcache_view(wdz_engine* e, const char* who, const wdz_qcache* c, QcView* v) 
     return e->fail(WDZ_EINVAL, "%s: the slots of the cache overlap", who);
   if (!aligned16(c->k_dev, c->slot_stride) || !aligned16(c->v_dev, c->slot_stride))
     return e->fail(WDZ_EINVAL, "%s: the cache's values must start on 16 bytes", who);
+  if (((uintptr_t)c->k_scale_dev | (uintptr_t)c->v_scale_dev) & 3) return e->fail(WDZ_EINVAL, "%s: scales must start on 4 bytes", who);
   *v = QcView{(int8_t*)c->k_dev, (int8_t*)c->v_dev, c->k_scale_dev, c->v_scale_dev, c->slot_stride, c->scale_slot_stride,
               c->n_slots, c->n_heads, c->n_blocks};
   return WDZ_OK;
@@ -2053,13 +2054,17 @@ int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_
   if (!e) return WDZ_EINVAL;
   int rc;
   if (x_dtype != WDZ_F32 && x_dtype != WDZ_BF16) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: unknown type %d", x_dtype);
-  if (M < 0 || M > 16 * 65535 || N < 1 || K < 1 || K > INT32_MAX - 128) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: %d x %d x %d", M, N, K);
+  if (M < 0 || N < 1 || K < 1 || K > INT32_MAX - 128) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: %d x %d x %d", M, N, K);
   if (group != 32 && group != 64 && group != 128) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: group %d (32, 64 or 128)", group);
+  if (M > 8 * 65535) return e->fail(WDZ_ECAPACITY, "wdz_linear_rows_packed: %d rows in one call, at most %d", M, 8 * 65535);
   if (M == 0) return WDZ_OK;
   if (!x_dev || !w_dev || !scale_dev || !y_dev) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: null argument");
   if (ldx < K && M > 1) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: rows overlap");
   if (((uintptr_t)w_dev & 15) || ((uintptr_t)scale_dev & 7))
     return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: weights must start on 16 bytes, scales on 8");
+  const uintptr_t own = x_dtype == WDZ_BF16 ? 1 : 3;
+  if (((uintptr_t)x_dev & own) || ((uintptr_t)bias_dev & own) || (((uintptr_t)residual_dev | (uintptr_t)y_dev) & 3))
+    return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: misaligned x, bias, residual or y");
   GemvPackedParams p{};
   p.x = x_dev; p.ldx = ldx; p.W = (const uint32_t*)w_dev; p.scale = (const bf16*)scale_dev; p.bias = bias_dev;
   p.residual = residual_dev; p.y = y_dev;

@@ -61,7 +61,7 @@ __device__ __forceinline__ void gp_unpack(uint32_t w, uint32_t (&r)[4]) {
 __device__ __forceinline__ uint4 gp_row(const bf16* row, int k0, int K, bool vec) {
   uint4 v = make_uint4(0, 0, 0, 0);
   if (vec) {
-    if (k0 < K) v = __ldg(reinterpret_cast<const uint4*>(row + k0));
+    if (k0 < K) v = *reinterpret_cast<const uint4*>(row + k0);   // plain loads: the kernel before may have written x
     return v;
   }
   const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
@@ -82,7 +82,7 @@ __device__ __forceinline__ void gp_row8(const bf16* row, int k0, int K, bool vec
 __device__ __forceinline__ void gp_row8(const float* row, int k0, int K, bool vec, float (&v)[8]) {
   if (vec) {
     float4 lo = make_float4(0, 0, 0, 0), hi = lo;
-    if (k0 < K) { lo = __ldg(reinterpret_cast<const float4*>(row + k0)); hi = __ldg(reinterpret_cast<const float4*>(row + k0 + 4)); }
+    if (k0 < K) { lo = *reinterpret_cast<const float4*>(row + k0); hi = *reinterpret_cast<const float4*>(row + k0 + 4); }
     v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
   } else {
 #pragma unroll
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(GP_WARPS * 32, 3) gemv_packed_s8_kernel(GemvPa
 
 // PAIRS: pairs of rows a CTA takes.  Block = 8 warps; grid = (tiles of 16 features x split / 8, rows / (2 PAIRS)).
 template <int PAIRS, int GS>
-__global__ void __launch_bounds__(GP_WARPS * 32) gemv_packed_f32_kernel(GemvPackedParams p) {
+__global__ void __launch_bounds__(GP_WARPS * 32, 2) gemv_packed_f32_kernel(GemvPackedParams p) {
   extern __shared__ __align__(16) uint4 xf[];   // [segment][pair][i][lane]: eight values of a lane's column
   __shared__ float red[GP_WARPS][2 * PAIRS][17];
   pdl_trigger();
@@ -311,20 +311,29 @@ __global__ void __launch_bounds__(GP_WARPS * 32) gemv_packed_f32_kernel(GemvPack
     fetch(0, first + part);
     fetch(1, first + part + p.split);
     __syncthreads();   // the pass before has read xf
-    for (int i = threadIdx.x; i < here * 16 * rows; i += GP_WARPS * 32) {
-      const int m = i / (here * 16), unit = i % (here * 16), sg = unit >> 4, at = (unit & 15) >> 2, tt = unit & 3;
-      float v[8];
-      gp_row8(x + (int64_t)m * p.ldx, first * 128 + 8 * unit, p.K, p.vec, v);
+    for (int unit = threadIdx.x; unit < here * 16; unit += GP_WARPS * 32) {   // of eight values, in every row
+      uint4* to = xf + (((unit >> 4) * PAIRS * 4 + ((unit & 15) >> 2)) * 32 + (unit & 3));
+#pragma unroll 1
+      for (int pair = 0; 2 * pair < rows; ++pair, to += 128) {
+        float v[2][8];
 #pragma unroll
-      for (int q = 0; q < 3; ++q) {   // the upper 16 bits of what is left, cut off, not rounded: nothing overflows
-        uint32_t w[4];
+        for (int k = 0; k < 2; ++k)
+          if (2 * pair + k < rows) gp_row8(x + (int64_t)(2 * pair + k) * p.ldx, first * 128 + 8 * unit, p.K, p.vec, v[k]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = __byte_perm(__float_as_uint(v[2 * j]), __float_as_uint(v[2 * j + 1]), 0x7632);
-        xf[((sg * PAIRS + (m >> 1)) * 4 + at) * 32 + ((m & 1) * 4 + q) * 4 + tt] = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int k = 0; k < 2; ++k) {
+          if (2 * pair + k >= rows) break;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float cut = __uint_as_float(__float_as_uint(v[j]) & 0xffff0000u);
-          v[j] = fabsf(v[j]) == INFINITY ? 0.0f : v[j] - cut;
+          for (int q = 0; q < 3; ++q) {   // the upper 16 bits of what is left, cut off, not rounded: nothing overflows
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = __byte_perm(__float_as_uint(v[k][2 * j]), __float_as_uint(v[k][2 * j + 1]), 0x7632);
+            to[16 * k + 4 * q] = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float cut = __uint_as_float(__float_as_uint(v[k][j]) & 0xffff0000u);
+              v[k][j] = fabsf(v[k][j]) == INFINITY ? 0.0f : v[k][j] - cut;
+            }
+          }
         }
       }
     }
@@ -344,6 +353,7 @@ __global__ void __launch_bounds__(GP_WARPS * 32) gemv_packed_f32_kernel(GemvPack
         gp_unpack(bw[i], rb);
 #pragma unroll
         for (int q = 0; q < PAIRS; ++q) {
+          if (2 * q >= rows) break;
           uint4 xb = make_uint4(0, 0, 0, 0);
           if ((g & 3) != 3 && 2 * q + (g >> 2) < rows) xb = xf[(((sg - first) * PAIRS + q) * 4 + i) * 32 + lane];
           if (i % (4 / GS) == 0) c[q][0] = c[q][1] = c[q][2] = c[q][3] = 0.0f;

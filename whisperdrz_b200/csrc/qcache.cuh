@@ -97,28 +97,55 @@ __device__ __forceinline__ uint2 qc_settle8(const float (&x)[8], const QcDivisor
   return qc_bytes(n);
 }
 
-// rint(q s_old / s_new), half to even, of eight bytes.  The rounded quotient is at most one off; both products are exact
-// in 64 bits, and so is their difference wherever it decides.
-__device__ __forceinline__ uint2 qc_recode8(uint2 w, float s_old, float s_new) {
-  const float r = __fdiv_rn(s_old, s_new);
-  const double so = s_old, sn = s_new, half = 0.5 * sn;
-  uint32_t out[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t word = 0;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int q = (int)(int8_t)((h ? w.y : w.x) >> (8 * b));
-      int n = __float2int_rn((float)q * r);
-      const double d = (double)q * so - (double)n * sn;
-      const bool odd = n & 1;
-      if (d > half || (d == half && odd)) ++n;
-      else if (d < -half || (d == -half && odd)) --n;
-      word |= (uint32_t)(n & 255) << (8 * b);
-    }
-    out[h] = word;
+// What a block's bytes are multiplied by when its scale grows: s_old / s_new rounded, and the floats next to that.
+struct QcRatio {
+  float s_old, s_new, above, below;
+  __device__ QcRatio(float o, float n) : s_old(o), s_new(n) {
+    const uint32_t r = __float_as_uint(__fdiv_rn(o, n));
+    above = __uint_as_float(r + 1);
+    below = __uint_as_float(r ? r - 1 : 0);
   }
-  return make_uint2(out[0], out[1]);
+};
+
+// rint(q s_old / s_new), half to even, of eight bytes: by the same bracket, and by the exact difference of the products, which
+// 64 bits hold, where its ends differ.
+__device__ __forceinline__ uint2 qc_recode8(uint2 w, const QcRatio& by) {
+  constexpr float MAGIC = 12582912.0f;
+  uint32_t n[8], differ = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float q = (float)(int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+    n[i] = __float_as_uint(fmaf(q, by.above, MAGIC));
+    differ |= n[i] ^ __float_as_uint(fmaf(q, by.below, MAGIC));
+  }
+  if (differ) {
+    const double so = by.s_old, sn = by.s_new, half = 0.5 * sn;
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      const int q = (int)(int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+      int m = __float2int_rn((float)q * by.above);
+      const double d = (double)q * so - (double)m * sn;
+      const bool odd = m & 1;
+      if (d > half || (d == half && odd)) ++m;
+      else if (d < -half || (d == -half && odd)) --m;
+      if (i < 4) w.x = (w.x & ~(255u << (8 * i))) | (uint32_t)(m & 255) << (8 * i);
+      else w.y = (w.y & ~(255u << (8 * i - 32))) | (uint32_t)(m & 255) << (8 * i - 32);
+    }
+    return w;
+  }
+  return qc_bytes(n);
+}
+
+// Pieces i0, i0 + step, .. below n, of eight bytes each, at(i) their places: rounded to a grown scale, four loads at a time.
+template <typename At, typename By>
+__device__ __forceinline__ void qc_recode(int i0, int n, int step, At at, By by) {
+  for (int i = i0; i < n; i += 4 * step) {
+    uint2 w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) if (i + j * step < n) w[j] = *at(i + j * step);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) if (i + j * step < n) *at(i + j * step) = qc_recode8(w[j], by(i + j * step));
+  }
 }
 
 __device__ __forceinline__ void qc_report(DevStatus* st, int code, int detail) {
@@ -283,11 +310,11 @@ __global__ void __launch_bounds__((SHARE == 1 ? 2 : SHARE) * 32) qcache_store_ke
     const float now = fmaxf(old, qc_scale(bits));
     if (part == 0 && lane == 0) place.s[b] = now;   // every lane has read the old one
     int8_t* to = place.q + (int64_t)(b * QC_BLOCK + (lane >> 3)) * QC_HD + 8 * (lane & 7);
-    if (now > old && entered)
-      for (int t = b * QC_BLOCK + (lane >> 3) + 4 * part; t < lo; t += 4 * SHARE) {
-        uint2* at = reinterpret_cast<uint2*>(place.q + (int64_t)t * QC_HD + 8 * (lane & 7));
-        *at = qc_recode8(*at, old, now);
-      }
+    if (now > old && entered) {
+      const QcRatio ratio(old, now);
+      uint2* kept = reinterpret_cast<uint2*>(place.q + (int64_t)b * (QC_BLOCK * QC_HD));
+      qc_recode(part * 32 + lane, 8 * (lo - b * QC_BLOCK), 32 * SHARE, [&](int i) { return kept + i; }, [&](int) { return ratio; });
+    }
     const QcDivisor by(now);
     if (odd) {
 #pragma unroll 1
@@ -312,7 +339,7 @@ __global__ void __launch_bounds__((SHARE == 1 ? 2 : SHARE) * 32) qcache_store_ke
 // One row a run (a decode step).  Block = a run; eight threads a head of K or V.  Where a scale grows, the whole block
 // rounds the unit's earlier tokens to it together: alone, its eight threads would take up to 63 turns.
 template <typename T>
-__global__ void __launch_bounds__(320) qcache_step_kernel(QcStoreParams p, DevStatus* status) {
+__global__ void __launch_bounds__(320, 3) qcache_step_kernel(QcStoreParams p, DevStatus* status) {
   constexpr int UNITS = 320 / 8;
   __shared__ float olds[UNITS], news[UNITS];
   __shared__ int grown[UNITS], n_grown;
@@ -364,12 +391,13 @@ __global__ void __launch_bounds__(320) qcache_step_kernel(QcStoreParams p, DevSt
     }
     __syncthreads();
     const int pieces = 8 * kept;   // of 8 bytes, a unit
-    for (int i = threadIdx.x; i < n_grown * pieces; i += blockDim.x) {
-      const int k = i / pieces, g = grown[k];
-      const QcPlace to(p.c, run.slot, g >= p.c.n_heads ? g - p.c.n_heads : g, g >= p.c.n_heads);
-      uint2* at = reinterpret_cast<uint2*>(to.q + (int64_t)b * (QC_BLOCK * QC_HD)) + (i - k * pieces);
-      *at = qc_recode8(*at, olds[k], news[k]);
-    }
+    qc_recode(threadIdx.x, n_grown * pieces, blockDim.x,
+              [&](int i) {
+                const int g = grown[i / pieces];
+                const QcPlace to(p.c, run.slot, g >= p.c.n_heads ? g - p.c.n_heads : g, g >= p.c.n_heads);
+                return reinterpret_cast<uint2*>(to.q + (int64_t)b * (QC_BLOCK * QC_HD)) + i % pieces;
+              },
+              [&](int i) { return QcRatio(olds[i / pieces], news[i / pieces]); });
   }
 }
 
@@ -701,6 +729,7 @@ __global__ void __launch_bounds__(QC_MAX_WARPS * 32) qcache_attend_kernel(QcAtte
   pdl_wait();
   const uint32_t item = blockIdx.x / (uint32_t)share;
   const QcRow row(p, item);
+  if (lane == 0) asm volatile("fence.proxy.async.global;" ::: "memory");   // the bulk copies see what the kernels before wrote
   const int tiles = row.tiles(), stride = share * warps, tile0 = rank * warps + warp;
   const int mine = tile0 < tiles ? (tiles - tile0 + stride - 1) / stride : 0;   // tiles of this warp
   // pieces: K and V of the warp's tiles in turn

@@ -433,8 +433,8 @@ class Engine:
     def qcache(self, n_slots: int | None = None, n_tokens: int | None = None, n_heads: int | None = None) -> QCache:
         """An empty 8-bit cache on the engine's device; by default the engine's slots, its encoder positions and the
         decoder's heads (the shape of one layer's cross cache)."""
-        return QCache.empty(n_slots or self.n_slots, n_tokens or self.dims.n_audio_ctx, n_heads or self.dims.n_text_head,
-                            self.device)
+        return QCache.empty(self.n_slots if n_slots is None else n_slots, self.dims.n_audio_ctx if n_tokens is None else n_tokens,
+                            self.dims.n_text_head if n_heads is None else n_heads, self.device)
 
     # The calls below take a few microseconds on the device, so their checks are written to cost little on the host.
     def _raw_stream(self) -> int:
