@@ -1897,25 +1897,54 @@ int qcache_view(wdz_engine* e, const char* who, const wdz_qcache* c, QcView* v) 
 // How a launch of qcache_attend_kernel is cut: warps to a CTA, CTAs to a cluster, lone CTAs (parts) to an item.
 struct QcAttendPlan { int warps, cluster, parts; };
 
-QcAttendPlan qcache_attend_plan(const wdz_engine* e, int64_t items, int tiles) {
-  QcAttendPlan plan{4, 1, 1};
+// The cut with the shortest estimated time, in microseconds.  What it weighs: CTAs come to an SM whole, so 640 items of
+// 1500 tokens are 4 or 5 to an SM and take 23 us with three warps each (five such CTAs fit), 27 with four (four fit: a second
+// wave) and 26 with two (ten warps do not draw an SM's share of the bandwidth); rows of a few tiles are over before a CTA of
+// four warps has started (7680 items of 128 tokens: 26 us with one warp, 32 with two, 50 with four); few items need
+// clusters (20 items of 1500 tokens: 4.5 us in clusters, 6.5 without).  The constants are fitted to 19 shapes from
+// 80 to 7680 items of 2 to 24 tiles, where the cut it takes is 1 % slower than the best of 4 x 4 on average.
+QcAttendPlan qcache_attend_plan(const wdz_engine* e, int64_t items, int tiles, int pairs) {
+  const double start = 3.0, per_tile = 1.2;              // a CTA's way to its first tile; a warp's time for a tile
+  const double kb = 8.2e-3, warp_rate = 4.0e-3, sm_rate = 52.0e-3, full_rate = 50.0e-3;   // MB a tile; MB a microsecond
   const int64_t sms = e->sm_count;
-  if (items * 4 <= sms * 8) {
-    while (plan.cluster < 8 && items * plan.cluster * 4 < sms * 8 && plan.cluster * 4 < tiles) plan.cluster *= 2;
-    if (plan.cluster == 8 && tiles > 8 * 4 * 4) {
-      // more than four tiles a warp: as many CTAs as the SMs take at four each, every warp with as many tiles as the next
-      int64_t parts = sms * 4 / items;
-      if (parts > QC_MAX_PARTS) parts = QC_MAX_PARTS;
-      const int64_t each = (tiles + 4 * parts - 1) / (4 * parts);
-      parts = (tiles + 4 * each - 1) / (4 * each);
-      if (parts > 8) plan.parts = (int)parts, plan.cluster = 1;
-    }
-  } else if (tiles <= 12) {
-    plan.warps = tiles <= 8 ? 1 : 2;
-  } else if (items > sms * 4 && items <= sms * 5) {
-    plan.warps = 3;
+  if (items > 0 && items * 2 < sms && tiles > 128) {
+    // A few long rows: a cluster leaves SMs idle.  As many lone CTAs as the SMs take at four each, every warp with as many
+    // tiles as the next (8 items of 512 tiles: 13.4 us with the merge, 16.4 in clusters of eight).
+    int64_t parts = sms * 4 / items;
+    if (parts > QC_MAX_PARTS) parts = QC_MAX_PARTS;
+    const int64_t each = (tiles + 4 * parts - 1) / (4 * parts);
+    parts = (tiles + 4 * each - 1) / (4 * each);
+    if (parts > 8) return QcAttendPlan{4, 1, (int)parts};
   }
-  return plan;
+  // Rows of a few tiles in more than a wave of single-warp CTAs: such caches fill up token by token, so most rows are short
+  // (lengths spread over 448 tokens: 40 us against 43 with two warps; all of 512 tokens: 79 against 76).
+  if (tiles <= 8 && pairs == 1 && items > 17 * sms) return QcAttendPlan{1, 1, 1};
+  QcAttendPlan best{4, 1, 1};
+  double least = 1e30;
+  const int even = tiles / 6 < 1 ? 1 : tiles / 6 > 4 ? 4 : tiles / 6;   // where the estimates agree: about six tiles a warp
+  for (int warps = 1; warps <= 4; ++warps) {
+    static const int by_memory[5] = {0, 17, 8, 5, 4};                  // CTAs of an SM by their rings
+    const int by_registers = (pairs == 1 ? 20 : pairs == 2 ? 16 : 11) / warps;
+    const int fit = by_memory[warps] < by_registers ? by_memory[warps] : by_registers;
+    for (int cluster = 1; cluster <= 8; cluster *= 2) {
+      if (cluster > 1 && (cluster - 1) * warps >= tiles) break;       // the last CTA would have no tile
+      const int each = (tiles + cluster - 1) / cluster;
+      const double latency = start + (each + warps - 1) / warps * per_tile;
+      auto wave = [&](double n, double top) {   // n CTAs of each SM at once
+        const double rate = warp_rate * warps * n < top ? warp_rate * warps * n : top, t = n * each * kb / rate;
+        return t > latency ? t : latency;
+      };
+      const int64_t ctas = items * cluster, slots = fit * sms, rest = ctas % slots;
+      double t = (double)(ctas / slots) * wave(fit, full_rate);
+      if (rest) t += wave((double)((rest + sms - 1) / sms), sm_rate);
+      const double memory = (double)items * tiles * 8.2e-3 / 6.9;     // the whole at 6.9 TB/s
+      if (t < memory) t = memory;
+      if (cluster > 1) t += cluster == 2 ? 2.0 : cluster == 4 ? 3.0 : 4.0;
+      t = (t + 2.0) * (1.0 + 0.01 * (warps > even ? warps - even : even - warps));
+      if (t < least) { least = t; best = QcAttendPlan{warps, cluster, 1}; }
+    }
+  }
+  return best;
 }
 
 }  // namespace
@@ -1924,7 +1953,7 @@ int64_t wdz_qcache_attention_scratch(const wdz_engine* e, const wdz_qcache* cach
   if (!e || !cache || n_rows < 0 || cache->n_heads < 1 || cache->n_blocks < 1 || n_q_heads < 1) return WDZ_EINVAL;
   const int group = n_q_heads / cache->n_heads, pairs = group <= 2 ? 1 : group <= 4 ? 2 : 4;
   const int64_t items = (int64_t)n_rows * cache->n_heads;
-  const QcAttendPlan plan = qcache_attend_plan(e, items, cache->n_blocks);
+  const QcAttendPlan plan = qcache_attend_plan(e, items, cache->n_blocks, pairs);
   return plan.parts > 1 ? (int64_t)sizeof(float) * items * plan.parts * 2 * pairs * (QC_HD + 2) : 0;
 }
 
@@ -1999,7 +2028,7 @@ int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_d
   DeviceScope on(e->device);
   const int64_t items = (int64_t)n_rows * p.c.n_heads;
   const int pairs = p.group <= 2 ? 1 : p.group <= 4 ? 2 : 4, step = 2 * pairs * (QC_HD + 2);
-  QcAttendPlan plan = qcache_attend_plan(e, items, p.c.n_blocks);
+  QcAttendPlan plan = qcache_attend_plan(e, items, p.c.n_blocks, pairs);
   if (plan.parts > 1) {
     const size_t need = sizeof(float) * (size_t)items * plan.parts * step;
     if (scratch_dev && scratch_bytes >= need && !((uintptr_t)scratch_dev & 15)) p.part = (float*)scratch_dev;
