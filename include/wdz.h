@@ -338,7 +338,8 @@ int wdz_qcache_store(wdz_engine* e, const wdz_qcache* cache, const void* k_dev, 
                      const int32_t* positions_dev, int n_runs, int max_run, wdz_stream s);
 /* Row r's n_q_heads queries (q_dtype [n_rows][n_q_heads * 64]) attend to the first lens_dev[r] tokens of slot
  * slot_ids_dev[r]: out = softmax(scale * q k^T) v, query head h over key head h / (n_q_heads / n_heads), at most 8
- * query heads to a key head.  fp32 or better throughout; out_dtype [n_rows][n_q_heads * 64].  Lengths are clamped
+ * query heads to a key head.  Queries and softmax weights are held to 2^-31 of the
+ * largest of their head or row, everything else in fp32; out_dtype [n_rows][n_q_heads * 64].  Lengths are clamped
  * to the slot; a row of length 0 gives zeros; a row whose slot is outside [0, n_slots) is left as it was, or
  * zeroed when clear_skipped != 0. */
 int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_dev, int64_t ldq, int q_dtype, int n_q_heads,
@@ -351,7 +352,8 @@ int64_t wdz_qcache_attention_scratch(const wdz_engine* e, const wdz_qcache* cach
  * may be y), W[n][k] = (u - 8) * scale[n][k / group], group 32, 64 or 128.  w_dev: K is padded to Kp, a multiple of
  * 128, with u = 8; row n is Kp / 8 32-bit words; of every 128 weights word 4 t + i (t, i < 4) holds elements
  * 32 i + 8 t + 0..7, element 2 j in its bits 4 j, element 2 j + 1 in its bits 4 (j + 4).  scale_dev: bf16
- * [N][Kp / group].  w_dev starts on 16 bytes, scale_dev on 8; x rows may have any alignment. */
+ * [N][Kp / group].  w_dev starts on 16 bytes, scale_dev on 8; x rows may have any alignment.  Products are exact and
+ * their sums fp32; bf16 rows are held exactly down to 2^-38 of their largest value, to 2^-46 of it below. */
 int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_dtype, int M, int K, const void* w_dev,
                            const void* scale_dev, int group, const void* bias_dev, const float* residual_dev, int N,
                            float* y_dev, wdz_stream s);

@@ -5,7 +5,8 @@ Tolerances, from the arithmetic that the interface promises (u = 2^-24, half a s
   attention  a score is a 64-term fp32 sum: off by at most 70 u scale max|q| sum|k| (that also covers a query held in 23 or
              more bits of its head's largest value); the exponential and the weight's fixed point add 2^-21, the sums of n
              weights n 2^-23, all relative to the largest |v|; a bf16 result is rounded once, 2^-8 of its value.
-  linear     an fp32 sum of K products in any order: (K + 8) u sum|x w|, and as much of the bias and the residual.
+  linear     an fp32 sum of K products in any order: (K + 8) u sum|x w|, and as much of the bias and the residual; bf16 rows
+             are promised to 2^-46 of their largest value, sum|w| of that.
 """
 import numpy as np
 import pytest
@@ -146,6 +147,25 @@ def test_store_extreme_values(eng, dtype, start):
     eng.device_status()                  # reported once
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_store_many_runs(eng, dtype):
+    """Enough units that each belongs to one warp: uneven runs that continue their slots, scales that grow, odd values."""
+    g = torch.Generator().manual_seed(11)
+    runs, heads, blocks = 50, 20, 5
+    lens = torch.randint(1, 201, (runs,), generator=g).tolist()
+    positions = [int(torch.randint(0, 64 * blocks - n + 1, (1,), generator=g)) for n in lens]
+    begin = [0] + np.cumsum(lens).tolist()
+    k, v = ((torch.randn(begin[-1], heads * 64, generator=g) * 4).to(dtype) for _ in range(2))
+    slots = torch.randperm(runs + 1, generator=g)[:runs].tolist()
+    _check_store(eng, _filled(runs + 1, heads, blocks, seed=5), k, v, slots, positions, begin, max_run=200)
+    eng.device_status()
+    k[begin[3], 70], v[begin[20] + 1, 1279], v[begin[30], 0] = float("nan"), float("inf"), float("-inf")
+    v[begin[40]:begin[41]] = 0
+    _check_store(eng, _filled(runs + 1, heads, blocks, seed=5), k, v, slots, positions, begin, max_run=200)
+    with pytest.raises(WdzError):
+        eng.device_status()
+
+
 def test_store_reports_runs_that_it_cannot_place(eng):
     """Positions and rows outside, a slot named twice: the run is left out, its neighbours are stored."""
     g = torch.Generator().manual_seed(3)
@@ -240,8 +260,11 @@ def test_attention_of_peaked_and_flat_rows(eng):
     q[1] *= 1e-6
     q[2] = 0
     q[3, ::7] *= 300
-    for scale in (0.125, 1.0, 0.0):
-        _check_attend(eng, parts, q, [0, 1, 2, 3, 4, 5], [192, 192, 100, 192, 5, 64], scale=scale)
+    q[4] *= 1e-34
+    q[5, 3] = 3e30
+    for scale in (0.125, 1.0, 0.0, 1e-30):
+        n = 6 if scale < 0.1 else 5          # the query of 3e30 only where its scores stay in range
+        _check_attend(eng, parts, q[:n], [0, 1, 2, 3, 4, 5][:n], [192, 192, 100, 192, 5, 64][:n], scale=scale)
 
 
 def test_attention_rows_of_one_slot_and_clamped_lengths(eng):
@@ -377,6 +400,8 @@ def _check_linear(eng, x, packed, w, b, residual=None, out=None):
     got = eng.linear_rows_packed(x.cuda(), packed, residual=residual, out=out)
     g = got.double().cpu().numpy()
     tol = (x.shape[1] + 8) * U * size
+    if x.dtype == BF16:   # one or two rows are held in whole numbers of 2^(e - 45), e the exponent of the row's largest value:
+        tol = tol + 2.0 ** -46 * np.abs(x64).max(1, keepdims=True, initial=0) * np.abs(w).sum(1)   # half a unit each, 2^-46 of it at most
     assert got.dtype == F32 and g.shape == want.shape
     assert (np.abs(g - want) <= tol).all(), float((np.abs(g - want) / np.maximum(tol, 1e-30)).max())
     assert np.linalg.norm(g - want) <= 1e-5 * max(np.linalg.norm(want), 1e-30)
@@ -426,7 +451,10 @@ def test_linear_rows_at_any_alignment(eng, k, dtype):
 def test_linear_range_and_nan(eng, dtype):
     """Rows of very different sizes, rows of zeros, and NaN and infinity that stay in their row."""
     packed, w, b = _packed(64, 384, 64, seed=5)
-    x = torch.randn(6, 384, generator=torch.Generator().manual_seed(3))
+    x = torch.randn(8, 384, generator=torch.Generator().manual_seed(3))
+    x[6] *= 1e-33
+    x[7] *= 1e-30
+    x[7, 5] = 2e30
     x[0] *= 1e-20
     x[1] *= 1e20
     x[2] = 0
@@ -435,12 +463,25 @@ def test_linear_range_and_nan(eng, dtype):
     got = _check_linear(eng, x[:3], packed, w, b), _check_linear(eng, x[3:], packed, w, b)
     both = eng.linear_rows_packed(x.cuda(), packed)
     assert torch.equal(both[:3], got[0]) and torch.equal(both[3:], got[1])
+    for i in range(8):                   # one and two rows go another way
+        _check_linear(eng, x[i:i + 1], packed, w, b)
+        if i < 7:
+            _check_linear(eng, x[i:i + 2], packed, w, b)
     x[1, 100], x[4, 0] = float("nan"), float("inf")
     bad = eng.linear_rows_packed(x.cuda(), packed)
     assert bad[1].isnan().all()
     assert (~bad[4].isfinite()).all()
-    keep = [0, 2, 3, 5]
+    keep = [0, 2, 3, 5, 6, 7]
     assert torch.equal(bad[keep], both[keep])
+    for one, other in ((1, 0), (4, 5)):
+        pair = eng.linear_rows_packed(x[[one, other]].cuda(), packed)
+        assert (~pair[0].isfinite()).all() and torch.equal(pair[1], eng.linear_rows_packed(x[[other]].cuda(), packed)[0])
+
+
+def test_pack_linear_on_the_device_is_the_same(eng):
+    w = torch.randn(40, 333, generator=torch.Generator().manual_seed(0))
+    a, b = pack_linear(w, 64), pack_linear(w.cuda(), 64)
+    assert torch.equal(a.weight, b.weight.cpu()) and torch.equal(a.scale, b.scale.cpu())
 
 
 def test_linear_from_packed_weights_is_near_the_weights(eng):

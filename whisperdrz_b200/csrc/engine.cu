@@ -1117,8 +1117,9 @@ int wdz_finalize(wdz_engine* e) {
     auto allow = [&](auto kern, int bytes) {
       if (ce4 == cudaSuccess) ce4 = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     };
-    allow(gemv_packed_s8_kernel<1>, GP_S8_CHUNK * 1024); allow(gemv_packed_s8_kernel<2>, GP_S8_CHUNK * 1024);
-    allow(gemv_packed_s8_kernel<4>, GP_S8_CHUNK * 1024);
+    allow(gemv_packed_s8_kernel<1, 1>, GP_S8_CHUNK<1> * 1024); allow(gemv_packed_s8_kernel<1, 2>, GP_S8_CHUNK<1> * 1024);
+    allow(gemv_packed_s8_kernel<1, 4>, GP_S8_CHUNK<1> * 1024); allow(gemv_packed_s8_kernel<2, 1>, GP_S8_CHUNK<2> * 2048);
+    allow(gemv_packed_s8_kernel<2, 2>, GP_S8_CHUNK<2> * 2048); allow(gemv_packed_s8_kernel<2, 4>, GP_S8_CHUNK<2> * 2048);
     allow(gemv_packed_f32_kernel<1, 1>, GP_F32_CHUNK<1> * 2048); allow(gemv_packed_f32_kernel<1, 2>, GP_F32_CHUNK<1> * 2048);
     allow(gemv_packed_f32_kernel<1, 4>, GP_F32_CHUNK<1> * 2048);
     allow(gemv_packed_f32_kernel<4, 1>, GP_F32_CHUNK<4> * 8192); allow(gemv_packed_f32_kernel<4, 2>, GP_F32_CHUNK<4> * 8192);
@@ -2120,8 +2121,10 @@ int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_
     by_group([&](auto gs) { go(gemv_packed_f32_kernel<1, decltype(gs)::value>, 2, held(GP_F32_CHUNK<1>) * 2048); });
   } else if (x_dtype == WDZ_F32) {
     by_group([&](auto gs) { go(gemv_packed_f32_kernel<4, decltype(gs)::value>, 8, held(GP_F32_CHUNK<4>) * 4 * 2048); });
-  } else if (M <= GP_S8_ROWS) {
-    by_group([&](auto gs) { go(gemv_packed_s8_kernel<decltype(gs)::value>, GP_S8_ROWS, held(GP_S8_CHUNK) * 1024); });
+  } else if (M == 1) {
+    by_group([&](auto gs) { go(gemv_packed_s8_kernel<1, decltype(gs)::value>, 1, held(GP_S8_CHUNK<1>) * 1024); });
+  } else if (M == 2) {
+    by_group([&](auto gs) { go(gemv_packed_s8_kernel<2, decltype(gs)::value>, 2, held(GP_S8_CHUNK<2>) * 2048); });
   } else if (M <= 8) {
     by_group([&](auto gs) { go(gemv_packed_bf16_kernel<1, decltype(gs)::value>, 8, 0); });
   } else {

@@ -11,8 +11,8 @@
 //
 //   gemv_packed_s8_kernel    bf16 rows, up to two.  m16n8k32 on bytes: a word becomes two operands with three
 //       instructions (a nibble in a byte's upper half is 16 times a signed weight).  x is written as a whole number of
-//       32 bits times a scale of its row, four signed bytes that take four columns: exact for values down to 2^-23 of the
-//       row's largest, off by at most 2^-32 of that below.  Sums of products of bytes are exact.
+//       48 bits times a power of two of its row, six signed bytes that take six columns: exact for values down to 2^-38 of
+//       the row's largest, off by at most 2^-46 of that below.  Sums of products of bytes are exact.
 //   gemv_packed_bf16_kernel  bf16 rows, three and more.  m16n8k16 on bf16: a row is one column, taken as it lies.  A word
 //       becomes four pairs of bf16 with a shift, a mask and one fused add each: bits u placed under the exponent of 128
 //       are 128 + u, minus 136 is the weight, exactly.
@@ -134,8 +134,8 @@ __device__ __forceinline__ void gp_finish(const GemvPackedParams& p, const float
   }
 }
 
-constexpr float GP_S8_STEPS = 127.0f * 16777216.0f;   // a row's largest value in steps: rounding up leaves its top byte a byte
-constexpr int GP_S8_ROWS = 2, GP_S8_CHUNK = 64;       // rows of a CTA, segments of x that one pass keeps in shared memory (64 KB)
+// The byte kernel: segments of x that one pass keeps in shared memory (64 KB).
+template <int ROWS> constexpr int GP_S8_CHUNK = ROWS == 1 ? 64 : 32;
 template <int PAIRS> constexpr int GP_F32_CHUNK = PAIRS == 1 ? 40 : 10;   // the same (80 KB)
 
 // The upper nibbles u of four bytes as 16 (u - 8): one instruction with both masks in registers.
@@ -145,29 +145,32 @@ __device__ __forceinline__ uint32_t gp_signed16(uint32_t w, uint32_t flip, uint3
   return r;
 }
 
-// Block = 8 warps; grid = (tiles of 16 features x split / 8, rows / 2).  GS: scales of a segment of 128 weights.
-template <int GS>
+// Block = 8 warps; grid = tiles of 16 features x split / 8.  ROWS = M, 1 or 2.  GS: scales of a segment of 128 weights.
+template <int ROWS, int GS>
 __global__ void __launch_bounds__(GP_WARPS * 32, 3) gemv_packed_s8_kernel(GemvPackedParams p) {
-  extern __shared__ __align__(16) uint2 xs[];   // [segment][i][lane]: a lane's two operand words
-  __shared__ float red[GP_WARPS][GP_S8_ROWS][17];
-  __shared__ float tops[GP_WARPS][GP_S8_ROWS];
+  extern __shared__ __align__(16) uint2 xs[];   // [segment][row][i][lane]: a lane's two operand words
+  __shared__ float red[GP_WARPS][ROWS][17];
+  __shared__ float tops[GP_WARPS][ROWS];
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int part = warp & (p.split - 1), tile = blockIdx.x * (GP_WARPS >> p.split_log) + (warp >> p.split_log);
-  const int m0 = blockIdx.y * GP_S8_ROWS, segs = p.Kp >> 7, rows = min(GP_S8_ROWS, p.M - m0);
+  const int segs = p.Kp >> 7;
   const int na = min(tile * 16 + g, p.N - 1), nb = min(tile * 16 + g + 8, p.N - 1);
   const uint4* wa = reinterpret_cast<const uint4*>(p.W + (int64_t)na * (p.Kp >> 3)) + t;   // a segment is four uint4
   const uint4* wb = reinterpret_cast<const uint4*>(p.W + (int64_t)nb * (p.Kp >> 3)) + t;
   const bf16* sa = p.scale + (int64_t)na * segs * GS;
   const bf16* sb = p.scale + (int64_t)nb * segs * GS;
-  const bf16* x = reinterpret_cast<const bf16*>(p.x) + (int64_t)m0 * p.ldx;
+  const bf16* x = reinterpret_cast<const bf16*>(p.x);
   pdl_wait();
 
-  float sum[2] = {0.0f, 0.0f};
-  const uint32_t xs_at = (uint32_t)__cvta_generic_to_shared(xs);
-  const uint32_t xs_mine = xs_at + 8 * ((rows == 1 ? lane & 15 : lane));   // a lone row's columns twice: no column is empty
-  for (int first = 0; first < segs; first += GP_S8_CHUNK) {
-    const int here = min(GP_S8_CHUNK, segs - first);
+  float sum[ROWS][2];
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m) sum[m][0] = sum[m][1] = 0.0f;
+  // columns 6 and 7 take the operands of 4 and 5 once more; what they give is left out below
+  const uint32_t xs_mine = (uint32_t)__cvta_generic_to_shared(xs) + 8 * ((g < 6 ? g : g - 2) * 4 + t);
+  constexpr int CHUNK = GP_S8_CHUNK<ROWS>;
+  for (int first = 0; first < segs; first += CHUNK) {
+    const int here = min(CHUNK, segs - first);
     const int n = part < here ? (here - part + p.split - 1) >> p.split_log : 0;   // segments of this warp
     uint4 a[GP_AHEAD], b[GP_AHEAD];
     GpScale<GS> fa[GP_AHEAD], fb[GP_AHEAD];
@@ -183,59 +186,65 @@ __global__ void __launch_bounds__(GP_WARPS * 32, 3) gemv_packed_s8_kernel(GemvPa
 
     // largest value of each row, 8 values a thread and step
     const int units = here * 16;
-    float top[GP_S8_ROWS];
+    float top[ROWS];
 #pragma unroll
-    for (int m = 0; m < GP_S8_ROWS; ++m) {
+    for (int m = 0; m < ROWS; ++m) {
       top[m] = 0.0f;
-      if (m < rows)
-        for (int i = threadIdx.x; i < units; i += GP_WARPS * 32) {
-          float v[8];
-          gp_row8(x + (int64_t)m * p.ldx, first * 128 + 8 * i, p.K, p.vec, v);
+      for (int i = threadIdx.x; i < units; i += GP_WARPS * 32) {
+        float v[8];
+        gp_row8(x + m * p.ldx, first * 128 + 8 * i, p.K, p.vec, v);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) top[m] = fabsf(v[j]) <= 3.402823466e38f ? fmaxf(top[m], fabsf(v[j])) : INFINITY;
-        }
+        for (int j = 0; j < 8; ++j) top[m] = fabsf(v[j]) <= 3.402823466e38f ? fmaxf(top[m], fabsf(v[j])) : INFINITY;
+      }
     }
     __syncthreads();   // the pass before has read xs and tops
 #pragma unroll
-    for (int m = 0; m < GP_S8_ROWS; ++m) {
+    for (int m = 0; m < ROWS; ++m) {
       top[m] = warp_max(top[m]);
       if (lane == 0) tops[warp][m] = top[m];
     }
     __syncthreads();
 #pragma unroll
-    for (int m = 0; m < GP_S8_ROWS; ++m) {
+    for (int m = 0; m < ROWS; ++m) {
 #pragma unroll
       for (int w = 0; w < GP_WARPS; ++w) top[m] = fmaxf(top[m], tops[w][m]);
-      if (m < rows) {
-        const float lift = top[m] < 1e-20f ? 18446744073709551616.0f : 1.0f;   // 2^64: keeps the quotient finite
-        const float steps = top[m] > 0.0f ? GP_S8_STEPS / (top[m] * lift) * lift : 0.0f;
-        for (int i = threadIdx.x; i < units; i += GP_WARPS * 32) {
-          float v[8];
-          gp_row8(x + (int64_t)m * p.ldx, first * 128 + 8 * i, p.K, p.vec, v);
-          // unit = word i of lane tt of a segment; the bytes' lower nibbles are elements 0 4 1 5, the upper 2 6 3 7
-          const int sg = i >> 4, wi = i & 15, at = wi >> 2, tt = wi & 3;
-          uint32_t n[8];
+      // x in units of 2^(e - 45), e the exponent of the largest: whole numbers below 2^46, exact down to 2^(e - 38)
+      const int e = max((int)(__float_as_uint(top[m]) >> 23), 1) - 127;
+      const double unit = top[m] < INFINITY ? __hiloint2double((1023 + 45 - e) << 20, 0) : 0.0;
+      for (int i = threadIdx.x; i < units; i += GP_WARPS * 32) {
+        float v[8];
+        gp_row8(x + m * p.ldx, first * 128 + 8 * i, p.K, p.vec, v);
+        // i = word of lane tt of a segment; the bytes' lower nibbles are elements 0 4 1 5, the upper 2 6 3 7
+        const int sg = i >> 4, wi = i & 15, at = wi >> 2, tt = wi & 3;
+        uint32_t lo[8], hi[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) n[j] = (uint32_t)__float2int_rn(v[j] * steps) + 0x80808080u;   // bytes + 128
-          uint2 d[4];   // columns d1, d0, d3, d2
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t e0 = n[2 * h], e1 = n[2 * h + 4], e2 = n[2 * h + 1], e3 = n[2 * h + 5];
-            const uint32_t x01 = __byte_perm(e0, e1, 0x5140), x23 = __byte_perm(e2, e3, 0x5140);
-            const uint32_t y01 = __byte_perm(e0, e1, 0x7362), y23 = __byte_perm(e2, e3, 0x7362);
-            (h ? d[0].y : d[0].x) = __byte_perm(x01, x23, 0x7632) ^ 0x80808080u;
-            (h ? d[1].y : d[1].x) = __byte_perm(x01, x23, 0x5410) ^ 0x80808080u;
-            (h ? d[2].y : d[2].x) = __byte_perm(y01, y23, 0x7632) ^ 0x80808080u;
-            (h ? d[3].y : d[3].x) = __byte_perm(y01, y23, 0x5410) ^ 0x80808080u;
-          }
-#pragma unroll
-          for (int q = 0; q < 4; ++q) xs[(sg * 4 + at) * 32 + (m * 4 + q) * 4 + tt] = d[q];
+        for (int j = 0; j < 8; ++j) {
+          const uint64_t w = unit > 0.0 ? (uint64_t)__double2ll_rn((double)v[j] * unit) + 0x808080808080ull : 0x808080808080ull;   // bytes + 128
+          lo[j] = (uint32_t)w; hi[j] = (uint32_t)(w >> 32);
         }
+        uint2 d[6];   // columns d1, d0, d3, d2, d5, d4
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int e0 = 2 * h, e1 = 2 * h + 4, e2 = 2 * h + 1, e3 = 2 * h + 5;
+          const uint32_t x01 = __byte_perm(lo[e0], lo[e1], 0x5140), x23 = __byte_perm(lo[e2], lo[e3], 0x5140);
+          const uint32_t y01 = __byte_perm(lo[e0], lo[e1], 0x7362), y23 = __byte_perm(lo[e2], lo[e3], 0x7362);
+          const uint32_t z01 = __byte_perm(hi[e0], hi[e1], 0x5140), z23 = __byte_perm(hi[e2], hi[e3], 0x5140);
+          (h ? d[0].y : d[0].x) = __byte_perm(x01, x23, 0x7632) ^ 0x80808080u;
+          (h ? d[1].y : d[1].x) = __byte_perm(x01, x23, 0x5410) ^ 0x80808080u;
+          (h ? d[2].y : d[2].x) = __byte_perm(y01, y23, 0x7632) ^ 0x80808080u;
+          (h ? d[3].y : d[3].x) = __byte_perm(y01, y23, 0x5410) ^ 0x80808080u;
+          (h ? d[4].y : d[4].x) = __byte_perm(z01, z23, 0x7632) ^ 0x80808080u;
+          (h ? d[5].y : d[5].x) = __byte_perm(z01, z23, 0x5410) ^ 0x80808080u;
+        }
+#pragma unroll
+        for (int q = 0; q < 6; ++q) xs[((sg * ROWS + m) * 4 + at) * 32 + q * 4 + tt] = d[q];
       }
     }
     __syncthreads();
 
-    float acc[2] = {0.0f, 0.0f};
+    float acc[ROWS][2];
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m) acc[m][0] = acc[m][1] = 0.0f;
     uint32_t flip = 0x80808080u, keep = 0xf0f0f0f0u;
     asm volatile("" : "+r"(flip), "+r"(keep));   // known to nobody: they stay in registers
     for (int j = 0; j < n; j += GP_AHEAD) {
@@ -255,33 +264,44 @@ __global__ void __launch_bounds__(GP_WARPS * 32, 3) gemv_packed_s8_kernel(GemvPa
 #pragma unroll
         for (int i = 0; i < GS; ++i) { sa_g[i] = fa[u].get(i); sb_g[i] = fb[u].get(i); }
         if (j + u + GP_AHEAD < n) fetch(u, j + u + GP_AHEAD);
-        const uint32_t xq = xs_mine + ((part + ((j + u) << p.split_log)) << 10);
-        int c[4];
+        const uint32_t xq = xs_mine + (part + ((j + u) << p.split_log)) * (ROWS * 1024);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint2 xb;
-          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(xb.x), "=r"(xb.y) : "r"(xq + 256 * i));
-          if (i % (4 / GS) == 0) mma_s8_16832_first(c, op[i][0], op[i][1], op[i][2], op[i][3], xb.x, xb.y);
-          else mma_s8_16832(c, op[i][0], op[i][1], op[i][2], op[i][3], xb.x, xb.y);
-          if ((i + 1) % (4 / GS) == 0) {   // the end of a group: columns (d1, d0) or (d3, d2) fold into one number
-            acc[0] = fmaf((float)(c[0] * 256 + c[1]), sa_g[i / (4 / GS)], acc[0]);
-            acc[1] = fmaf((float)(c[2] * 256 + c[3]), sb_g[i / (4 / GS)], acc[1]);
+        for (int m = 0; m < ROWS; ++m) {
+          int c[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint2 xb;
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(xb.x), "=r"(xb.y) : "r"(xq + 1024 * m + 256 * i) : "memory");
+            if (i % (4 / GS) == 0) mma_s8_16832_first(c, op[i][0], op[i][1], op[i][2], op[i][3], xb.x, xb.y);
+            else mma_s8_16832(c, op[i][0], op[i][1], op[i][2], op[i][3], xb.x, xb.y);
+            if ((i + 1) % (4 / GS) == 0) {   // the end of a group: columns (d1, d0), (d3, d2) or (d5, d4) fold into one number
+              acc[m][0] = fmaf((float)(c[0] * 256 + c[1]), sa_g[i / (4 / GS)], acc[m][0]);
+              acc[m][1] = fmaf((float)(c[2] * 256 + c[3]), sb_g[i / (4 / GS)], acc[m][1]);
+            }
           }
         }
       }
     }
-    // a step of the row, / 16 for the shifted nibble; an infinite or NaN row: infinity times zero is NaN
-    const float step = (t >> 1 && rows > 1 ? top[1] : top[0]) * (1.0f / (16.0f * GP_S8_STEPS)) * (t & 1 ? 65536.0f : 1.0f);
-    sum[0] = fmaf(acc[0], step, sum[0]);
-    sum[1] = fmaf(acc[1], step, sum[1]);
+    // times 2^-45 of the unit, 2^-4 of the shifted nibble and the column's 2^16 t; the row's own size last, so that nothing
+    // underflows before the result does.  An infinite or NaN row: infinity times zero is NaN.
+    const float column = t == 0 ? 1.7763568394002505e-15f : t == 1 ? 1.1641532182693481e-10f : t == 2 ? 7.62939453125e-6f : 0.0f;
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m) {
+      const float size = top[m] < INFINITY ? ldexpf(1.0f, max((int)(__float_as_uint(top[m]) >> 23), 1) - 127) : INFINITY;
+      sum[m][0] = fmaf(acc[m][0] * column, size, sum[m][0]);
+      sum[m][1] = fmaf(acc[m][1] * column, size, sum[m][1]);
+    }
   }
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const float v = sum[h] + __shfl_xor_sync(0xffffffffu, sum[h], 1);
-    if (!(t & 1)) red[warp][t >> 1][g + 8 * h] = v;
-  }
+  for (int m = 0; m < ROWS; ++m)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float v = sum[m][h] + __shfl_xor_sync(0xffffffffu, sum[m][h], 1);
+      v += __shfl_xor_sync(0xffffffffu, v, 2);
+      if (t == 0) red[warp][m][g + 8 * h] = v;
+    }
   __syncthreads();
-  gp_finish<bf16>(p, red, m0);
+  gp_finish<bf16>(p, red, 0);
 }
 
 // PAIRS: pairs of rows a CTA takes.  Block = 8 warps; grid = (tiles of 16 features x split / 8, rows / (2 PAIRS)).

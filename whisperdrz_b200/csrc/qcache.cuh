@@ -593,13 +593,13 @@ __device__ __forceinline__ void qc_query(const QcAttendParams& p, int r, int hk,
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const float lift = top < 1e-20f ? 18446744073709551616.0f : 1.0f;   // 2^64: keeps the quotient below finite
-    const float steps = top > 0.0f ? QC_STEPS / (top * lift) * lift : 0.0f;
+    const float steps = top > 0.0f ? QC_STEPS / (top * lift) : 0.0f;
     const uint32_t digit = ((g & 3) ^ 1) * 0x11 + 0x40;   // columns d1, d0, d3, d2: that byte of two numbers
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       uint32_t n[4];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) n[b] = (uint32_t)__float2int_rn(x[4 * w + b] * steps) + 0x80808080u;   // digits + 128
+      for (int b = 0; b < 4; ++b) n[b] = (uint32_t)__float2int_rn(x[4 * w + b] * lift * steps) + 0x80808080u;   // digits + 128
       qb[nt][w] = __byte_perm(__byte_perm(n[0], n[1], digit), __byte_perm(n[2], n[3], digit), 0x5410) ^ 0x80808080u;
     }
     // an infinite or NaN query: infinity times zero makes the row NaN
