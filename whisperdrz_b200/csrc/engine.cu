@@ -1120,10 +1120,12 @@ int wdz_finalize(wdz_engine* e) {
     allow(gemv_packed_s8_kernel<1, 1>, GP_S8_CHUNK<1> * 1024); allow(gemv_packed_s8_kernel<1, 2>, GP_S8_CHUNK<1> * 1024);
     allow(gemv_packed_s8_kernel<1, 4>, GP_S8_CHUNK<1> * 1024); allow(gemv_packed_s8_kernel<2, 1>, GP_S8_CHUNK<2> * 2048);
     allow(gemv_packed_s8_kernel<2, 2>, GP_S8_CHUNK<2> * 2048); allow(gemv_packed_s8_kernel<2, 4>, GP_S8_CHUNK<2> * 2048);
-    allow(gemv_packed_f32_kernel<1, 1>, GP_F32_CHUNK<1> * 2048); allow(gemv_packed_f32_kernel<1, 2>, GP_F32_CHUNK<1> * 2048);
-    allow(gemv_packed_f32_kernel<1, 4>, GP_F32_CHUNK<1> * 2048);
-    allow(gemv_packed_f32_kernel<4, 1>, GP_F32_CHUNK<4> * 8192); allow(gemv_packed_f32_kernel<4, 2>, GP_F32_CHUNK<4> * 8192);
-    allow(gemv_packed_f32_kernel<4, 4>, GP_F32_CHUNK<4> * 8192);
+    allow(gemv_packed_mma_kernel<float, 1, 1>, 200 * 1024); allow(gemv_packed_mma_kernel<float, 1, 2>, 200 * 1024);
+    allow(gemv_packed_mma_kernel<float, 1, 4>, 200 * 1024); allow(gemv_packed_mma_kernel<float, 4, 1>, 200 * 1024);
+    allow(gemv_packed_mma_kernel<float, 4, 2>, 200 * 1024); allow(gemv_packed_mma_kernel<float, 4, 4>, 200 * 1024);
+    allow(gemv_packed_mma_kernel<bf16, 1, 1>, 200 * 1024); allow(gemv_packed_mma_kernel<bf16, 1, 2>, 200 * 1024);
+    allow(gemv_packed_mma_kernel<bf16, 1, 4>, 200 * 1024); allow(gemv_packed_mma_kernel<bf16, 2, 1>, 200 * 1024);
+    allow(gemv_packed_mma_kernel<bf16, 2, 2>, 200 * 1024); allow(gemv_packed_mma_kernel<bf16, 2, 4>, 200 * 1024);
     // CTAs of a few warps that share an SM by their shared memory: always the largest part of it
     auto share = [&](auto kern) {
       if (ce4 == cudaSuccess) ce4 = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
@@ -1995,7 +1997,7 @@ int wdz_qcache_store(wdz_engine* e, const wdz_qcache* cache, const void* k_dev, 
   // 15.4; 32 windows of 1500 tokens, 32000 units, 93 us against 67 with one warp).
   const bool few = (int64_t)blocks * 2 * p.c.n_heads * n_runs < 64ll * e->sm_count;
   const int warps = few ? 4 : 2, held = few ? 1 : 2;   // units of a CTA
-  const dim3 grid(blocks, (2 * p.c.n_heads + held - 1) / held, n_runs);
+  const dim3 grid(blocks, 2 * p.c.n_heads / held, n_runs);
   auto go = [&](auto kern, int unit_bytes) { launch_pdl(e, kern, grid, dim3(32 * warps), held * unit_bytes, (cudaStream_t)s, p, e->status); };
   if (dtype == WDZ_BF16) { if (few) go(qcache_store_kernel<bf16, 4>, QC_UNIT<bf16>); else go(qcache_store_kernel<bf16, 1>, QC_UNIT<bf16>); }
   else { if (few) go(qcache_store_kernel<float, 4>, QC_UNIT<float>); else go(qcache_store_kernel<float, 1>, QC_UNIT<float>); }
@@ -2117,19 +2119,24 @@ int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_
     else run(std::integral_constant<int, 1>());
   };
   auto held = [&](int chunk) { return (size_t)(segs < chunk ? segs : chunk); };   // segments of x in shared memory
-  if (x_dtype == WDZ_F32 && M <= 2) {
-    by_group([&](auto gs) { go(gemv_packed_f32_kernel<1, decltype(gs)::value>, 2, held(GP_F32_CHUNK<1>) * 2048); });
-  } else if (x_dtype == WDZ_F32) {
-    by_group([&](auto gs) { go(gemv_packed_f32_kernel<4, decltype(gs)::value>, 8, held(GP_F32_CHUNK<4>) * 4 * 2048); });
-  } else if (M == 1) {
-    by_group([&](auto gs) { go(gemv_packed_s8_kernel<1, decltype(gs)::value>, 1, held(GP_S8_CHUNK<1>) * 1024); });
-  } else if (M == 2) {
-    by_group([&](auto gs) { go(gemv_packed_s8_kernel<2, decltype(gs)::value>, 2, held(GP_S8_CHUNK<2>) * 2048); });
-  } else if (M <= 8) {
-    by_group([&](auto gs) { go(gemv_packed_bf16_kernel<1, decltype(gs)::value>, 8, 0); });
-  } else {
-    by_group([&](auto gs) { go(gemv_packed_bf16_kernel<2, decltype(gs)::value>, 16, 0); });
-  }
+  auto mma = [&](auto tx, auto tiles_c, auto gs) {
+    using T = decltype(tx);
+    constexpr int TILES = decltype(tiles_c)::value;
+    // x in one pass where every SM has a CTA at most; otherwise no more than lets two or three share an SM
+    const int rows = TILES * GP_TILE_ROWS<T>, per = GP_WARPS / p.split;
+    const bool alone = (int64_t)((tiles + per - 1) / per) * ((M + rows - 1) / rows) <= e->sm_count;
+    p.chunk = (alone ? 200 : TILES == 1 ? 64 : 80) / (2 * TILES);
+    go(gemv_packed_mma_kernel<T, TILES, decltype(gs)::value>, rows, held(p.chunk) * TILES * 2048);
+  };
+  using one = std::integral_constant<int, 1>;
+  using two = std::integral_constant<int, 2>;
+  using four = std::integral_constant<int, 4>;
+  // Two rows and fewer in bf16 leave six of a tile's columns empty: there bytes are cheaper (one row over 51866 features 9 us
+  // against 11 to 12 on bf16 operands).
+  if (x_dtype == WDZ_F32) by_group([&](auto gs) { if (M <= 2) mma(0.0f, one(), gs); else mma(0.0f, four(), gs); });
+  else if (M == 1) by_group([&](auto gs) { go(gemv_packed_s8_kernel<1, decltype(gs)::value>, 1, held(GP_S8_CHUNK<1>) * 1024); });
+  else if (M == 2) by_group([&](auto gs) { go(gemv_packed_s8_kernel<2, decltype(gs)::value>, 2, held(GP_S8_CHUNK<2>) * 2048); });
+  else by_group([&](auto gs) { if (M <= 8) mma(bf16(), one(), gs); else mma(bf16(), two(), gs); });
   e->span_end(sp, (cudaStream_t)s);
   WDZ_LAUNCH_CHECK(e, "gemv_packed");
   return WDZ_OK;

@@ -13,11 +13,9 @@
 //       instructions (a nibble in a byte's upper half is 16 times a signed weight).  x is written as a whole number of
 //       48 bits times a power of two of its row, six signed bytes that take six columns: exact for values down to 2^-38 of
 //       the row's largest, off by at most 2^-46 of that below.  Sums of products of bytes are exact.
-//   gemv_packed_bf16_kernel  bf16 rows, three and more.  m16n8k16 on bf16: a row is one column, taken as it lies.  A word
-//       becomes four pairs of bf16 with a shift, a mask and one fused add each: bits u placed under the exponent of 128
-//       are 128 + u, minus 136 is the weight, exactly.
-//   gemv_packed_f32_kernel   f32 rows: the same, a row cut into three bf16 pieces (8 + 8 + 8 bits) that add up to it and
-//       take three columns; whole numbers would not do for rows whose largest value is far above the rest.
+//   gemv_packed_mma_kernel   all others.  m16n8k16 on bf16.  A word becomes four pairs of bf16 with a shift, a mask and one
+//       fused add each: bits u placed under the exponent of 128 are 128 + u, minus 136 is the weight, exactly.  A bf16 row
+//       is one column, as it is; an f32 row is cut into three bf16 pieces (8 + 8 + 8 bits) that add up to it and take three.
 // Either way a group's sum is multiplied by its scale in fp32.
 //
 // Measured (B200, device time): one bf16 row, 1280 x 1280 2.9 us (a launch's latency; the weights' bytes alone 0.13); one row
@@ -39,6 +37,7 @@ struct GemvPackedParams {
   int M, N, K, Kp, group;
   int split, split_log;    // warps that share a tile of 16 features: 1, 2, 4 or 8
   bool vec;                // rows of x can be read in pieces of eight
+  int chunk;               // segments of x that one pass of gemv_packed_mma_kernel keeps in shared memory
 };
 
 constexpr int GP_WARPS = 8;
@@ -55,13 +54,21 @@ __device__ __forceinline__ void mma_s8_16832_first(int (&c)[4], uint32_t a0, uin
                : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 
-// One 32-bit word of weights -> pairs (element 2 j, element 2 j + 1), j = 0..3, as bf16.
-__device__ __forceinline__ void gp_unpack(uint32_t w, uint32_t (&r)[4]) {
+// bf16 product whose accumulator starts from zeros.
+__device__ __forceinline__ void mma_bf16_16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// One 32-bit word of weights -> pairs (element 2 j, element 2 j + 1), j = 0..3, as bf16.  low = 0x000f000f, base = 128 twice:
+// both in registers, so that mask and exponent are one instruction.
+__device__ __forceinline__ void gp_unpack(uint32_t w, uint32_t low, uint32_t base, uint32_t (&r)[4]) {
   const __nv_bfloat162 off = __halves2bfloat162(__float2bfloat16_rn(-136.0f), __float2bfloat16_rn(-136.0f));
   const __nv_bfloat162 one = __halves2bfloat162(__float2bfloat16_rn(1.0f), __float2bfloat16_rn(1.0f));
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t u = ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u;
+    uint32_t u;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(u) : "r"(w >> (4 * j)), "r"(low), "r"(base));   // (w & low) | base
     const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&u), one, off);
     r[j] = *reinterpret_cast<const uint32_t*>(&v);
   }
@@ -74,14 +81,19 @@ __device__ __forceinline__ uint4 gp_row(const bf16* row, int k0, int K, bool vec
     if (k0 < K) v = *reinterpret_cast<const uint4*>(row + k0);   // plain loads: the kernel before may have written x
     return v;
   }
-  const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
-  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+  // rows at any two bytes: the words that hold the values, shifted by half a word where they start in the middle of one.
+  // A word is only read where a value of the row lies in it, so it lies in the row's allocation.
+  const uint32_t half = (uint32_t)((uintptr_t)(row + k0) & 2) >> 1;
+  const uint32_t* w = reinterpret_cast<const uint32_t*>((uintptr_t)(row + k0) & ~(uintptr_t)3);
+  uint32_t in[5], out[4];
+#pragma unroll
+  for (int j = 0; j < 5; ++j) in[j] = k0 + 2 * j - (int)half < K && (j < 4 || half) && k0 < K ? w[j] : 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t lo = k0 + 2 * j < K ? r[k0 + 2 * j] : 0, hi = k0 + 2 * j + 1 < K ? r[k0 + 2 * j + 1] : 0;
-    w[j] = lo | hi << 16;
+    out[j] = half ? __funnelshift_r(in[j], in[j + 1], 16) : in[j];
+    if (k0 + 2 * j + 1 >= K) out[j] = k0 + 2 * j < K ? out[j] & 0xffffu : 0;
   }
-  return v;
+  return make_uint4(out[0], out[1], out[2], out[3]);
 }
 __device__ __forceinline__ void gp_row8(const bf16* row, int k0, int K, bool vec, float (&v)[8]) {
   const uint4 u = gp_row(row, k0, K, vec);
@@ -122,21 +134,30 @@ template <> struct GpScale<4> {
 template <typename T, int ROWS>
 __device__ __forceinline__ void gp_finish(const GemvPackedParams& p, const float (&red)[GP_WARPS][ROWS][17], int m0) {
   const int rows = min(ROWS, p.M - m0), shift = 7 - p.split_log, cols = 1 << shift, n_first = blockIdx.x << shift;
-  for (int i = threadIdx.x; i < rows << shift; i += GP_WARPS * 32) {
-    const int row = i >> shift, col = i & (cols - 1), n = n_first + col;
-    if (n >= p.N) continue;
-    const int64_t at = (int64_t)(m0 + row) * p.N + n;
-    float v = p.residual ? p.residual[at] : 0.0f;
-    if (p.bias) v += to_f(reinterpret_cast<const T*>(p.bias)[n]);
-    float sum = 0.0f;
-    for (int w = 0; w < p.split; ++w) sum += red[((col >> 4) << p.split_log) + w][row][col & 15];
-    p.y[at] = v + sum;
+  for (int i0 = threadIdx.x; i0 < rows << shift; i0 += 4 * GP_WARPS * 32) {   // four loads of bias and residual at a time
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + k * GP_WARPS * 32, n = n_first + (i & (cols - 1));
+      v[k] = 0.0f;
+      if (i < rows << shift && n < p.N) {
+        if (p.residual) v[k] = p.residual[(int64_t)(m0 + (i >> shift)) * p.N + n];
+        if (p.bias) v[k] += to_f(reinterpret_cast<const T*>(p.bias)[n]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + k * GP_WARPS * 32, row = i >> shift, col = i & (cols - 1), n = n_first + col;
+      if (i >= rows << shift || n >= p.N) continue;
+      float sum = 0.0f;
+      for (int w = 0; w < p.split; ++w) sum += red[((col >> 4) << p.split_log) + w][row][col & 15];
+      p.y[(int64_t)(m0 + row) * p.N + n] = v[k] + sum;
+    }
   }
 }
 
 // The byte kernel: segments of x that one pass keeps in shared memory (64 KB).
 template <int ROWS> constexpr int GP_S8_CHUNK = ROWS == 1 ? 64 : 32;
-template <int PAIRS> constexpr int GP_F32_CHUNK = PAIRS == 1 ? 40 : 10;   // the same (80 KB)
 
 // The upper nibbles u of four bytes as 16 (u - 8): one instruction with both masks in registers.
 __device__ __forceinline__ uint32_t gp_signed16(uint32_t w, uint32_t flip, uint32_t keep) {
@@ -304,204 +325,139 @@ __global__ void __launch_bounds__(GP_WARPS * 32, 3) gemv_packed_s8_kernel(GemvPa
   gp_finish<bf16>(p, red, 0);
 }
 
-// PAIRS: pairs of rows a CTA takes.  Block = 8 warps; grid = (tiles of 16 features x split / 8, rows / (2 PAIRS)).
-template <int PAIRS, int GS>
-__global__ void __launch_bounds__(GP_WARPS * 32, 2) gemv_packed_f32_kernel(GemvPackedParams p) {
-  extern __shared__ __align__(16) uint4 xf[];   // [segment][pair][i][lane]: eight values of a lane's column
-  __shared__ float red[GP_WARPS][2 * PAIRS][17];
+// Rows as bf16 operands.  A tile is the eight columns of an operand: eight bf16 rows, or two f32 rows of three pieces each (the
+// fourth column is never written and never read).  x is brought into shared memory once a CTA, in the operand's order, so that
+// rows of any alignment cost the loop nothing (value by value from global memory: 37 us instead of 9 for 7 rows, 1275 ->
+// 47372).  Block = 8 warps; grid = (tiles of 16 features x split / 8, rows / rows of TILES tiles).
+template <typename T> constexpr int GP_TILE_ROWS = sizeof(T) == 2 ? 8 : 2;
+
+template <typename T, int TILES, int GS>
+__global__ void __launch_bounds__(GP_WARPS * 32, TILES == 1 ? 3 : 2) gemv_packed_mma_kernel(GemvPackedParams p) {
+  constexpr int TILE_ROWS = GP_TILE_ROWS<T>, ROWS = TILES * TILE_ROWS;
+  extern __shared__ __align__(16) uint4 xf[];   // [segment][tile][i][lane]: eight values of a lane's column
+  __shared__ float red[GP_WARPS][ROWS][17];
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int part = warp & (p.split - 1), tile = blockIdx.x * (GP_WARPS >> p.split_log) + (warp >> p.split_log);
-  const int m0 = blockIdx.y * 2 * PAIRS, segs = p.Kp >> 7, rows = min(2 * PAIRS, p.M - m0);
-  const int na = min(tile * 16 + g, p.N - 1), nb = min(tile * 16 + g + 8, p.N - 1);
-  const uint4* wa = reinterpret_cast<const uint4*>(p.W + (int64_t)na * (p.Kp >> 3)) + t;
-  const uint4* wb = reinterpret_cast<const uint4*>(p.W + (int64_t)nb * (p.Kp >> 3)) + t;
-  const bf16* sa = p.scale + (int64_t)na * segs * GS;
-  const bf16* sb = p.scale + (int64_t)nb * segs * GS;
-  const float* x = reinterpret_cast<const float*>(p.x) + (int64_t)m0 * p.ldx;
-  pdl_wait();
-
-  float acc[PAIRS][4];
-#pragma unroll
-  for (int q = 0; q < PAIRS; ++q)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[q][j] = 0.0f;
-  for (int first = 0; first < segs; first += GP_F32_CHUNK<PAIRS>) {
-    const int here = min(GP_F32_CHUNK<PAIRS>, segs - first), last = first + here;
-    uint4 a[2], b[2];
-    GpScale<GS> fa[2], fb[2];
-    auto fetch = [&](int u, int sg) {
-      if (sg < last) {
-        a[u] = __ldg(wa + 4 * sg);
-        b[u] = __ldg(wb + 4 * sg);
-        fa[u].load(sa + sg * GS);
-        fb[u].load(sb + sg * GS);
-      }
-    };
-    fetch(0, first + part);
-    fetch(1, first + part + p.split);
-    __syncthreads();   // the pass before has read xf
-    for (int unit = threadIdx.x; unit < here * 16; unit += GP_WARPS * 32) {   // of eight values, in every row
-      uint4* to = xf + (((unit >> 4) * PAIRS * 4 + ((unit & 15) >> 2)) * 32 + (unit & 3));
-#pragma unroll 1
-      for (int pair = 0; 2 * pair < rows; ++pair, to += 128) {
-        float v[2][8];
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          if (2 * pair + k < rows) gp_row8(x + (int64_t)(2 * pair + k) * p.ldx, first * 128 + 8 * unit, p.K, p.vec, v[k]);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          if (2 * pair + k >= rows) break;
-#pragma unroll
-          for (int q = 0; q < 3; ++q) {   // the upper 16 bits of what is left, cut off, not rounded: nothing overflows
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = __byte_perm(__float_as_uint(v[k][2 * j]), __float_as_uint(v[k][2 * j + 1]), 0x7632);
-            to[16 * k + 4 * q] = make_uint4(w[0], w[1], w[2], w[3]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float cut = __uint_as_float(__float_as_uint(v[k][j]) & 0xffff0000u);
-              v[k][j] = fabsf(v[k][j]) == INFINITY ? 0.0f : v[k][j] - cut;
-            }
-          }
-        }
-      }
-    }
-    __syncthreads();
-#pragma unroll 2
-    for (int sg = first + part, u = 0; sg < last; sg += p.split, u ^= 1) {
-      const uint4 a_now = a[u], b_now = b[u];
-      const GpScale<GS> fa_now = fa[u], fb_now = fb[u];
-      fetch(u, sg + 2 * p.split);
-      const uint32_t* aw = reinterpret_cast<const uint32_t*>(&a_now);
-      const uint32_t* bw = reinterpret_cast<const uint32_t*>(&b_now);
-      float c[PAIRS][4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t ra[4], rb[4];
-        gp_unpack(aw[i], ra);
-        gp_unpack(bw[i], rb);
-#pragma unroll
-        for (int q = 0; q < PAIRS; ++q) {
-          if (2 * q >= rows) break;
-          uint4 xb = make_uint4(0, 0, 0, 0);
-          if ((g & 3) != 3 && 2 * q + (g >> 2) < rows) xb = xf[(((sg - first) * PAIRS + q) * 4 + i) * 32 + lane];
-          if (i % (4 / GS) == 0) c[q][0] = c[q][1] = c[q][2] = c[q][3] = 0.0f;
-          mma_bf16_16816(c[q], ra[0], rb[0], ra[1], rb[1], xb.x, xb.y);
-          mma_bf16_16816(c[q], ra[2], rb[2], ra[3], rb[3], xb.z, xb.w);
-          if ((i + 1) % (4 / GS) == 0) {
-            const float sa_g = fa_now.get(i / (4 / GS)), sb_g = fb_now.get(i / (4 / GS));
-            acc[q][0] = fmaf(sa_g, c[q][0], acc[q][0]);
-            acc[q][1] = fmaf(sa_g, c[q][1], acc[q][1]);
-            acc[q][2] = fmaf(sb_g, c[q][2], acc[q][2]);
-            acc[q][3] = fmaf(sb_g, c[q][3], acc[q][3]);
-          }
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int q = 0; q < PAIRS; ++q)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {   // the pieces' columns: two in a lane, the third in the next
-      const float two = acc[q][2 * h] + acc[q][2 * h + 1];
-      const float v = two + __shfl_xor_sync(0xffffffffu, two, 1);
-      if (!(t & 1)) red[warp][2 * q + (t >> 1)][g + 8 * h] = v;
-    }
-  __syncthreads();
-  gp_finish<float>(p, red, m0);
-}
-
-// Block = 8 warps; grid = (tiles of 16 features x split / 8, rows / (8 NT)).  GS: scales of a segment of 128 weights.
-template <int NT, int GS>
-__global__ void __launch_bounds__(GP_WARPS * 32) gemv_packed_bf16_kernel(GemvPackedParams p) {
-  __shared__ float red[GP_WARPS][8 * NT][17];
-  pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int part = warp & (p.split - 1), tile = blockIdx.x * (GP_WARPS >> p.split_log) + (warp >> p.split_log);
-  const int m0 = blockIdx.y * 8 * NT, segs = p.Kp >> 7;
+  const int m0 = blockIdx.y * ROWS, segs = p.Kp >> 7, rows = min(ROWS, p.M - m0), tiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
   const int na = min(tile * 16 + g, p.N - 1), nb = min(tile * 16 + g + 8, p.N - 1);
   const uint4* wa = reinterpret_cast<const uint4*>(p.W + (int64_t)na * (p.Kp >> 3)) + t;   // a segment is four uint4
   const uint4* wb = reinterpret_cast<const uint4*>(p.W + (int64_t)nb * (p.Kp >> 3)) + t;
   const bf16* sa = p.scale + (int64_t)na * segs * GS;
   const bf16* sb = p.scale + (int64_t)nb * segs * GS;
-  const bf16* x = reinterpret_cast<const bf16*>(p.x);
+  const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)m0 * p.ldx;
+  const uint32_t xf_mine = (uint32_t)__cvta_generic_to_shared(xf) + 16 * lane;
   pdl_wait();
 
-  float acc[NT][4];
+  float acc[TILES][4];
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
+  for (int q = 0; q < TILES; ++q)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-
-  // weights two segments ahead, x one: both are under way while a segment is worked on
-  uint4 a[2], b[2], xn[NT][4];
-  GpScale<GS> fa[2], fb[2];
-  auto fetch_w = [&](int u, int sg) {
-    if (sg < segs) {
+    for (int j = 0; j < 4; ++j) acc[q][j] = 0.0f;
+  for (int first = 0; first < segs; first += p.chunk) {
+    const int here = min(p.chunk, segs - first);
+    const int n = part < here ? (here - part + p.split - 1) >> p.split_log : 0;   // segments of this warp
+    uint4 a[2], b[2];
+    GpScale<GS> fa[2], fb[2];
+    auto fetch = [&](int u, int j) {
+      const int sg = first + part + (j << p.split_log);
       a[u] = __ldg(wa + 4 * sg);
       b[u] = __ldg(wb + 4 * sg);
       fa[u].load(sa + sg * GS);
       fb[u].load(sb + sg * GS);
-    }
-  };
-  auto fetch_x = [&](int sg) {
+    };
+    if (n > 0) fetch(0, 0);
+    if (n > 1) fetch(1, 1);
+    __syncthreads();   // the pass before has read xf
+    for (int unit = threadIdx.x; unit < here * 16; unit += GP_WARPS * 32) {   // of eight values, in every row
+      uint4* to = xf + (((unit >> 4) * TILES * 4 + ((unit & 15) >> 2)) * 32 + (unit & 3));
+      const int k0 = first * 128 + 8 * unit;
+      if (sizeof(T) == 2 && p.vec) {   // as it lies: asynchronous copies, all under way at once
+        for (int m = 0; m < rows; ++m)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to + (m >> 3) * 128 + (m & 7) * 4)),
+                       "l"(k0 < p.K ? x + (int64_t)m * p.ldx + k0 : x), "r"(k0 < p.K ? 16 : 0) : "memory");
+      } else if constexpr (sizeof(T) == 2) {
+#pragma unroll 4
+        for (int m = 0; m < rows; ++m) to[(m >> 3) * 128 + (m & 7) * 4] = gp_row(x + (int64_t)m * p.ldx, k0, p.K, false);
+      } else {
+#pragma unroll 1
+        for (int pair = 0; 2 * pair < rows; ++pair, to += 128) {
+          float v[2][8];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int m = m0 + 8 * nt + g;
+          for (int k = 0; k < 2; ++k)
+            if (2 * pair + k < rows) gp_row8(x + (int64_t)(2 * pair + k) * p.ldx, k0, p.K, p.vec, v[k]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        xn[nt][i] = make_uint4(0, 0, 0, 0);
-        if (m < p.M && sg < segs) xn[nt][i] = gp_row(x + (int64_t)m * p.ldx, sg * 128 + 32 * i + 8 * t, p.K, p.vec);
-      }
-    }
-  };
-  fetch_w(0, part);
-  fetch_w(1, part + p.split);
-  fetch_x(part);
-#pragma unroll 2
-  for (int sg = part, u = 0; sg < segs; sg += p.split, u ^= 1) {
-    const uint4 wa_now = a[u], wb_now = b[u];
-    const GpScale<GS> fa_now = fa[u], fb_now = fb[u];
-    uint4 xc[NT][4];
+          for (int k = 0; k < 2; ++k) {
+            if (2 * pair + k >= rows) break;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+            for (int q = 0; q < 3; ++q) {   // the upper 16 bits of what is left, cut off, not rounded: nothing overflows
+              uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) xc[nt][i] = xn[nt][i];
-    fetch_w(u, sg + 2 * p.split);
-    fetch_x(sg + p.split);
-    const uint32_t* aw = reinterpret_cast<const uint32_t*>(&wa_now);
-    const uint32_t* bw = reinterpret_cast<const uint32_t*>(&wb_now);
-    float c[NT][4];
+              for (int j = 0; j < 4; ++j) w[j] = __byte_perm(__float_as_uint(v[k][2 * j]), __float_as_uint(v[k][2 * j + 1]), 0x7632);
+              to[16 * k + 4 * q] = make_uint4(w[0], w[1], w[2], w[3]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t ra[4], rb[4];
-      gp_unpack(aw[i], ra);
-      gp_unpack(bw[i], rb);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (i % (4 / GS) == 0) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
-        mma_bf16_16816(c[nt], ra[0], rb[0], ra[1], rb[1], xc[nt][i].x, xc[nt][i].y);
-        mma_bf16_16816(c[nt], ra[2], rb[2], ra[3], rb[3], xc[nt][i].z, xc[nt][i].w);
-        if ((i + 1) % (4 / GS) == 0) {   // the end of a group
-          const float sa_g = fa_now.get(i / (4 / GS)), sb_g = fb_now.get(i / (4 / GS));
-          acc[nt][0] = fmaf(sa_g, c[nt][0], acc[nt][0]);
-          acc[nt][1] = fmaf(sa_g, c[nt][1], acc[nt][1]);
-          acc[nt][2] = fmaf(sb_g, c[nt][2], acc[nt][2]);
-          acc[nt][3] = fmaf(sb_g, c[nt][3], acc[nt][3]);
+              for (int j = 0; j < 8; ++j) {
+                const float cut = __uint_as_float(__float_as_uint(v[k][j]) & 0xffff0000u);
+                v[k][j] = fabsf(v[k][j]) == INFINITY ? 0.0f : v[k][j] - cut;
+              }
+            }
+          }
         }
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    uint32_t low = 0x000f000fu, base = 0x43004300u;
+    asm volatile("" : "+r"(low), "+r"(base));   // known to nobody: they stay in registers
+    for (int j = 0; j < n; j += 2) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (j + u >= n) break;
+        const uint32_t aw[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, bw[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
+        const uint32_t xq = xf_mine + (part + ((j + u) << p.split_log)) * (TILES * 2048);
+        float c[TILES][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t ra[4], rb[4];
+          gp_unpack(aw[i], low, base, ra);
+          gp_unpack(bw[i], low, base, rb);
+#pragma unroll
+          for (int q = 0; q < TILES; ++q) {
+            if (q >= tiles) break;
+            uint4 xb;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(xb.x), "=r"(xb.y), "=r"(xb.z), "=r"(xb.w) : "r"(xq + 2048 * q + 512 * i) : "memory");
+            if (i % (4 / GS) == 0) mma_bf16_16816_first(c[q], ra[0], rb[0], ra[1], rb[1], xb.x, xb.y);
+            else mma_bf16_16816(c[q], ra[0], rb[0], ra[1], rb[1], xb.x, xb.y);
+            mma_bf16_16816(c[q], ra[2], rb[2], ra[3], rb[3], xb.z, xb.w);
+            if ((i + 1) % (4 / GS) == 0) {   // the end of a group
+              const float sa_g = fa[u].get(i / (4 / GS)), sb_g = fb[u].get(i / (4 / GS));
+              acc[q][0] = fmaf(sa_g, c[q][0], acc[q][0]);
+              acc[q][1] = fmaf(sa_g, c[q][1], acc[q][1]);
+              acc[q][2] = fmaf(sb_g, c[q][2], acc[q][2]);
+              acc[q][3] = fmaf(sb_g, c[q][3], acc[q][3]);
+            }
+          }
+        }
+        if (j + u + 2 < n) fetch(u, j + u + 2);   // into the registers just used; the other segment's work covers its way
+      }
+    }
   }
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    red[warp][8 * nt + 2 * t][g] = acc[nt][0];
-    red[warp][8 * nt + 2 * t + 1][g] = acc[nt][1];
-    red[warp][8 * nt + 2 * t][g + 8] = acc[nt][2];
-    red[warp][8 * nt + 2 * t + 1][g + 8] = acc[nt][3];
-  }
+  for (int q = 0; q < TILES; ++q)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if constexpr (sizeof(T) == 2) {
+        red[warp][8 * q + 2 * t][g + 8 * h] = acc[q][2 * h];
+        red[warp][8 * q + 2 * t + 1][g + 8 * h] = acc[q][2 * h + 1];
+      } else {   // the pieces' columns: two in a lane, the third in the next
+        const float mine = t & 1 ? acc[q][2 * h] : acc[q][2 * h] + acc[q][2 * h + 1];
+        const float v = mine + __shfl_xor_sync(0xffffffffu, mine, 1);
+        if (!(t & 1)) red[warp][2 * q + (t >> 1)][g + 8 * h] = v;
+      }
+    }
   __syncthreads();
-  gp_finish<bf16>(p, red, m0);
+  gp_finish<T>(p, red, m0);
 }
 
 }  // namespace wdz

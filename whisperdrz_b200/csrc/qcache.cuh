@@ -206,24 +206,25 @@ __device__ __forceinline__ float qc_finite_top(const QcRaw<T>& r, float m) {   /
   return m;
 }
 
-// A run's place; ok is false (and reported, unless its slot is outside or it is empty) where it cannot be stored.
+// A run's place; ok is false where it cannot be stored, `outside` where that has to be reported.
 struct QcRun {
   int slot, p0, p1, r0;
-  bool ok;
-  __device__ QcRun(const QcStoreParams& p, int run, bool reports, DevStatus* status) {   // by all threads of the block
+  bool ok, outside;
+  __device__ QcRun(const QcStoreParams& p, int run) {
     slot = p.slots[run];
     p0 = p.positions[run];
     r0 = p.row_begin ? p.row_begin[run] : run;
     const int r1 = p.row_begin ? p.row_begin[run + 1] : run + 1, room = p.c.n_blocks * QC_BLOCK;
+    ok = slot >= 0 && slot < p.c.n_slots && r1 > r0;
+    outside = ok && (r0 < 0 || r1 > p.n_rows || p0 < 0 || p0 > room - (r1 - r0));
+    ok = ok && !outside;
+    p1 = ok ? p0 + (r1 - r0) : 0;
+  }
+  // By all threads of the block, while the rows are on their way: does a later run name the slot?  The last one counts.
+  __device__ bool named_again(const QcStoreParams& p, int run) const {
     int again = 0;
     for (int j = run + 1 + threadIdx.x; j < p.n_runs; j += blockDim.x) again |= p.slots[j] == slot;
-    again = __syncthreads_or(again);   // a later run names the slot: the last one counts
-    ok = slot >= 0 && slot < p.c.n_slots && r1 > r0;
-    if (ok && (r0 < 0 || r1 > p.n_rows || p0 < 0 || p0 > room - (r1 - r0) || again)) {
-      if (reports && threadIdx.x == 0) qc_report(status, WDZ_EINVAL, 2000000 + run);
-      ok = false;
-    }
-    p1 = ok ? p0 + (r1 - r0) : 0;
+    return __syncthreads_or(again);
   }
 };
 
@@ -263,9 +264,13 @@ __global__ void __launch_bounds__((SHARE == 1 ? 2 : SHARE) * 32) qcache_store_ke
   const int unit = SHARE > 1 ? blockIdx.y : blockIdx.y * 2 + warp;
   uint8_t* mine = qc_rows + (SHARE > 1 ? 0 : warp) * QC_UNIT<T> + lane * 16;   // 16 bytes of each lane side by side
   pdl_wait();
-  const QcRun run(p, blockIdx.z, blockIdx.x == 0 && blockIdx.y == 0, status);
-  if (!run.ok || unit >= 2 * p.c.n_heads) return;
-  const bool is_v = unit >= p.c.n_heads;
+  const QcRun run(p, blockIdx.z);
+  const bool reports = blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0;
+  if (!run.ok) {
+    if (run.outside && reports) qc_report(status, WDZ_EINVAL, 2000000 + (int)blockIdx.z);
+    return;
+  }
+  const bool is_v = unit >= p.c.n_heads;   // 2 n_heads units: the grid has no other
   const int head = is_v ? unit - p.c.n_heads : unit;
   const QcPlace place(p.c, run.slot, head, is_v);
   const int64_t ld = (is_v ? p.ldv : p.ldk) * (int64_t)sizeof(T);
@@ -280,6 +285,7 @@ __global__ void __launch_bounds__((SHARE == 1 ? 2 : SHARE) * 32) qcache_store_ke
     }
     return bits;
   };
+  bool asked = false;
   for (int b = run.p0 / QC_BLOCK + blockIdx.x; b * QC_BLOCK < run.p1; b += gridDim.x) {
     const int lo = max(run.p0, b * QC_BLOCK), hi = min(run.p1, (b + 1) * QC_BLOCK), t0 = b * QC_BLOCK + (lane >> 3);
     const int i0 = (lo - b * QC_BLOCK) >> 2, i1 = (hi - b * QC_BLOCK + 3) >> 2;   // steps of four tokens that the run reaches
@@ -297,7 +303,13 @@ __global__ void __launch_bounds__((SHARE == 1 ? 2 : SHARE) * 32) qcache_store_ke
     asm volatile("cp.async.commit_group;" ::: "memory");
     const bool entered = lo > b * QC_BLOCK;   // behind the block's first token: what it holds stays
     const float old = entered ? place.s[b] : 0.0f;
+    const bool again = !asked && run.named_again(p, blockIdx.z);
+    asked = true;
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (again) {   // nothing has been written yet
+      if (reports) qc_report(status, WDZ_EINVAL, 2000000 + (int)blockIdx.z);
+      return;
+    }
     float top = 0.0f;
 #pragma unroll 8
     for (int i = is; i < i1; i += SHARE) top = QcRaw<T>(mine + i * STEP).top(top);
@@ -350,8 +362,13 @@ __global__ void __launch_bounds__(320, 3) qcache_step_kernel(QcStoreParams p, De
   pdl_trigger();
   const int c = threadIdx.x & 7, mine = threadIdx.x >> 3, units = 2 * p.c.n_heads;
   pdl_wait();
-  const QcRun run(p, blockIdx.x, true, status);
+  const QcRun run(p, blockIdx.x);
+  if (run.outside && threadIdx.x == 0) qc_report(status, WDZ_EINVAL, 2000000 + (int)blockIdx.x);
   if (!run.ok) return;
+  if (run.named_again(p, blockIdx.x)) {
+    if (threadIdx.x == 0) qc_report(status, WDZ_EINVAL, 2000000 + (int)blockIdx.x);
+    return;
+  }
   const int b = run.p0 / QC_BLOCK, kept = run.p0 % QC_BLOCK;
   for (int first = 0; first < units; first += UNITS) {
     const int unit = first + mine;
