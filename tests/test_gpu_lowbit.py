@@ -412,11 +412,32 @@ def _check_linear(eng, x, packed, w, b, residual=None, out=None):
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("m,n,k", [(1, 1280, 1280), (1, 17, 130), (2, 64, 64), (3, 100, 1), (5, 33, 1237), (8, 256, 5120), (9, 31, 640),
                                    (16, 160, 256), (17, 48, 384), (33, 16, 136), (70, 15, 127), (2, 40, 9000), (1, 16, 20000),
-                                   (4, 24, 8192)])
+                                   (4, 24, 8192), (5, 24, 14000), (12, 17, 9001), (3, 40, 5003)])
 def test_linear_shapes(eng, m, n, k, group, dtype):
     packed, w, b = _packed(n, k, group, seed=m + n, bias=dtype if m % 2 else None)
     x = torch.randn(m, k, generator=torch.Generator().manual_seed(k)).to(dtype)
     _check_linear(eng, x, packed, w, b)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("m", [1, 2, 4, 9, 16, 19])
+def test_linear_of_many_features(eng, m, dtype):
+    """Enough features that an SM has several blocks, and more inputs than one pass of theirs holds; the reference in 64 bits
+    on the device."""
+    n, k, group = 19001, 4250, 64
+    g = torch.Generator(device="cuda").manual_seed(m)
+    kp = (k + 127) // 128 * 128
+    q = torch.randint(-8, 8, (n, kp), generator=g, device="cuda", dtype=torch.int32)
+    q[:, k:] = 0
+    scale = (0.02 * torch.exp(0.5 * torch.randn(n, kp // group, generator=g, device="cuda"))).bfloat16()
+    w = (q.double().view(n, -1, group) * scale.double()[..., None]).view(n, kp)[:, :k]
+    x = torch.randn(m, k, generator=g, device="cuda").to(dtype)
+    r = torch.randn(m, n, generator=g, device="cuda")
+    got = eng.linear_rows_packed(x, PackedLinear(pack_nibbles(q), scale, k, group), residual=r).double()
+    want = x.double() @ w.T + r.double()
+    tol = (k + 8) * U * (x.double().abs() @ w.abs().T + r.double().abs()) + 2.0 ** -46 * x.double().abs().amax(1, True) * w.abs().sum(1)
+    assert bool(((got - want).abs() <= tol).all())
+    assert float((got - want).norm() / want.norm()) <= 1e-5
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
@@ -572,6 +593,32 @@ def test_attention_in_place_of_its_queries(eng):
     both = q.cuda()
     assert eng.qcache_attention(both, c, [2, 0, 1], [190, 64, 0], out=both) is both
     assert torch.equal(both, want)
+
+
+def test_operators_of_a_bf16_engine_without_overlapped_launches():
+    """The other kind of engine, its default output type, and its launches without programmatic dependence."""
+    from whisperdrz_b200 import capi
+    from whisperdrz_b200.engine import Engine
+    dims = ModelDimensions.from_name("test-small")
+    e = Engine(dims, init_state_dict(dims, 0), dtype=BF16, n_slots=1, max_clips=1, max_rows=1, flags=capi.FLAG_NO_PDL)
+    try:
+        parts = _filled(3, 4, 2, seed=1)
+        c = e.qcache(n_slots=3, n_tokens=100, n_heads=4)
+        for t, p in zip((c.k, c.v, c.k_scale, c.v_scale), parts):
+            t.copy_(p)
+        q = torch.randn(3, 256, generator=torch.Generator().manual_seed(3))
+        before = e.launch_count()
+        got = e.qcache_attention(q.cuda(), c, [2, 0, 1], [100, 64, 1])
+        assert got.dtype == BF16 and e.launch_count() == before + 1
+        _check_attend(e, parts, q, [2, 0, 1], [100, 64, 1], out_dtype=BF16)
+        _check_store(e, parts, q, q, [0, 2, 1], [3, 64, 127])
+        packed, w, b = _packed(40, 300, 32, seed=1)
+        _check_linear(e, q.new_ones(2, 300).to(BF16), packed, w, b)
+        default = e.qcache()
+        assert (default.n_slots, default.n_heads, default.n_tokens) == (1, dims.n_text_head, 1536)
+        e.device_status()
+    finally:
+        e.close()
 
 
 def test_calls_refuse_tensors_elsewhere(eng):
