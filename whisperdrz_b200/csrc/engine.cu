@@ -1120,12 +1120,14 @@ int wdz_finalize(wdz_engine* e) {
     allow(gemv_packed_s8_kernel<1, 1>, GP_S8_CHUNK<1> * 1024); allow(gemv_packed_s8_kernel<1, 2>, GP_S8_CHUNK<1> * 1024);
     allow(gemv_packed_s8_kernel<1, 4>, GP_S8_CHUNK<1> * 1024); allow(gemv_packed_s8_kernel<2, 1>, GP_S8_CHUNK<2> * 2048);
     allow(gemv_packed_s8_kernel<2, 2>, GP_S8_CHUNK<2> * 2048); allow(gemv_packed_s8_kernel<2, 4>, GP_S8_CHUNK<2> * 2048);
-    allow(gemv_packed_mma_kernel<float, 1, 1>, 200 * 1024); allow(gemv_packed_mma_kernel<float, 1, 2>, 200 * 1024);
-    allow(gemv_packed_mma_kernel<float, 1, 4>, 200 * 1024); allow(gemv_packed_mma_kernel<float, 4, 1>, 200 * 1024);
-    allow(gemv_packed_mma_kernel<float, 4, 2>, 200 * 1024); allow(gemv_packed_mma_kernel<float, 4, 4>, 200 * 1024);
-    allow(gemv_packed_mma_kernel<bf16, 1, 1>, 200 * 1024); allow(gemv_packed_mma_kernel<bf16, 1, 2>, 200 * 1024);
-    allow(gemv_packed_mma_kernel<bf16, 1, 4>, 200 * 1024); allow(gemv_packed_mma_kernel<bf16, 2, 1>, 200 * 1024);
-    allow(gemv_packed_mma_kernel<bf16, 2, 2>, 200 * 1024); allow(gemv_packed_mma_kernel<bf16, 2, 4>, 200 * 1024);
+    auto packed = [&](auto gs) {
+      constexpr int GS = decltype(gs)::value, bytes = 200 * 1024;
+      allow(gemv_packed_mma_kernel<float, 1, GS, 2>, bytes); allow(gemv_packed_mma_kernel<float, 1, GS, 3>, bytes);
+      allow(gemv_packed_mma_kernel<float, 2, GS, 2>, bytes); allow(gemv_packed_mma_kernel<float, 3, GS, 2>, bytes);
+      allow(gemv_packed_mma_kernel<float, 4, GS, 2>, bytes); allow(gemv_packed_mma_kernel<bf16, 2, GS, 2>, bytes);
+      allow(gemv_packed_mma_kernel<bf16, 1, GS, 2>, bytes); allow(gemv_packed_mma_kernel<bf16, 1, GS, 3>, bytes);
+    };
+    packed(std::integral_constant<int, 1>()); packed(std::integral_constant<int, 2>()); packed(std::integral_constant<int, 4>());
     // CTAs of a few warps that share an SM by their shared memory: always the largest part of it
     auto share = [&](auto kern) {
       if (ce4 == cudaSuccess) ce4 = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
@@ -2121,19 +2123,30 @@ int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_
   auto held = [&](int chunk) { return (size_t)(segs < chunk ? segs : chunk); };   // segments of x in shared memory
   auto mma = [&](auto tx, auto tiles_c, auto gs) {
     using T = decltype(tx);
-    constexpr int TILES = decltype(tiles_c)::value;
-    // x in one pass where every SM has a CTA at most; otherwise no more than lets two or three share an SM
+    constexpr int TILES = decltype(tiles_c)::value, GS = decltype(gs)::value;
     const int rows = TILES * GP_TILE_ROWS<T>, per = GP_WARPS / p.split;
-    const bool alone = (int64_t)((tiles + per - 1) / per) * ((M + rows - 1) / rows) <= e->sm_count;
-    p.chunk = (alone ? 200 : TILES == 1 ? 64 : 80) / (2 * TILES);
-    go(gemv_packed_mma_kernel<T, TILES, decltype(gs)::value>, rows, held(p.chunk) * TILES * 2048);
+    const int64_t ctas = (int64_t)((tiles + per - 1) / per) * ((M + rows - 1) / rows);
+    // x in one pass where every SM has a CTA at most; otherwise no more than lets two or three share an SM
+    p.chunk = (ctas <= e->sm_count ? 200 : TILES == 1 ? 64 : 80) / (2 * TILES);
+    const size_t smem = held(p.chunk) * TILES * 2048;
+    if constexpr (TILES == 1) {
+      if (ctas > 2 * e->sm_count && ctas <= 3 * e->sm_count) return go(gemv_packed_mma_kernel<T, 1, GS, 3>, rows, smem);
+    }
+    go(gemv_packed_mma_kernel<T, TILES, GS, 2>, rows, smem);
   };
   using one = std::integral_constant<int, 1>;
   using two = std::integral_constant<int, 2>;
+  using three = std::integral_constant<int, 3>;
   using four = std::integral_constant<int, 4>;
   // Two rows and fewer in bf16 leave six of a tile's columns empty: there bytes are cheaper (one row over 51866 features 9 us
   // against 11 to 12 on bf16 operands).
-  if (x_dtype == WDZ_F32) by_group([&](auto gs) { if (M <= 2) mma(0.0f, one(), gs); else mma(0.0f, four(), gs); });
+  if (x_dtype == WDZ_F32)
+    by_group([&](auto gs) {
+      if (M <= 2) mma(0.0f, one(), gs);
+      else if (M <= 4) mma(0.0f, two(), gs);
+      else if (M <= 6) mma(0.0f, three(), gs);
+      else mma(0.0f, four(), gs);
+    });
   else if (M == 1) by_group([&](auto gs) { go(gemv_packed_s8_kernel<1, decltype(gs)::value>, 1, held(GP_S8_CHUNK<1>) * 1024); });
   else if (M == 2) by_group([&](auto gs) { go(gemv_packed_s8_kernel<2, decltype(gs)::value>, 2, held(GP_S8_CHUNK<2>) * 2048); });
   else by_group([&](auto gs) { if (M <= 8) mma(bf16(), one(), gs); else mma(bf16(), two(), gs); });

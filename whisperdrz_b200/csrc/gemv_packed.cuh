@@ -268,6 +268,7 @@ __global__ void __launch_bounds__(GP_WARPS * 32, 3) gemv_packed_s8_kernel(GemvPa
     for (int m = 0; m < ROWS; ++m) acc[m][0] = acc[m][1] = 0.0f;
     uint32_t flip = 0x80808080u, keep = 0xf0f0f0f0u;
     asm volatile("" : "+r"(flip), "+r"(keep));   // known to nobody: they stay in registers
+    uint32_t xq = xs_mine + part * (ROWS * 1024);
     for (int j = 0; j < n; j += GP_AHEAD) {
 #pragma unroll
       for (int u = 0; u < GP_AHEAD; ++u) {
@@ -285,7 +286,6 @@ __global__ void __launch_bounds__(GP_WARPS * 32, 3) gemv_packed_s8_kernel(GemvPa
 #pragma unroll
         for (int i = 0; i < GS; ++i) { sa_g[i] = fa[u].get(i); sb_g[i] = fb[u].get(i); }
         if (j + u + GP_AHEAD < n) fetch(u, j + u + GP_AHEAD);
-        const uint32_t xq = xs_mine + (part + ((j + u) << p.split_log)) * (ROWS * 1024);
 #pragma unroll
         for (int m = 0; m < ROWS; ++m) {
           int c[4];
@@ -301,6 +301,7 @@ __global__ void __launch_bounds__(GP_WARPS * 32, 3) gemv_packed_s8_kernel(GemvPa
             }
           }
         }
+        xq += (ROWS * 1024) << p.split_log;
       }
     }
     // times 2^-45 of the unit, 2^-4 of the shifted nibble and the column's 2^16 t; the row's own size last, so that nothing
@@ -328,18 +329,20 @@ __global__ void __launch_bounds__(GP_WARPS * 32, 3) gemv_packed_s8_kernel(GemvPa
 // Rows as bf16 operands.  A tile is the eight columns of an operand: eight bf16 rows, or two f32 rows of three pieces each (the
 // fourth column is never written and never read).  x is brought into shared memory once a CTA, in the operand's order, so that
 // rows of any alignment cost the loop nothing (value by value from global memory: 37 us instead of 9 for 7 rows, 1275 ->
-// 47372).  Block = 8 warps; grid = (tiles of 16 features x split / 8, rows / rows of TILES tiles).
+// 47372).  FIT: CTAs that share an SM.  Three where that makes one wave of what would be two (7 rows over 47372 features: 13 us
+// against 16), else two, whose registers save a third of the instructions (3 rows over 36319: 10 us against 13.5).
+// Block = 8 warps; grid = (tiles of 16 features x split / 8, rows / rows of TILES tiles).
 template <typename T> constexpr int GP_TILE_ROWS = sizeof(T) == 2 ? 8 : 2;
 
-template <typename T, int TILES, int GS>
-__global__ void __launch_bounds__(GP_WARPS * 32, TILES == 1 ? 3 : 2) gemv_packed_mma_kernel(GemvPackedParams p) {
+template <typename T, int TILES, int GS, int FIT>
+__global__ void __launch_bounds__(GP_WARPS * 32, FIT) gemv_packed_mma_kernel(GemvPackedParams p) {
   constexpr int TILE_ROWS = GP_TILE_ROWS<T>, ROWS = TILES * TILE_ROWS;
   extern __shared__ __align__(16) uint4 xf[];   // [segment][tile][i][lane]: eight values of a lane's column
   __shared__ float red[GP_WARPS][ROWS][17];
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int part = warp & (p.split - 1), tile = blockIdx.x * (GP_WARPS >> p.split_log) + (warp >> p.split_log);
-  const int m0 = blockIdx.y * ROWS, segs = p.Kp >> 7, rows = min(ROWS, p.M - m0), tiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
+  const int m0 = blockIdx.y * ROWS, segs = p.Kp >> 7, rows = min(ROWS, p.M - m0);
   const int na = min(tile * 16 + g, p.N - 1), nb = min(tile * 16 + g + 8, p.N - 1);
   const uint4* wa = reinterpret_cast<const uint4*>(p.W + (int64_t)na * (p.Kp >> 3)) + t;   // a segment is four uint4
   const uint4* wb = reinterpret_cast<const uint4*>(p.W + (int64_t)nb * (p.Kp >> 3)) + t;
@@ -409,12 +412,12 @@ __global__ void __launch_bounds__(GP_WARPS * 32, TILES == 1 ? 3 : 2) gemv_packed
     __syncthreads();
     uint32_t low = 0x000f000fu, base = 0x43004300u;
     asm volatile("" : "+r"(low), "+r"(base));   // known to nobody: they stay in registers
+    uint32_t xq = xf_mine + part * (TILES * 2048);
     for (int j = 0; j < n; j += 2) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         if (j + u >= n) break;
         const uint32_t aw[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, bw[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
-        const uint32_t xq = xf_mine + (part + ((j + u) << p.split_log)) * (TILES * 2048);
         float c[TILES][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -423,7 +426,6 @@ __global__ void __launch_bounds__(GP_WARPS * 32, TILES == 1 ? 3 : 2) gemv_packed
           gp_unpack(bw[i], low, base, rb);
 #pragma unroll
           for (int q = 0; q < TILES; ++q) {
-            if (q >= tiles) break;
             uint4 xb;
             asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                          : "=r"(xb.x), "=r"(xb.y), "=r"(xb.z), "=r"(xb.w) : "r"(xq + 2048 * q + 512 * i) : "memory");
@@ -439,6 +441,7 @@ __global__ void __launch_bounds__(GP_WARPS * 32, TILES == 1 ? 3 : 2) gemv_packed
             }
           }
         }
+        xq += (TILES * 2048) << p.split_log;
         if (j + u + 2 < n) fetch(u, j + u + 2);   // into the registers just used; the other segment's work covers its way
       }
     }
