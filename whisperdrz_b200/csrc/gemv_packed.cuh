@@ -18,9 +18,9 @@
 //       is one column, as it is; an f32 row is cut into three bf16 pieces (8 + 8 + 8 bits) that add up to it and take three.
 // Either way a group's sum is multiplied by its scale in fp32.
 //
-// Measured (B200, device time): one bf16 row, 1280 x 1280 2.9 us (a launch's latency; the weights' bytes alone 0.13); one row
-// over 51866 x 1280 9.1 us, 3.8 TB/s (19 us on bf16 operands: 88 instructions against 24 to take 64 weights apart); 16 rows,
-// 5120 -> 1280 6.0 us; five f32 rows, 1237 -> 5003 8.6 us.
+// Measured (B200, device time): one bf16 row, 1280 x 1280 3.0 us (a launch's latency; the weights' bytes alone 0.13); one row
+// over 51866 x 1280 9.1 us, 3.8 TB/s, and 11.7 us for three on bf16 operands (88 instructions against 24 to take 64 weights
+// apart); 16 rows, 5120 -> 1280 6.0 us; five f32 rows, 1237 -> 5003 7.2 us.
 #pragma once
 #include "common.cuh"
 #include "gemv_mma.cuh"

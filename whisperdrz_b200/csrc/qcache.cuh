@@ -456,8 +456,8 @@ struct QcAttendParams {
 //
 // Measured (B200, 20 heads, one query head each; device time): 384 rows of 1500 tokens 206 us, 7.1 TB/s of K, V and scales
 // (a plain version on the CUDA cores: 910 us); 32 rows 23 us; 384 rows of lengths spread over 448 tokens 40 us; one row
-// 4.5 us; 2 rows of 32749 tokens, 4 key heads shared by 4 query heads each, 13.4 us with the merge.  About 350 instructions a
-// tile and scheduler keep issue slots 46 % busy at the largest size: the rest is memory.
+// 4.5 us; 2 rows of 32749 tokens, 4 key heads shared by 4 query heads each, 13.4 us with the merge.  Some 700 instructions a
+// tile, prologue and merge among them, keep the issue slots 45 % busy at the largest size: the time is the memory's.
 constexpr int QC_MAX_WARPS = 8;
 constexpr float QC_STEPS = 127.0f * 16777216.0f;   // a query's largest value in steps: rounding up leaves d3 a byte
 constexpr float QC_ONE = 4294967040.0f;            // the weight 1 in steps: the largest fp32 below 2^32
