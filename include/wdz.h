@@ -308,8 +308,8 @@ int wdz_dtw(wdz_engine* e, const float* matrix_dev, int64_t chunk_stride, int64_
  * No counterpart in the reference, whose FlashKVCache (model.py:98-147) and nn.Linear hold 16 or 32 bits.
  * The operators stand beside wdz_cross_kv / the decode step's attention and wdz_linear_rows; they work on
  * caller-held memory of any head count, need an engine only for its device, status word and error text, and
- * take no scratch.  All index arrays are device int32; rows are given by a pointer to row 0 and the elements
- * from one row to the next, rows and caches start on 16 bytes, and heads have 64 values.
+ * keep nothing between calls.  All index arrays are device int32; rows are given by a pointer to row 0 and the
+ * elements from one row to the next, rows and caches start on 16 bytes, and heads have 64 values.
  *
  * The cache: value(slot, head, token, c) = int8 * scale of the token's block of WDZ_QCACHE_BLOCK tokens.
  *   k_dev / v_dev              int8 [n_slots][n_heads][n_blocks * 64][64], slot_stride values from slot to slot
@@ -338,10 +338,10 @@ int wdz_qcache_store(wdz_engine* e, const wdz_qcache* cache, const void* k_dev, 
                      const int32_t* positions_dev, int n_runs, int max_run, wdz_stream s);
 /* Row r's n_q_heads queries (q_dtype [n_rows][n_q_heads * 64]) attend to the first lens_dev[r] tokens of slot
  * slot_ids_dev[r]: out = softmax(scale * q k^T) v, query head h over key head h / (n_q_heads / n_heads), at most 8
- * query heads to a key head.  Queries and softmax weights are held to 2^-31 of the
- * largest of their head or row, everything else in fp32; out_dtype [n_rows][n_q_heads * 64].  Lengths are clamped
- * to the slot; a row of length 0 gives zeros; a row whose slot is outside [0, n_slots) is left as it was, or
- * zeroed when clear_skipped != 0. */
+ * query heads to a key head.  Queries and softmax weights are held to 2^-31 of the largest of their head or row,
+ * everything else in fp32; out: out_dtype [n_rows][n_q_heads * 64], which may be q itself.  Lengths are clamped to
+ * the slot; a row of length 0 gives zeros; a row whose slot is outside [0, n_slots) is left as it was, or zeroed
+ * when clear_skipped != 0. */
 int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_dev, int64_t ldq, int q_dtype, int n_q_heads,
                          const int32_t* slot_ids_dev, const int32_t* lens_dev, int n_rows, float scale, void* out_dev,
                          int64_t ldo, int out_dtype, int clear_skipped, void* scratch_dev, size_t scratch_bytes, wdz_stream s);
