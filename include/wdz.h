@@ -313,7 +313,8 @@ int wdz_dtw(wdz_engine* e, const float* matrix_dev, int64_t chunk_stride, int64_
  *
  * The cache: value(slot, head, token, c) = int8 * scale of the token's block of WDZ_QCACHE_BLOCK tokens.
  *   k_dev / v_dev              int8 [n_slots][n_heads][n_blocks * 64][64], slot_stride values from slot to slot
- *   k_scale_dev / v_scale_dev  f32  [n_slots][n_heads][n_blocks], scale_slot_stride scales from slot to slot */
+ *   k_scale_dev / v_scale_dev  f32  [n_slots][n_heads][n_blocks], scale_slot_stride scales from slot to slot
+ * with n_heads <= 4096 and n_blocks <= 2^24. */
 #define WDZ_QCACHE_BLOCK 64
 typedef struct wdz_qcache {
   void *k_dev, *v_dev;

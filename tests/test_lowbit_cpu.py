@@ -142,7 +142,7 @@ def test_abi_refuses_bad_arguments_before_it_looks_at_the_engine(lib, handle):
     not_ready = -4
     assert store() == not_ready and attend() == not_ready and linear() == not_ready
     caches = [_desc(k=None), _desc(v_scale=None), _desc(k=257), _desc(slot_stride=2 * 2 * 4096 - 16), _desc(slot_stride=2 * 2 * 4096 + 8),
-              _desc(scale_slot_stride=3), _desc(n_slots=0), _desc(n_heads=0), _desc(n_blocks=0), _desc(n_blocks=2 ** 30),
+              _desc(scale_slot_stride=3), _desc(n_slots=0), _desc(n_heads=0), _desc(n_blocks=0), _desc(n_blocks=2 ** 30), _desc(n_blocks=2 ** 24 + 1, slot_stride=2 ** 40, scale_slot_stride=2 ** 30), _desc(n_heads=4097),
               _desc(v_scale=2050)]
     for c in caches:
         assert store(cache=c) == -1 and attend(cache=c) == -1

@@ -1886,7 +1886,7 @@ bool aligned16(const void* p, int64_t stride_bytes) { return (((uintptr_t)p) & 1
 
 int qcache_view(wdz_engine* e, const char* who, const wdz_qcache* c, QcView* v) {
   if (!c || !c->k_dev || !c->v_dev || !c->k_scale_dev || !c->v_scale_dev) return e->fail(WDZ_EINVAL, "%s: null cache", who);
-  if (c->n_slots < 1 || c->n_heads < 1 || c->n_heads > 4096 || c->n_blocks < 1 || c->n_blocks > (INT32_MAX >> 6) - 1)
+  if (c->n_slots < 1 || c->n_heads < 1 || c->n_heads > 4096 || c->n_blocks < 1 || c->n_blocks > 1 << 24)
     return e->fail(WDZ_EINVAL, "%s: a cache of %d slots, %d heads, %d blocks", who, c->n_slots, c->n_heads, c->n_blocks);
   const int64_t blocks = (int64_t)c->n_heads * c->n_blocks;
   if (c->slot_stride < blocks * QC_BLOCK * QC_HD || c->scale_slot_stride < blocks)
