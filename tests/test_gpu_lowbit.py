@@ -499,6 +499,25 @@ def test_linear_range_and_nan(eng, dtype):
         assert (~pair[0].isfinite()).all() and torch.equal(pair[1], eng.linear_rows_packed(x[[other]].cuda(), packed)[0])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("k", [384, 381, 9001])
+@pytest.mark.parametrize("m", [1, 2, 3, 9])
+def test_linear_of_infinities_is_what_the_formula_gives(eng, m, k, dtype):
+    """One infinity times a weight is an infinity of its sign, times a weight of zero NaN; two of them may cancel to NaN."""
+    packed, w, b = _packed(70, k, 64, seed=m, bias=dtype)
+    inf = float("inf")
+    for places in ({5: inf}, {k - 1: -inf}, {0: inf, k - 1: inf}, {k // 2: -inf, 7: inf}, {k - 2: float("nan")}):
+        x = torch.randn(m, k, generator=torch.Generator().manual_seed(k)).to(dtype)
+        for at, v in places.items():
+            x[m - 1, at] = v
+        got = eng.linear_rows_packed(x.cuda(), packed).double().cpu().numpy()
+        with np.errstate(invalid="ignore"):
+            want = (x[m - 1].double().numpy() * w).sum(1)
+        assert not np.isfinite(want).any()
+        np.testing.assert_array_equal(got[m - 1], want)   # NaN where NaN is wanted, and the same infinities
+        assert np.isfinite(got[:m - 1]).all()
+
+
 def test_pack_linear_on_the_device_is_the_same(eng):
     w = torch.randn(40, 333, generator=torch.Generator().manual_seed(0))
     a, b = pack_linear(w, 64), pack_linear(w.cuda(), 64)
