@@ -29,7 +29,7 @@ extern "C" {
 #define WDZ_ECUDA (-3)     /* a CUDA call failed */
 #define WDZ_ESTATE (-4)    /* engine not finalized, or a tensor was never bound */
 #define WDZ_ECAPACITY (-5) /* more clips / rows / slots than the engine was built for */
-#define WDZ_ENAN (-6)      /* a row of logits held NaN */
+#define WDZ_ENAN (-6)      /* a row of logits held NaN; a row stored into an 8-bit cache was not finite */
 #define WDZ_ETIMEOUT (-7)  /* a bounded device-side wait ran out */
 
 #define WDZ_F32 0
@@ -117,9 +117,13 @@ int wdz_bind(wdz_engine* e, const char* name, const void* dev, int64_t numel);
 int wdz_finalize(wdz_engine* e);
 const char* wdz_last_error(const wdz_engine* e);
 const char* wdz_version(void);
-/* Reads and clears the device-side error word (WDZ_OK, WDZ_ENAN, WDZ_ETIMEOUT).
- * Synchronises the stream. */
+/* Reads the device-side error words and clears the one that it tells of (WDZ_OK: there is none left).  The engine's
+ * own kernels leave WDZ_ENAN or WDZ_ETIMEOUT; the operators on caller-held memory (wdz_qcache_*) have words of their own,
+ * for waits that ran out (WDZ_ETIMEOUT, told before all else) and for what they were given (WDZ_EINVAL, WDZ_ENAN, told
+ * last).  Of several reports in one word the first stands.  Synchronises the stream. */
 int wdz_device_status(wdz_engine* e, wdz_stream s);
+/* The same for the engine's own word alone: what a decode loop asks after a step. */
+int wdz_decode_status(wdz_engine* e, wdz_stream s);
 
 /* ---- measurement (no counterpart in the reference, which ships no profiling) ---- */
 #define WDZ_PROF_CROSS_ATTN 0 /* decode cross-attention kernel; work = K/V bytes read */
@@ -253,8 +257,8 @@ int wdz_ts_first(wdz_engine* e, const float* logits_dev, const int32_t* slot_ids
 int wdz_ts_steps(wdz_engine* e, const int32_t* slot_ids_dev, int n, int k, wdz_stream s);
 /* Copies all slot states to host (24 x int32 per slot: max_new, n_new, timing_count, last_timing,
  * last_was_timing, n_recent, done, last_token, recent[10], 6 spare).  Synchronises the stream.
- * The device status word is read in the same round trip: when a kernel since the last poll gave up a
- * bounded wait or met a NaN logits row, the call returns that code (WDZ_ETIMEOUT, WDZ_ENAN) and clears it. */
+ * The engine's own status word (wdz_decode_status) is read in the same round trip: when a kernel since the last
+ * poll gave up a bounded wait or met a NaN logits row, the call returns that code (WDZ_ETIMEOUT, WDZ_ENAN) and clears it. */
 int wdz_ts_poll(wdz_engine* e, int32_t* out_host, wdz_stream s);
 /* Copies the first cap generated tokens of one slot to host.  Synchronises the stream. */
 int wdz_ts_tokens(wdz_engine* e, int slot, int32_t* out_host, int cap, wdz_stream s);

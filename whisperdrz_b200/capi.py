@@ -68,6 +68,7 @@ SYMBOLS = {
     "wdz_last_error": (C.c_char_p, [P]),
     "wdz_version": (C.c_char_p, []),
     "wdz_device_status": (I, [P, P]),
+    "wdz_decode_status": (I, [P, P]),
     "wdz_launch_count": (I, [P, C.POINTER(I64)]),
     "wdz_profile": (I, [P, I]),
     "wdz_profile_read": (I, [P, I, C.POINTER(C.c_double), C.POINTER(I64), C.POINTER(C.c_double)]),

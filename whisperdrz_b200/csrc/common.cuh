@@ -97,10 +97,13 @@ __device__ __forceinline__ float gelu_fast(float x) {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// Device-side error word shared by all kernels of an engine (0 = fine).
+// Device-side error words of an engine (code 0 = fine).  The engine's own kernels (encoder, decode loop, alignment) share one;
+// the operators on caller-held memory have two of theirs, so that what they are given never looks like a failed step, and a
+// wait that ran out is never hidden behind a value that was not finite.
 struct DevStatus {
   int code;
   int detail;
 };
+enum { STATUS_ENGINE, STATUS_OP_WAIT, STATUS_OP_DATA, STATUS_WORDS };
 
 }  // namespace wdz

@@ -196,7 +196,7 @@ size_t carve(wdz_engine* e, char* base) {
   };
   const int64_t B = c.max_clips, Ta = c.n_audio_ctx, da = c.n_audio_state, R = c.max_rows, dt = c.n_text_state;
   const int H = c.n_text_head;
-  e->status = (DevStatus*)take(sizeof(DevStatus));
+  e->status = (DevStatus*)take(sizeof(DevStatus) * STATUS_WORDS);
   e->mel_raw = (float*)take(sizeof(float) * B * c.n_mels * MEL_MAX_FRAMES);
   e->clipmax = (int*)take(sizeof(int) * B);
   e->col1 = take(es * B * 2 * Ta * 3 * c.n_mels);
@@ -980,7 +980,7 @@ int wdz_set_workspace(wdz_engine* e, void* dev, size_t bytes) {
   carve(e, base);
   e->ws = base;
   e->ws_bytes = bytes;
-  if (cudaMemset(e->status, 0, sizeof(DevStatus)) != cudaSuccess ||
+  if (cudaMemset(e->status, 0, sizeof(DevStatus) * STATUS_WORDS) != cudaSuccess ||
       cudaMemset(e->att_counters, 0, sizeof(int) * e->cfg.max_rows) != cudaSuccess) {
     cudaGetLastError();
     return e->fail(WDZ_ECUDA, "cannot clear the status word");
@@ -1160,23 +1160,30 @@ int wdz_finalize(wdz_engine* e) {
   return WDZ_OK;
 }
 
-int wdz_device_status(wdz_engine* e, wdz_stream s) {
+namespace {
+// Reads the status words, the operators' too or the engine's alone, and clears the one that it tells of.
+int read_status(wdz_engine* e, bool operators, cudaStream_t st) {
   int rc = check_ready(e);
   if (rc) return rc;
-  DevStatus h{};
-  cudaStream_t st = (cudaStream_t)s;
-  if (cudaMemcpyAsync(&h, e->status, sizeof h, cudaMemcpyDeviceToHost, st) != cudaSuccess ||
+  DevStatus h[STATUS_WORDS]{};
+  if (cudaMemcpyAsync(h, e->status, sizeof h, cudaMemcpyDeviceToHost, st) != cudaSuccess ||
       cudaStreamSynchronize(st) != cudaSuccess) {
     cudaError_t ce = cudaGetLastError();
     return e->fail(WDZ_ECUDA, "status read: %s", cudaGetErrorString(ce));
   }
-  if (h.code != 0) {
-    cudaMemsetAsync(e->status, 0, sizeof(DevStatus), st);
-    cudaMemsetAsync(e->att_counters, 0, sizeof(int) * e->cfg.max_rows, st);   // a kernel that gave up may have left counts behind
-    return e->fail(h.code, "device reported status %d (detail %d)", h.code, h.detail);
+  for (int w : {STATUS_OP_WAIT, STATUS_ENGINE, STATUS_OP_DATA}) {
+    if (h[w].code == 0 || (w != STATUS_ENGINE && !operators)) continue;
+    cudaMemsetAsync(e->status + w, 0, sizeof(DevStatus), st);
+    if (w == STATUS_ENGINE)
+      cudaMemsetAsync(e->att_counters, 0, sizeof(int) * e->cfg.max_rows, st);   // a kernel that gave up may have left counts behind
+    return e->fail(h[w].code, "device reported status %d (detail %d)", h[w].code, h[w].detail);
   }
   return WDZ_OK;
 }
+}  // namespace
+
+int wdz_device_status(wdz_engine* e, wdz_stream s) { return read_status(e, true, (cudaStream_t)s); }
+int wdz_decode_status(wdz_engine* e, wdz_stream s) { return read_status(e, false, (cudaStream_t)s); }
 
 int wdz_linear(wdz_engine* e, const void* x_dev, int M, int K, const void* w_dev, const void* bias_dev, int N,
                int gelu, void* y_dev, int cuda_cores_only, wdz_stream s) {

@@ -148,7 +148,9 @@ __device__ __forceinline__ void qc_recode(int i0, int n, int step, At at, By by)
   }
 }
 
-__device__ __forceinline__ void qc_report(DevStatus* st, int code, int detail) {
+// words: the engine's status words.  The first of a kind counts until it is read.
+__device__ __forceinline__ void qc_report(DevStatus* words, int code, int detail) {
+  DevStatus* st = words + (code == WDZ_ETIMEOUT ? STATUS_OP_WAIT : STATUS_OP_DATA);
   if (atomicCAS(&st->code, 0, code) == 0) st->detail = detail;
 }
 

@@ -196,8 +196,13 @@ class Engine:
             pass
 
     def device_status(self) -> None:
-        """Raises if a kernel flagged an error (NaN logits row, exhausted wait)."""
+        """Raises if a kernel flagged an error: an exhausted wait, a NaN logits row, what the 8-bit cache was given.  Tells
+        of one at a time, so ask until it returns."""
         self._check(self.lib.wdz_device_status(self.h, self._stream()))
+
+    def decode_status(self) -> None:
+        """``device_status`` for the engine's own kernels alone: a store into somebody's 8-bit cache is no failed step."""
+        self._check(self.lib.wdz_decode_status(self.h, self._stream()))
 
     # ----------------------------------------------------------- measurement
     def launch_count(self) -> int:

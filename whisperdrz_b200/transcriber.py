@@ -474,7 +474,8 @@ class Transcriber:
             self.steps += 1
             self.launch_rows += len(active)
             self._accept(active, nxt.tolist())
-            eng.device_status()          # a kernel that gave up (bounded wait, NaN row) must not pass for a token
+            # a kernel that gave up (bounded wait, NaN row) must not pass for a token
+            getattr(eng, "decode_status", eng.device_status)()
         if self.aligner is not None:
             fin = [s for s in self.states if s.status == "finished"]
             if fin:
