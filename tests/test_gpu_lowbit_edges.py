@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from test_gpu_lowbit import _cuda_cache, _filled, eng  # noqa: F401
+from test_gpu_lowbit import _check_store, _cuda_cache, _filled, eng  # noqa: F401
 from whisperdrz_b200.capi import WdzError
 
 pytestmark = pytest.mark.gpu
@@ -45,4 +45,14 @@ def test_each_kind_of_report_is_told_and_a_wait_that_ran_out_first(eng):
         eng.ts_poll()
     assert "WDZ_ENAN" in str(err.value)
     eng.ts_poll()
+    eng.device_status()
+
+
+# ---------------------------------------------------------------------- store
+def test_store_of_a_padded_batch(eng):
+    g = torch.Generator().manual_seed(3)
+    rows = torch.randn(9, 128, generator=g)
+    for device_index in (True, False):
+        _check_store(eng, _filled(3, 2, 1), rows[:4], rows[4:8], [2, -1, -1, 0], [5, 0, 0, 9], device_index=device_index)
+        _check_store(eng, _filled(3, 2, 1), rows, rows.flip(0), [1, 3, 3, -1, -1], [5, 0, 0, 9, 70], [0, 4, 5, 6, 8, 9], device_index=device_index)
     eng.device_status()

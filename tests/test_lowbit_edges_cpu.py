@@ -1,6 +1,8 @@
 """CPU checks of the low-bit operators' host side: what is refused, what is let through, and what the scheduler asks for."""
+import pytest
 import torch
 
+from test_lowbit_cpu import _cache, host  # noqa: F401
 from test_scheduler_cpu import StubEngine, _patch_rules_dev
 from whisperdrz_b200.transcriber import Transcriber
 
@@ -21,3 +23,14 @@ def test_scheduler_asks_for_the_decode_loop_s_own_status():
     _patch_rules_dev(tr)
     assert len(tr.transcribe(torch.randn(16000 * 30)).raw_chunks) == 1
     assert eng.asked > 0
+
+
+def test_a_padded_batch_names_no_slot_twice(host):  # noqa: F811
+    """Runs of slots outside the cache are skipped, however many: only a slot of the cache may not come twice."""
+    rows = torch.zeros(3, 128)
+    for slots in ([0, -1, -1], [2, 2, 1], [-1, -1, -1], [5, 0, 5]):
+        with pytest.raises(AttributeError):      # as far as the library, which this host does not have
+            host.qcache_store(_cache(), rows, rows, slots, [0, 0, 0])
+    for slots in ([1, -1, 1], [0, 0, 0]):
+        with pytest.raises(ValueError):
+            host.qcache_store(_cache(), rows, rows, slots, [0, 0, 0])

@@ -480,7 +480,7 @@ class Engine:
         is rows row_begin[i] .. row_begin[i + 1] (``None``: one row a run) and goes to tokens positions[i], ... of slot
         slots[i].  A block of 64 tokens that a run enters at its first token gets the scale max|x| / 127 of the run's
         own values; one that is entered later keeps the larger of that and its scale, and what it holds is rounded to
-        it.  A slot may be named once; ``max_run`` sizes the launch when row_begin is on the device (default: all
+        it.  A slot of the cache may be named once; ``max_run`` sizes the launch when row_begin is on the device (default: all
         rows).  Non-finite values, places outside the cache and slots named twice are told by ``device_status()``;
         slots outside the cache are skipped."""
         width = cache.n_heads * HEAD_DIM
@@ -506,7 +506,8 @@ class Engine:
             most = n if max_run is None else int(max_run)
         if not isinstance(slots, torch.Tensor):
             slots = [int(x) for x in slots]
-            if len(set(slots)) != len(slots):
+            kept = [x for x in slots if 0 <= x < cache.n_slots]   # the others are skipped, however often
+            if len(set(kept)) != len(kept):
                 raise ValueError("qcache_store: a slot is named twice")
         sl, ps = self._index("slots", slots, n_runs), self._index("positions", positions, n_runs)
         if n == 0 or n_runs == 0:
