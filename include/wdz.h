@@ -358,8 +358,8 @@ int64_t wdz_qcache_attention_scratch(const wdz_engine* e, const wdz_qcache* cach
  * 128, with u = 8; row n is Kp / 8 32-bit words; of every 128 weights word 4 t + i (t, i < 4) holds elements
  * 32 i + 8 t + 0..7, element 2 j in its bits 4 j, element 2 j + 1 in its bits 4 (j + 4).  scale_dev: bf16
  * [N][Kp / group].  w_dev starts on 16 bytes, scale_dev on 8; x rows may have any alignment.  Products are exact and
- * their sums fp32; bf16 rows are held exactly down to 2^-38 of their largest value, to 2^-46 of it below.  A group's sum
- * before its scale has to fit fp32.  Infinities and NaN in x give what the formula gives, in their row. */
+ * their sums fp32; bf16 rows are held exactly down to 2^-38 of their largest value, to 2^-46 of it below.  Of f32 rows and
+ * of three bf16 rows or more, a group's sum before its scale has to fit fp32.  Scales of padding have to be finite.  Infinities and NaN in x give what the formula gives, in their row. */
 int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_dtype, int M, int K, const void* w_dev,
                            const void* scale_dev, int group, const void* bias_dev, const float* residual_dev, int N,
                            float* y_dev, wdz_stream s);

@@ -1,10 +1,12 @@
 """The low-bit operators at the ends of their ranges and on their rarer paths, on the GPU against the definitions in 64 bits
 (lowbit_ref.py).  Tolerances are those of test_gpu_lowbit.py unless a test derives its own (u = 2^-24)."""
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_lowbit import _check_store, _cuda_cache, _filled, eng  # noqa: F401
+from test_gpu_lowbit import U, _check_store, _cuda_cache, _filled, eng  # noqa: F401
 from whisperdrz_b200.capi import WdzError
+from whisperdrz_b200.lowbit import PackedLinear, pack_nibbles
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +58,49 @@ def test_store_of_a_padded_batch(eng):
         _check_store(eng, _filled(3, 2, 1), rows[:4], rows[4:8], [2, -1, -1, 0], [5, 0, 0, 9], device_index=device_index)
         _check_store(eng, _filled(3, 2, 1), rows, rows.flip(0), [1, 3, 3, -1, -1], [5, 0, 0, 9, 70], [0, 4, 5, 6, 8, 9], device_index=device_index)
     eng.device_status()
+
+
+# --------------------------------------------------------------------- linear
+def _scaled(n, k, group, seed, scale):
+    """Packed weights whose group scales are ``scale`` (a number, or one for each group) times 1 to 2."""
+    g = torch.Generator().manual_seed(seed)
+    kp = (k + 127) // 128 * 128
+    q = torch.randint(-8, 8, (n, kp), generator=g)
+    q[:, k:] = 0
+    s = ((1 + torch.rand(n, kp // group, generator=g, dtype=torch.float64)) * torch.as_tensor(scale, dtype=torch.float64)).bfloat16()
+    w = (q.numpy() * np.repeat(s.double().numpy(), group, axis=1))[:, :k]
+    return PackedLinear(pack_nibbles(q).cuda(), s.cuda(), k, group), w
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m", [1, 2])
+@pytest.mark.parametrize("x_size,scale", [(1e-20, 1e33), (1e-35, 1e36), (1e-38, 1e37), (1.0, 1e33), (1e-3, 1e34), (30.0, 1e-33),
+                                          (1e20, 1e-33), (1e35, 1e-38), (1e3, 1e30), (1e12, 1e-12)])
+def test_linear_of_far_scales(eng, x_size, scale, m, group):
+    """A result that fits fp32 comes out whatever the sizes of x and the scales; half a step of the smallest fp32 number, 2^-150,
+    for each of the sums that a result below 2^-126 passes through: 16 at most here."""
+    packed, w = _scaled(40, 300, group, seed=m, scale=scale)
+    x = (torch.randn(m, 300, generator=torch.Generator().manual_seed(5)) * x_size).bfloat16()
+    x64 = x.double().numpy()
+    want, size = x64 @ w.T, np.abs(x64) @ np.abs(w).T
+    got = eng.linear_rows_packed(x.cuda(), packed).double().cpu().numpy()
+    tol = 308 * U * size + 2.0 ** -46 * np.abs(x64).max(1, keepdims=True) * np.abs(w).sum(1) + 16 * 2.0 ** -150
+    assert size.max() < 1e38 and (np.abs(got - want) <= tol).all()
+
+
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("m", [1, 2])
+def test_linear_of_groups_with_far_scales(eng, m, group):
+    """Loud values under a small scale beside quiet ones, 2^-33 of them, under a large one that makes the result."""
+    groups = 384 // group
+    scale = torch.full((groups,), 1e-18, dtype=torch.float64)
+    scale[groups // 3:] = 1e27
+    packed, w = _scaled(40, 384, group, seed=m, scale=scale)
+    x = torch.randn(m, 384, generator=torch.Generator().manual_seed(5)) * 1e8
+    x[:, :128] *= 1e10
+    x64 = x.bfloat16().double().numpy()
+    got = eng.linear_rows_packed(x.bfloat16().cuda(), packed).double().cpu().numpy()
+    # the elementwise bound of a row in whole numbers of 2^-45 of its largest value's power of two: half of one is up to 2^-46 of
+    # 4e18, 6e4 on values of 1e8, so no bound relative to the result (1e-5 of its norm, say) follows from it here
+    tol = 392 * U * (np.abs(x64) @ np.abs(w).T) + 2.0 ** -46 * np.abs(x64).max(1, keepdims=True) * np.abs(w).sum(1)
+    assert (np.abs(got - x64 @ w.T) <= tol).all()
