@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_lowbit import U, _check_store, _cuda_cache, _filled, eng  # noqa: F401
+from test_gpu_lowbit import U, _check_attend, _check_store, _cuda_cache, _filled, eng  # noqa: F401
 from whisperdrz_b200.capi import WdzError
 from whisperdrz_b200.lowbit import PackedLinear, pack_nibbles
 
@@ -104,3 +104,24 @@ def test_linear_of_groups_with_far_scales(eng, m, group):
     # 4e18, 6e4 on values of 1e8, so no bound relative to the result (1e-5 of its norm, say) follows from it here
     tol = 392 * U * (np.abs(x64) @ np.abs(w).T) + 2.0 ** -46 * np.abs(x64).max(1, keepdims=True) * np.abs(w).sum(1)
     assert (np.abs(got - x64 @ w.T) <= tol).all()
+
+
+# ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("group", [1, 2, 4])
+@pytest.mark.parametrize("size", [1e-35, 1e-32, 1e-28, 1e-24, 1e30, 1e34])
+def test_attention_over_values_of_any_size(eng, size, group):
+    parts = _filled(3, 2, 4, seed=group)
+    parts[3].mul_(size)
+    q = torch.randn(3, 2 * group * 64, generator=torch.Generator().manual_seed(0)) * 0.3
+    _check_attend(eng, parts, q, [2, 0, 1], [250, 64, 3])
+
+
+@pytest.mark.parametrize("group", [1, 4])
+def test_attention_over_blocks_of_far_scales(eng, group):
+    parts = _filled(2, 2, 40, seed=group)
+    size = torch.ones(2, 2, 40, dtype=torch.float64)
+    size[0], size[0, :, 17:19], size[1, 1, 30] = 1e-28, 1e30, 1e36
+    parts = (*parts[:3], (parts[3] * size).float())
+    q = torch.randn(2, 2 * group * 64, generator=torch.Generator().manual_seed(0)) * 0.3
+    for lens in ([1088, 1920], [2500, 2560], [1089, 1921]):
+        _check_attend(eng, parts, q, [0, 1], lens)

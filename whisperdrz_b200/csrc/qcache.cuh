@@ -464,6 +464,7 @@ struct QcAttendParams {
 constexpr int QC_MAX_WARPS = 4;   // of a CTA
 constexpr float QC_STEPS = 127.0f * 16777216.0f;   // a query's largest value in steps: rounding up leaves d3 a byte
 constexpr float QC_ONE = 4294967040.0f;            // the weight 1 in steps: the largest fp32 below 2^32
+constexpr float QC_LARGE = 18446744073709551616.0f;   // 2^64: block scales up to here are summed as they are
 
 // A signed, B unsigned; the first of a sum starts from zeros.
 __device__ __forceinline__ void qc_mma_su(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -633,7 +634,7 @@ __device__ __forceinline__ void qc_query(const QcAttendParams& p, int r, int hk,
 template <int NT, bool ONE, typename Release, typename Behind>
 __device__ __forceinline__ bool qc_tile(QcRing& ring, int tokens, int g, int t, const uint32_t (&qb)[NT][4],
                                         const float (&q_mul)[NT], float (&m)[NT], float (&l)[NT], float (&acc)[NT][8],
-                                        DevStatus* status, Release release, Behind behind) {
+                                        float& shrink, DevStatus* status, Release release, Behind behind) {
   if (!ring.wait(behind(), status)) return false;
   uint32_t pb[NT][4];      // the weights' bytes: word 2 ks + r
   float alpha[NT];
@@ -703,7 +704,17 @@ __device__ __forceinline__ bool qc_tile(QcRing& ring, int tokens, int g, int t, 
     }
   }
   if (!ring.wait(behind(), status)) return false;
-  const float v_now = ring.scale() * ((t & 1 ? 65536.0f : 1.0f) / QC_ONE);
+  // acc counts in the weights' steps times 1 / shrink: a step's share of a block's scale would underflow for values below
+  // 1e-32, and the sums of scales above 2^64 might overflow, so from the first such block on they are 2^-64 of that.
+  float v_now = ring.scale() * shrink;
+  if (v_now > QC_LARGE) {
+    shrink = 1.0f / QC_LARGE;
+    v_now *= 1.0f / QC_LARGE;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[nt][i] *= 1.0f / QC_LARGE;
+  }
   const uint8_t* vt = ring.data() + t * QC_HD + 8 * g;
   // V's bytes, four tokens of one value to a word: a[2 ks + r][value 8 g + i]
   uint32_t a[4][8];
@@ -785,7 +796,7 @@ __global__ void __launch_bounds__(QC_MAX_WARPS * 32) qcache_attend_kernel(QcAtte
   uint32_t qb[NT][4];
   float q_mul[NT];
   qc_query<TQ, NT>(p, row.r, row.hk, g, t, qb, q_mul);
-  float m[NT], l[NT], acc[NT][8];
+  float m[NT], l[NT], acc[NT][8], shrink = 1.0f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     m[nt] = -INFINITY; l[nt] = 0.0f;
@@ -794,11 +805,12 @@ __global__ void __launch_bounds__(QC_MAX_WARPS * 32) qcache_attend_kernel(QcAtte
   }
   int taken = 0;
   for (int i = 0; i < mine; ++i) {
-    if (!qc_tile<NT, ONE>(ring, row.tokens(tile0 + i * stride), g, t, qb, q_mul, m, l, acc, status, fetch,
+    if (!qc_tile<NT, ONE>(ring, row.tokens(tile0 + i * stride), g, t, qb, q_mul, m, l, acc, shrink, status, fetch,
                           [&] { return asked - ++taken; })) break;
   }
 
   // the warp's partial results
+  const float step = (t & 1 ? 65536.0f : 1.0f) / QC_ONE * (shrink < 1.0f ? QC_LARGE : 1.0f);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], 4);
@@ -807,7 +819,7 @@ __global__ void __launch_bounds__(QC_MAX_WARPS * 32) qcache_attend_kernel(QcAtte
     float* dst = warp_part + warp * STEP + (2 * nt + (t >> 1)) * (QC_HD + 2);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float o = acc[nt][i] + __shfl_xor_sync(0xffffffffu, acc[nt][i], 1);
+      const float mine = acc[nt][i] * step, o = mine + __shfl_xor_sync(0xffffffffu, mine, 1);
       if (!(t & 1)) dst[8 * g + i] = o;
     }
     if (g == 0 && !(t & 1)) { dst[QC_HD] = m[nt]; dst[QC_HD + 1] = l[nt]; }
