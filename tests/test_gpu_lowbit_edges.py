@@ -125,3 +125,10 @@ def test_attention_over_blocks_of_far_scales(eng, group):
     q = torch.randn(2, 2 * group * 64, generator=torch.Generator().manual_seed(0)) * 0.3
     for lens in ([1088, 1920], [2500, 2560], [1089, 1921]):
         _check_attend(eng, parts, q, [0, 1], lens)
+
+
+def test_attention_with_the_largest_scale(eng):
+    """Tiny queries times a scale near the largest number: scores of ordinary size."""
+    parts = _filled(3, 2, 2, seed=3)
+    q = torch.randn(3, 128, generator=torch.Generator().manual_seed(0)) * 1e-38
+    _check_attend(eng, parts, q, [2, 0, 1], [128, 64, 3], scale=2.9e38)

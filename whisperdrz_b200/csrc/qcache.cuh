@@ -624,7 +624,7 @@ __device__ __forceinline__ void qc_query(const QcAttendParams& p, int r, int hk,
       qb[nt][w] = __byte_perm(__byte_perm(n[0], n[1], digit), __byte_perm(n[2], n[3], digit), 0x5410) ^ 0x80808080u;
     }
     // an infinite or NaN query: infinity times zero makes the row NaN
-    const float mul = (top * lift) * (1.0f / QC_STEPS) * (p.scale * 1.4426950408889634f) / lift;
+    const float mul = (top * lift) * (1.4426950408889634f / QC_STEPS) * p.scale / lift;   // the scale alone may be 3e38
     q_mul[nt] = __shfl_sync(0xffffffffu, mul, 16 * (t >> 1)) * (t & 1 ? 65536.0f : 1.0f);   // of the head whose scores this lane gets
   }
 }
