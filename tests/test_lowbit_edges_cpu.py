@@ -2,8 +2,9 @@
 import pytest
 import torch
 
-from test_lowbit_cpu import _cache, host  # noqa: F401
+from test_lowbit_cpu import _cache, handle, host, lib  # noqa: F401
 from test_scheduler_cpu import StubEngine, _patch_rules_dev
+from whisperdrz_b200 import capi
 from whisperdrz_b200.transcriber import Transcriber
 
 
@@ -34,3 +35,13 @@ def test_a_padded_batch_names_no_slot_twice(host):  # noqa: F811
     for slots in ([1, -1, 1], [0, 0, 0]):
         with pytest.raises(ValueError):
             host.qcache_store(_cache(), rows, rows, slots, [0, 0, 0])
+
+
+def test_linear_refuses_features_that_its_places_cannot_count(lib, handle):  # noqa: F811
+    """A block covers up to 128 features at places of 32 bits: the last of nearly 2^31 would have wrapped below zero.  The
+    addresses are never followed."""
+    def linear(N):
+        return lib.wdz_linear_rows_packed(handle, 4096, 128, capi.WDZ_BF16, 1, 128, 4096, 4096, 64, None, None, N, 4096, None)
+
+    assert linear(2 ** 31 - 1) == -1 and linear(2 ** 31 - 128) == -1
+    assert linear(2 ** 31 - 129) == -4       # as far as the engine, which is not ready

@@ -2095,7 +2095,8 @@ int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_
   if (!e) return WDZ_EINVAL;
   int rc;
   if (x_dtype != WDZ_F32 && x_dtype != WDZ_BF16) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: unknown type %d", x_dtype);
-  if (M < 0 || N < 1 || K < 1 || K > INT32_MAX - 128) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: %d x %d x %d", M, N, K);
+  // the last block's features and the padded inputs are counted in 32 bits
+  if (M < 0 || N < 1 || N > INT32_MAX - 128 || K < 1 || K > INT32_MAX - 128) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: %d x %d x %d", M, N, K);
   if (group != 32 && group != 64 && group != 128) return e->fail(WDZ_EINVAL, "wdz_linear_rows_packed: group %d (32, 64 or 128)", group);
   if (M > 8 * 65535) return e->fail(WDZ_ECAPACITY, "wdz_linear_rows_packed: %d rows in one call, at most %d", M, 8 * 65535);
   if (M == 0) return WDZ_OK;
