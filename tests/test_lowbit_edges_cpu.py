@@ -45,3 +45,20 @@ def test_linear_refuses_features_that_its_places_cannot_count(lib, handle):  # n
 
     assert linear(2 ** 31 - 1) == -1 and linear(2 ** 31 - 128) == -1
     assert linear(2 ** 31 - 129) == -4       # as far as the engine, which is not ready
+
+
+def test_rows_of_three_dimensions_are_heads_of_64(host):  # noqa: F811
+    """[n, heads, 64] only: other splits of the same width lie in another order."""
+    rows, q = torch.zeros(3, 2, 64), torch.zeros(3, 4, 64)
+    for call in (lambda: host.qcache_store(_cache(), rows, rows, [0, 1, 2], [0, 0, 0]),
+                 lambda: host.qcache_store(_cache(), rows.view(3, 128), rows, [0, 1, 2], [0, 0, 0]),
+                 lambda: host.qcache_attention(q, _cache(), [0, 1, 1], [1, 1, 1])):
+        with pytest.raises(AttributeError):      # as far as the library, which this host does not have
+            call()
+    for bad in (rows.transpose(1, 2), rows.view(3, 1, 128), rows.view(3, 4, 32)):
+        with pytest.raises(ValueError):
+            host.qcache_store(_cache(), bad, rows, [0, 1, 2], [0, 0, 0])
+        with pytest.raises(ValueError):
+            host.qcache_store(_cache(), rows, bad, [0, 1, 2], [0, 0, 0])
+        with pytest.raises(ValueError):
+            host.qcache_attention(bad, _cache(), [0, 1, 1], [1, 1, 1])

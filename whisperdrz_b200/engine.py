@@ -452,7 +452,7 @@ class Engine:
 
     def _rows(self, name: str, t: torch.Tensor, width: int) -> torch.Tensor:
         """``t`` as rows [n, width] in a type and at places that the kernels take: no copy where it has them already."""
-        if t.dim() == 3:
+        if t.dim() == 3 and t.shape[2] == HEAD_DIM:
             t = t.flatten(1)
         if t.dtype not in _TORCH_DTYPE or t.dim() != 2 or t.shape[1] != width:
             raise ValueError(f"{name} must be [rows, {width}] in float32 or bfloat16, got {t.dtype} {tuple(t.shape)}")
@@ -527,10 +527,10 @@ class Engine:
         to 8, consecutive query heads sharing a key head.  Returns [n, q_heads * 64] in ``out_dtype`` (default: the
         engine's type), or fills ``out``.  Length 0 gives zeros; a row whose slot lies outside the cache is left as it
         was (zeros when ``out`` is not given)."""
-        if q.dim() == 3:
+        if q.dim() == 3 and q.shape[2] == HEAD_DIM:
             q = q.flatten(1)
         elif q.dim() != 2:
-            raise ValueError(f"q must be [rows, q_heads * {HEAD_DIM}], got {tuple(q.shape)}")
+            raise ValueError(f"q must be [rows, q_heads * {HEAD_DIM}] or [rows, q_heads, {HEAD_DIM}], got {tuple(q.shape)}")
         n, width = q.shape
         shared, rest = divmod(width, cache.n_heads * HEAD_DIM)
         if rest or not 1 <= shared <= 8:
