@@ -1,4 +1,5 @@
 """CPU checks of the low-bit operators' host side: what is refused, what is let through, and what the scheduler asks for."""
+import numpy
 import pytest
 import torch
 
@@ -62,3 +63,22 @@ def test_rows_of_three_dimensions_are_heads_of_64(host):  # noqa: F811
             host.qcache_store(_cache(), rows, bad, [0, 1, 2], [0, 0, 0])
         with pytest.raises(ValueError):
             host.qcache_attention(bad, _cache(), [0, 1, 1], [1, 1, 1])
+
+
+def test_index_tensors_keep_what_they_say(host):  # noqa: F811
+    """64-bit entries that no int32 holds stay outside the cache instead of wrapping into it; lengths stay long."""
+    far = torch.tensor([2 ** 32 + 1, -2 ** 32, 2 ** 31, 5, -1])
+    assert host._index("slots", far, 5).tolist() == [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 5, -1]
+    for t in (torch.uint8, torch.int16, torch.int32, torch.int64):
+        x = host._index("lens", torch.tensor([3, 0], dtype=t), 2)
+        assert x.dtype == torch.int32 and x.tolist() == [3, 0]
+    for bad in (torch.tensor([1.5, 2.0]), torch.tensor([True, False]), [1.5, 2.0], torch.tensor([1, 2, 3]), [1]):
+        with pytest.raises(ValueError):
+            host._index("slots", bad, 2)
+    assert host._index("slots", [1, 2], 2).tolist() == [1, 2]
+    assert host._index("slots", numpy.array([1, 2]), 2).tolist() == [1, 2]
+    rows = torch.zeros(2, 128)
+    with pytest.raises(ValueError):
+        host.qcache_store(_cache(), rows, rows, [0.5, 1], [0, 0])
+    with pytest.raises(ValueError):
+        host.qcache_store(_cache(), rows, rows, [0], [0], row_begin=[0, 1.5])

@@ -463,13 +463,29 @@ class Engine:
         return t
 
     def _index(self, name: str, x, n: int) -> torch.Tensor:
-        """An int32 index tensor of ``n`` entries on the device; host sequences are uploaded."""
+        """An int32 index tensor of ``n`` entries on the device; host sequences are uploaded.  Entries that no int32 holds
+        become its ends: outside every cache, longer than every row."""
         if isinstance(x, torch.Tensor) and x.dtype is torch.int32 and x.numel() == n and x.is_contiguous() and x.get_device() == self._ordinal:
             return x
+        lo, hi = -2 ** 31, 2 ** 31 - 1
+        if not isinstance(x, torch.Tensor):
+            x = [min(max(v, lo), hi) for v in self._whole(name, x)]
+        elif x.dtype is torch.bool or x.is_floating_point() or x.is_complex():
+            raise ValueError(f"{name} must be whole numbers, got {x.dtype}")
+        elif x.dtype is torch.int64:
+            x = x.clamp(lo, hi)
         x = self._i32(x)
         if x.numel() != n:
             raise ValueError(f"{name} must have {n} entries, got {tuple(x.shape)}")
         return x
+
+    @staticmethod
+    def _whole(name: str, values) -> list[int]:
+        values = list(values)
+        whole = [int(v) for v in values]
+        if any(w != v for w, v in zip(whole, values)):
+            raise ValueError(f"{name} must be whole numbers")
+        return whole
 
     def qcache_store(self, cache: QCache, k: torch.Tensor, v: torch.Tensor, slots, positions, row_begin=None,
                      max_run: int | None = None) -> None:
@@ -494,7 +510,7 @@ class Engine:
             n_runs, most = n, 1
         else:
             if not isinstance(row_begin, torch.Tensor):
-                row_begin = [int(b) for b in row_begin]
+                row_begin = self._whole("row_begin", row_begin)
                 if not row_begin or row_begin[0] < 0 or row_begin[-1] > n or any(b > c for b, c in zip(row_begin, row_begin[1:])):
                     raise ValueError(f"row_begin must rise from 0 or more to at most {n}")
                 if max_run is None:
@@ -505,7 +521,7 @@ class Engine:
             rb = self._index("row_begin", row_begin, n_runs + 1)
             most = n if max_run is None else int(max_run)
         if not isinstance(slots, torch.Tensor):
-            slots = [int(x) for x in slots]
+            slots = self._whole("slots", slots)
             kept = [x for x in slots if 0 <= x < cache.n_slots]   # the others are skipped, however often
             if len(set(kept)) != len(kept):
                 raise ValueError("qcache_store: a slot is named twice")
