@@ -344,7 +344,7 @@ int wdz_qcache_store(wdz_engine* e, const wdz_qcache* cache, const void* k_dev, 
 /* Row r's n_q_heads queries (q_dtype [n_rows][n_q_heads * 64]) attend to the first lens_dev[r] tokens of slot
  * slot_ids_dev[r]: out = softmax(scale * q k^T) v, query head h over key head h / (n_q_heads / n_heads), at most 8
  * query heads to a key head.  Queries and softmax weights are held to 2^-31 of the largest of their head or row,
- * everything else in fp32; out: out_dtype [n_rows][n_q_heads * 64], which may be q itself.  Lengths are clamped to
+ * everything else in fp32; out: out_dtype [n_rows][n_q_heads * 64], which may be q itself (its rows and type) and overlaps it in no other way.  Lengths are clamped to
  * the slot; a row of length 0 gives zeros; a row whose slot is outside [0, n_slots) is left as it was, or zeroed
  * when clear_skipped != 0. */
 int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_dev, int64_t ldq, int q_dtype, int n_q_heads,
@@ -354,7 +354,7 @@ int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_d
  * above takes a few long rows apart over all SMs; 0 where it wants none.  Without it those rows are slower. */
 int64_t wdz_qcache_attention_scratch(const wdz_engine* e, const wdz_qcache* cache, int n_q_heads, int n_rows);
 /* wdz_linear_rows with 4-bit weights: y f32 [M][N] = x[M][K] W^T (+ bias, x_dtype [N]) (+ residual f32 [M][N], which
- * may be y), W[n][k] = (u - 8) * scale[n][k / group], group 32, 64 or 128.  w_dev: K is padded to Kp, a multiple of
+ * may be y; y overlaps x and the residual in no other way), W[n][k] = (u - 8) * scale[n][k / group], group 32, 64 or 128.  w_dev: K is padded to Kp, a multiple of
  * 128, with u = 8; row n is Kp / 8 32-bit words; of every 128 weights word 4 t + i (t, i < 4) holds elements
  * 32 i + 8 t + 0..7, element 2 j in its bits 4 j, element 2 j + 1 in its bits 4 (j + 4).  scale_dev: bf16
  * [N][Kp / group].  w_dev starts on 16 bytes, scale_dev on 8; x rows may have any alignment.  Products are exact and

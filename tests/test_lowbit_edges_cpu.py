@@ -6,6 +6,7 @@ import torch
 from test_lowbit_cpu import _cache, handle, host, lib  # noqa: F401
 from test_scheduler_cpu import StubEngine, _patch_rules_dev
 from whisperdrz_b200 import capi
+from whisperdrz_b200.lowbit import pack_linear
 from whisperdrz_b200.transcriber import Transcriber
 
 
@@ -82,3 +83,33 @@ def test_index_tensors_keep_what_they_say(host):  # noqa: F811
         host.qcache_store(_cache(), rows, rows, [0.5, 1], [0, 0])
     with pytest.raises(ValueError):
         host.qcache_store(_cache(), rows, rows, [0], [0], row_begin=[0, 1.5])
+
+
+def test_results_may_not_lie_over_what_is_still_read(host):  # noqa: F811
+    """Blocks of a launch read x and q while others write: in place means the queries' own rows, or the residual."""
+    w = pack_linear(torch.zeros(128, 128))
+    x = torch.zeros(4, 128)
+    buf = torch.zeros(9, 128)
+    good = (dict(x=x), dict(x=x, out=torch.zeros(4, 128), residual=x), dict(x=x, out=buf[4:8], residual=buf[4:8]),
+            dict(x=buf[:4], out=buf[4:8]), dict(x=buf[:4].bfloat16(), out=buf[:4]), dict(x=buf[:4], out=buf[4:8], residual=buf[:4]))
+    bad = (dict(x=x, out=x), dict(x=buf[:4], out=buf[3:7]), dict(x=buf[4:8], out=buf[1:5]), dict(x=x, out=buf[:4], residual=buf[1:5]))
+    for kw in good:
+        with pytest.raises(AttributeError):      # as far as the library, which this host does not have
+            host.linear_rows_packed(w=w, **kw)
+    for kw in bad:
+        with pytest.raises(ValueError):
+            host.linear_rows_packed(w=w, **kw)
+    p = torch.zeros(4, 384)                      # a fused product
+    half = torch.zeros(8, 128, dtype=torch.bfloat16)
+    good = (dict(q=p[:, :128], out=p[:, :128]), dict(q=p[:, :128], out=p[:, 128:256]), dict(q=p[:, 256:], out=p[:, :128]), dict(q=p[:2, :128], out=p[2:, :128]),
+            dict(q=p[:1, :128], out=p[0:1, 128:256]), dict(q=half[:4], out=half[4:]), dict(q=p[:, 128:256], out=torch.zeros(4, 128)))
+    bad = (dict(q=p[:, :128], out=p[:, 64:192]), dict(q=p[:3, :128], out=p[1:, :128]), dict(q=p[:, 64:192], out=p[:, :128]), dict(q=half[:4], out=half[1:5]),
+           dict(q=x.view(-1).view(torch.bfloat16).view(8, 128)[:4], out=x), dict(q=p[1:, :128], out=p[:3, 64:192]))
+    for kw in good:
+        n = kw["q"].shape[0]
+        with pytest.raises(AttributeError):
+            host.qcache_attention(cache=_cache(4), slots=[0, 1, 2, 3][:n], lens=[1] * n, **kw)
+    for kw in bad:
+        n = kw["q"].shape[0]
+        with pytest.raises(ValueError):
+            host.qcache_attention(cache=_cache(4), slots=[0, 1, 2, 3][:n], lens=[1] * n, **kw)

@@ -16,6 +16,22 @@ from .lowbit import HEAD_DIM, PackedLinear, QCache
 _TORCH_DTYPE = {torch.float32: capi.WDZ_F32, torch.bfloat16: capi.WDZ_BF16}
 
 
+def _rows_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether a byte of one's rows is a byte of the other's.  Rows [n, width] with unit stride, none over another of its own."""
+    n = a.shape[0]
+    if n == 0:
+        return False
+    pa, pb = a.data_ptr(), b.data_ptr()
+    wa, wb = a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
+    sa = a.stride(0) * a.element_size() if n > 1 else wa
+    sb = b.stride(0) * b.element_size() if n > 1 else wb
+    if pa + (n - 1) * sa + wa <= pb or pb + (n - 1) * sb + wb <= pa:
+        return False
+    if sa == sb and wa <= (pb - pa) % sa <= sa - wb:     # columns of one product
+        return False
+    return any(max(0, (lo - wa - pa) // sa + 1) <= min(n - 1, (lo + wb - 1 - pa) // sa) for lo in range(pb, pb + n * sb, sb))
+
+
 def pack_weights(sd: dict, dims: ModelDimensions, dtype: torch.dtype, device) -> dict[str, torch.Tensor]:
     """Reference state_dict (model.py names) -> the tensors the engine binds:
     q/k/v stacked per attention (key bias = 0, model.py:259), conv kernels
@@ -541,7 +557,7 @@ class Engine:
 
         q: f32 or bf16 [n, q_heads * 64] (or [n, q_heads, 64]); q_heads is the cache's head count or a multiple of it up
         to 8, consecutive query heads sharing a key head.  Returns [n, q_heads * 64] in ``out_dtype`` (default: the
-        engine's type), or fills ``out``.  Length 0 gives zeros; a row whose slot lies outside the cache is left as it
+        engine's type), or fills ``out``, which may be q itself.  Length 0 gives zeros; a row whose slot lies outside the cache is left as it
         was (zeros when ``out`` is not given)."""
         if q.dim() == 3 and q.shape[2] == HEAD_DIM:
             q = q.flatten(1)
@@ -574,6 +590,9 @@ class Engine:
                 raise ValueError(f"out must be [{n}, {width}] rows in float32 or bfloat16 that start on 16 bytes")
             self._here("out", out.get_device())
             out_step = out.stride(0)
+            same = out.data_ptr() == at and to == code and (n == 1 or out_step == step)
+            if not same and _rows_overlap(q, out):
+                raise ValueError("out may be q itself, but not lie over a part of it")
         slots, lens = self._index("slots", slots, n), self._index("lens", lens, n)
         if n == 0:
             return out
@@ -591,7 +610,7 @@ class Engine:
     def linear_rows_packed(self, x: torch.Tensor, w: PackedLinear, residual: torch.Tensor | None = None,
                            out: torch.Tensor | None = None) -> torch.Tensor:
         """``linear_rows`` with 4-bit weights (``lowbit.pack_linear``): x f32 or bf16 [M, K] @ W[N, K].T (+ bias)
-        (+ residual f32 [M, N]) -> f32 [M, N].  ``residual`` and ``out`` may be the same tensor."""
+        (+ residual f32 [M, N]) -> f32 [M, N].  ``residual`` and ``out`` may be the same tensor; ``out`` may not lie over x."""
         code, ordinal = _TORCH_DTYPE.get(x.dtype), self._ordinal
         if code is None or x.dim() != 2:
             raise ValueError(f"x must be [rows, {w.in_features}] in float32 or bfloat16, got {x.dtype} {tuple(x.shape)}")
@@ -612,6 +631,8 @@ class Engine:
             out = x.new_empty((M, N), dtype=torch.float32)
         else:
             self._f32_rows("out", out, M, N)
+            if _rows_overlap(x, out) or (residual is not None and add != out.data_ptr() and _rows_overlap(residual, out)):
+                raise ValueError("out may be residual itself, but not lie over x or a part of residual")
         b = w.bias
         if b is not None and b.dtype is not x.dtype:
             b = b.to(x.dtype)
