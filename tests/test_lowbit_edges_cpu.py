@@ -113,3 +113,16 @@ def test_results_may_not_lie_over_what_is_still_read(host):  # noqa: F811
         n = kw["q"].shape[0]
         with pytest.raises(ValueError):
             host.qcache_attention(cache=_cache(4), slots=[0, 1, 2, 3][:n], lens=[1] * n, **kw)
+
+
+def test_operands_keep_the_tensors_that_their_addresses_belong_to():
+    """The kernels get addresses taken when the operand was made: another tensor in its place would leave them dangling."""
+    c, w = _cache(), pack_linear(torch.zeros(4, 128), bias=torch.zeros(4))
+    for name in ("k", "v", "k_scale", "v_scale"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, getattr(c, name).clone())
+        assert getattr(c.desc, name) == getattr(c, name).data_ptr()
+    for name in ("weight", "scale"):
+        with pytest.raises(AttributeError):
+            setattr(w, name, getattr(w, name).clone())
+    assert (w.at, w.scale_at) == (w.weight.data_ptr(), w.scale.data_ptr())

@@ -15,10 +15,17 @@ HEAD_DIM = 64
 SEGMENT = 128   # weights of a row that are packed together
 
 
+def _fixed(name: str) -> property:
+    """A tensor whose address the operand has handed on: it may be written into, not replaced."""
+    return property(lambda self: self.__dict__["_" + name])
+
+
 class QCache:
     """An 8-bit cache by its tensors: ``k`` / ``v`` int8 [n_slots, n_heads, 64 * n_blocks, 64], ``k_scale`` / ``v_scale``
     f32 [n_slots, n_heads, n_blocks].  A token's values are its int8 times the scale of its block of 64 tokens.  Slots may
     lie further apart than their size (a layer of a larger allocation); K and V alike."""
+
+    k, v, k_scale, v_scale = map(_fixed, ("k", "v", "k_scale", "v_scale"))
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.dim() != 4 or k.shape[3] != HEAD_DIM or k.shape[2] == 0 or k.shape[2] % BLOCK or k.shape != v.shape:
@@ -44,7 +51,7 @@ class QCache:
             raise ValueError("QCache: the slots overlap")
         if step % 16 or k.data_ptr() % 16 or v.data_ptr() % 16:
             raise ValueError("QCache: values must start on 16 bytes")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
         self.n_slots, self.n_heads, self.n_tokens, self.device, self.ordinal = n_slots, n_heads, n_tokens, k.device, k.get_device()
         self.desc = capi.QCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), step, scale_step,
                                     n_slots, n_heads, n_tokens // BLOCK)
@@ -65,6 +72,8 @@ class PackedLinear:
     (wdz_linear_rows_packed), ``scale`` bf16 [N, Kp / group], optional ``bias`` [N]; Kp is ``in_features`` rounded up
     to a multiple of 128."""
 
+    weight, scale = map(_fixed, ("weight", "scale"))
+
     def __init__(self, weight: torch.Tensor, scale: torch.Tensor, in_features: int, group: int, bias: torch.Tensor | None = None):
         if group not in (32, 64, 128):
             raise ValueError(f"PackedLinear: groups of 32, 64 or 128 weights, got {group}")
@@ -79,7 +88,7 @@ class PackedLinear:
             raise ValueError("PackedLinear: the tensors lie on different devices")
         if not weight.is_contiguous() or not scale.is_contiguous() or weight.data_ptr() % 16 or scale.data_ptr() % 8:
             raise ValueError("PackedLinear: contiguous tensors, the weights on 16 bytes and the scales on 8")
-        self.weight, self.scale, self.in_features, self.group = weight, scale, int(in_features), int(group)
+        self._weight, self._scale, self.in_features, self.group = weight, scale, int(in_features), int(group)
         self.out_features, self.device, self.ordinal = weight.shape[0], weight.device, weight.get_device()
         self.bias = None if bias is None else bias.contiguous()
         self.at, self.scale_at = weight.data_ptr(), scale.data_ptr()
