@@ -6,7 +6,7 @@ import torch
 from test_lowbit_cpu import _cache, handle, host, lib  # noqa: F401
 from test_scheduler_cpu import StubEngine, _patch_rules_dev
 from whisperdrz_b200 import capi
-from whisperdrz_b200.lowbit import pack_linear
+from whisperdrz_b200.lowbit import QCache, pack_linear
 from whisperdrz_b200.transcriber import Transcriber
 
 
@@ -126,3 +126,18 @@ def test_operands_keep_the_tensors_that_their_addresses_belong_to():
         with pytest.raises(AttributeError):
             setattr(w, name, getattr(w, name).clone())
     assert (w.at, w.scale_at) == (w.weight.data_ptr(), w.scale.data_ptr())
+
+
+def test_store_refuses_keys_and_values_in_one_place(host):  # noqa: F811
+    """Rows of both would be rounded into the same bytes, in no order; attending over such a cache is all right."""
+    rows = torch.zeros(2, 128)
+    k, s = torch.zeros(2, 2, 128, 64, dtype=torch.int8), torch.zeros(2, 2, 2)
+    both, scales = torch.zeros(2, 2, 2, 128, 64, dtype=torch.int8), torch.zeros(2, 2, 2, 2)     # K and V of a slot side by side
+    for cache in (QCache(k, k, s, s), QCache(k, k.clone(), s, s), QCache(k, k, s, s.clone()), QCache(k[:1], k[:1], s[:1], s[1:])):
+        with pytest.raises(ValueError):
+            host.qcache_store(cache, rows, rows, [0, 1], [0, 0])
+        with pytest.raises(AttributeError):      # as far as the library, which this host does not have
+            host.qcache_attention(rows, cache, [0, 0], [1, 1])
+    for cache in (QCache(both[:, 0], both[:, 1], scales[:, 0], scales[:, 1]), QCache(k[:1], k[1:], s[:1], s[1:])):
+        with pytest.raises(AttributeError):
+            host.qcache_store(cache, rows, rows, [0, 1], [0, 0])

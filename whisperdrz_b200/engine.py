@@ -11,25 +11,9 @@ import torch
 
 from . import capi, frontend
 from .dims import ModelDimensions
-from .lowbit import HEAD_DIM, PackedLinear, QCache
+from .lowbit import HEAD_DIM, PackedLinear, QCache, rows_overlap
 
 _TORCH_DTYPE = {torch.float32: capi.WDZ_F32, torch.bfloat16: capi.WDZ_BF16}
-
-
-def _rows_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether a byte of one's rows is a byte of the other's.  Rows [n, width] with unit stride, none over another of its own."""
-    n = a.shape[0]
-    if n == 0:
-        return False
-    pa, pb = a.data_ptr(), b.data_ptr()
-    wa, wb = a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
-    sa = a.stride(0) * a.element_size() if n > 1 else wa
-    sb = b.stride(0) * b.element_size() if n > 1 else wb
-    if pa + (n - 1) * sa + wa <= pb or pb + (n - 1) * sb + wb <= pa:
-        return False
-    if sa == sb and wa <= (pb - pa) % sa <= sa - wb:     # columns of one product
-        return False
-    return any(max(0, (lo - wa - pa) // sa + 1) <= min(n - 1, (lo + wb - 1 - pa) // sa) for lo in range(pb, pb + n * sb, sb))
 
 
 def pack_weights(sd: dict, dims: ModelDimensions, dtype: torch.dtype, device) -> dict[str, torch.Tensor]:
@@ -517,6 +501,8 @@ class Engine:
         slots outside the cache are skipped."""
         width = cache.n_heads * HEAD_DIM
         self._here("the cache", cache.ordinal)
+        if not cache.apart:
+            raise ValueError("qcache_store: the cache's keys and values lie in one place")
         k, v = self._rows("k", k, width), self._rows("v", v, width)
         if k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError("k and v must have the same shape and type")
@@ -591,7 +577,7 @@ class Engine:
             self._here("out", out.get_device())
             out_step = out.stride(0)
             same = out.data_ptr() == at and to == code and (n == 1 or out_step == step)
-            if not same and _rows_overlap(q, out):
+            if not same and rows_overlap(q, out):
                 raise ValueError("out may be q itself, but not lie over a part of it")
         slots, lens = self._index("slots", slots, n), self._index("lens", lens, n)
         if n == 0:
@@ -631,7 +617,7 @@ class Engine:
             out = x.new_empty((M, N), dtype=torch.float32)
         else:
             self._f32_rows("out", out, M, N)
-            if _rows_overlap(x, out) or (residual is not None and add != out.data_ptr() and _rows_overlap(residual, out)):
+            if rows_overlap(x, out) or (residual is not None and add != out.data_ptr() and rows_overlap(residual, out)):
                 raise ValueError("out may be residual itself, but not lie over x or a part of residual")
         b = w.bias
         if b is not None and b.dtype is not x.dtype:

@@ -15,6 +15,22 @@ HEAD_DIM = 64
 SEGMENT = 128   # weights of a row that are packed together
 
 
+def rows_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether a byte of one's rows is a byte of the other's.  Rows [n, width] with unit stride, none over another of its own."""
+    n = a.shape[0]
+    if n == 0:
+        return False
+    pa, pb = a.data_ptr(), b.data_ptr()
+    wa, wb = a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
+    sa = a.stride(0) * a.element_size() if n > 1 else wa
+    sb = b.stride(0) * b.element_size() if n > 1 else wb
+    if pa + (n - 1) * sa + wa <= pb or pb + (n - 1) * sb + wb <= pa:
+        return False
+    if sa == sb and wa <= (pb - pa) % sa <= sa - wb:     # columns of one product
+        return False
+    return any(max(0, (lo - wa - pa) // sa + 1) <= min(n - 1, (lo + wb - 1 - pa) // sa) for lo in range(pb, pb + n * sb, sb))
+
+
 def _fixed(name: str) -> property:
     """A tensor whose address the operand has handed on: it may be written into, not replaced."""
     return property(lambda self: self.__dict__["_" + name])
@@ -56,6 +72,7 @@ class QCache:
         self.desc = capi.QCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), step, scale_step,
                                     n_slots, n_heads, n_tokens // BLOCK)
         self.ref = C.byref(self.desc)
+        self.apart = not (rows_overlap(k.flatten(1), v.flatten(1)) or rows_overlap(k_scale.flatten(1), v_scale.flatten(1)))
         self.scratch: dict = {}   # bytes of scratch by call shape, as the library told them
 
     @classmethod
