@@ -334,8 +334,8 @@ typedef struct wdz_qcache {
  *   q = rint(x / scale'), half to even (the quotient is rounded exactly)
  *   tokens of the block before the run: q' = rint(q * scale / scale') where the scale grew
  * Tokens behind the run keep their bytes, which are void until written.  An infinity is stored as the largest
- * value and a NaN as zero, without part in the scale, and the status word says WDZ_ENAN; a < 2^-117 stores
- * zeros.  Runs of slots outside [0, n_slots) are skipped.  A run outside the rows or the slot, and every run but
+ * value and a NaN as zero, without part in the scale, and the status word says WDZ_ENAN; a < 2^-117
+ * counts as 0 (a scale' of 0 stores zeros); quotients end at +-127.  Runs of slots outside [0, n_slots) are skipped.  A run outside the rows or the slot, and every run but
  * the last of several that name one slot, is not stored and the status word says WDZ_EINVAL.  max_run: the longest
  * run's length, as far as the host knows it (it sizes the launch, no more). */
 int wdz_qcache_store(wdz_engine* e, const wdz_qcache* cache, const void* k_dev, int64_t ldk, const void* v_dev, int64_t ldv,

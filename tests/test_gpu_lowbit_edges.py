@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_lowbit import U, _check_attend, _check_store, _cuda_cache, _filled, eng  # noqa: F401
+from test_gpu_lowbit import BF16, F32, U, _check_attend, _check_store, _cuda_cache, _filled, eng  # noqa: F401
 from whisperdrz_b200.capi import WdzError
 from whisperdrz_b200.lowbit import PackedLinear, pack_nibbles
 
@@ -132,3 +132,20 @@ def test_attention_with_the_largest_scale(eng):
     parts = _filled(3, 2, 2, seed=3)
     q = torch.randn(3, 128, generator=torch.Generator().manual_seed(0)) * 1e-38
     _check_attend(eng, parts, q, [2, 0, 1], [128, 64, 3], scale=2.9e38)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("old", [1e-45, 1e-40, 1e-38, 3e-37, 4e-36])
+def test_store_behind_a_scale_that_no_store_leaves(eng, old, dtype):
+    """Blocks whose scale lies below 2^-124 (a caller's own cache), continued with rows below 2^-117, which leave it: quotients
+    saturate at 127; and with ordinary rows, which replace it."""
+    g = torch.Generator().manual_seed(2)
+    small = torch.rand(5, 128, generator=g) * 1.1e-35 - 5.5e-36
+    small[1, ::2], small[2], small[3, ::3] = 0.0, 1e-38, -1e-40
+    for rows in (small, small * 3e35):
+        parts = _filled(5, 2, 1)
+        parts[2].fill_(old)
+        parts[3].fill_(old * 2)
+        _check_store(eng, parts, rows.to(dtype), rows.flip(0).to(dtype), [1], [3], [0, 5])
+        _check_store(eng, parts, rows.to(dtype), rows.flip(0).to(dtype), [0, 1, 2, 3, 4], [3, 60, 9, 1, 63])
+    eng.device_status()

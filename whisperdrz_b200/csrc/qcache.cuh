@@ -16,6 +16,7 @@ namespace wdz {
 constexpr int QC_BLOCK = WDZ_QCACHE_BLOCK;   // tokens that share a scale
 constexpr int QC_HD = 64;
 constexpr float QC_TINY = 6.0185310762e-36f;   // 2^-117: below it the store's remainders would underflow; such a block is zero
+constexpr float QC_LEAST = 4.7019774033e-38f;  // 2^-124: no store leaves a smaller scale than that of QC_TINY, but a caller's cache may
 
 struct QcView {
   int8_t *k, *v;
@@ -90,10 +91,13 @@ __device__ __forceinline__ uint2 qc_code8(const float (&x)[8], const QcDivisor& 
   }
   return qc_bytes(n);
 }
-__device__ __forceinline__ uint2 qc_settle8(const float (&x)[8], const QcDivisor& by) {
+// Eight values that need not be finite, and scales below QC_LEAST, which values below QC_TINY left as they were: 1 / scale may
+// overflow there and values be more than 127 scales, so both are taken 2^64 times.
+__device__ __forceinline__ uint2 qc_settle8(const float (&x)[8], float scale) {
+  const float lift = scale < QC_LEAST ? 18446744073709551616.0f : 1.0f, s = scale * lift, inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
   uint32_t n[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) n[i] = (uint32_t)qc_code(x[i], by.s, by.inv);
+  for (int i = 0; i < 8; ++i) n[i] = (uint32_t)qc_code(x[i] * lift, s, inv);
   return qc_bytes(n);
 }
 
@@ -333,12 +337,12 @@ __global__ void __launch_bounds__((SHARE == 1 ? 2 : SHARE) * 32) qcache_store_ke
       qc_recode(part * 32 + lane, 8 * (lo - b * QC_BLOCK), 32 * SHARE, [&](int i) { return kept + i; }, [&](int) { return ratio; });
     }
     const QcDivisor by(now);
-    if (odd) {
+    if (odd || now < QC_LEAST) {
 #pragma unroll 1
       for (int i = is; i < i1; i += SHARE) {
         float x[8];
         QcRaw<T>(mine + i * STEP).get(x);
-        if (t0 + 4 * i >= lo && t0 + 4 * i < hi) *reinterpret_cast<uint2*>(to + 4 * i * QC_HD) = qc_settle8(x, by);
+        if (t0 + 4 * i >= lo && t0 + 4 * i < hi) *reinterpret_cast<uint2*>(to + 4 * i * QC_HD) = qc_settle8(x, now);
       }
     } else {
 #pragma unroll 4
@@ -404,7 +408,7 @@ __global__ void __launch_bounds__(320, 3) qcache_step_kernel(QcStoreParams p, De
       float x[8];
       raw.get(x);
       const QcDivisor by(now);
-      *reinterpret_cast<uint2*>(place.q + (int64_t)run.p0 * QC_HD + 8 * c) = odd ? qc_settle8(x, by) : qc_code8(x, by);
+      *reinterpret_cast<uint2*>(place.q + (int64_t)run.p0 * QC_HD + 8 * c) = odd || now < QC_LEAST ? qc_settle8(x, now) : qc_code8(x, by);
       if (c == 0) {
         if (!kept || now > old) place.s[b] = now;
         if (kept && now > old) {
