@@ -4,7 +4,9 @@ import numpy as np
 import pytest
 import torch
 
+import lowbit_ref as ref
 from test_gpu_lowbit import BF16, F32, U, _check_attend, _check_store, _cuda_cache, _filled, eng  # noqa: F401
+from whisperdrz_b200 import capi
 from whisperdrz_b200.capi import WdzError
 from whisperdrz_b200.lowbit import PackedLinear, pack_nibbles
 
@@ -148,4 +150,56 @@ def test_store_behind_a_scale_that_no_store_leaves(eng, old, dtype):
         parts[3].fill_(old * 2)
         _check_store(eng, parts, rows.to(dtype), rows.flip(0).to(dtype), [1], [3], [0, 5])
         _check_store(eng, parts, rows.to(dtype), rows.flip(0).to(dtype), [0, 1, 2, 3, 4], [3, 60, 9, 1, 63])
+    eng.device_status()
+
+
+def _raw_attend(eng, cache, q, slots, lens, out, clear, scratch_bytes):
+    """The C call with a scratch of ``scratch_bytes``, none for 0."""
+    put = lambda x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    heads = q.shape[1] // 64
+    sl, ln = put(slots), put(lens)
+    scratch = torch.full((max(scratch_bytes, 16),), 255, dtype=torch.uint8, device="cuda")   # its contents count for nothing
+    rc = eng.lib.wdz_qcache_attention(eng.h, cache.ref, q.data_ptr(), q.stride(0), capi.WDZ_F32, heads, sl.data_ptr(), ln.data_ptr(),
+                                      q.shape[0], 0.125, out.data_ptr(), out.stride(0), capi.WDZ_F32, clear,
+                                      scratch.data_ptr() if scratch_bytes else None, scratch_bytes, eng._raw_stream())
+    assert rc == 0
+    return out
+
+
+@pytest.mark.parametrize("heads,group,tokens", [(4, 4, 20000), (2, 1, 9000), (1, 2, 12001), (2, 8, 33000)])
+def test_attention_of_long_rows_in_parts(eng, heads, group, tokens):
+    """A few long rows over all SMs, with query heads that share their keys; and the same rows with no scratch, or too little."""
+    parts = _filled(3, heads, (tokens + 63) // 64, seed=group, spread=0.2)
+    q = torch.randn(3, heads * group * 64, generator=torch.Generator().manual_seed(1)) * 0.3
+    lens = [tokens, 70, tokens // 2 + 1]
+    cache = _cuda_cache(parts)
+    got = _check_attend(eng, parts, q, [1, 2, 0], lens, cache=cache)
+    need = eng.lib.wdz_qcache_attention_scratch(eng.h, cache.ref, heads * group, 3)
+    assert need > 0
+    on = q.cuda()
+    for have in (need, 0, need - 4):
+        out = _raw_attend(eng, cache, on, [1, 2, 0], lens, torch.full_like(on, 7.0), 0, have)
+        if have == need:
+            assert torch.equal(out, got)
+        want, weight, top = ref.attend(q.numpy(), *(t.numpy() for t in parts), [1, 2, 0], lens, 0.125)
+        tol = top * (2 * 70 * U * weight + 2.0 ** -21 + np.asarray(lens, dtype=np.float64).reshape(-1, 1, 1) * 2.0 ** -23)
+        tol = np.repeat(tol.reshape(3, -1), 64, axis=1) + U * np.abs(want)
+        assert (np.abs(out.double().cpu().numpy() - want) <= tol).all(), have
+
+
+def test_attention_in_parts_of_skipped_and_empty_rows(eng):
+    cache = _cuda_cache(_filled(2, 2, 200, seed=1))
+    q = torch.randn(4, 256, generator=torch.Generator().manual_seed(1)).cuda()
+    slots, lens = [0, -1, 1, 2], [12000, 12000, 0, 5]
+    need = eng.lib.wdz_qcache_attention_scratch(eng.h, cache.ref, 4, 4)
+    assert need > 0
+    for have in (need, 0):
+        left = _raw_attend(eng, cache, q, slots, lens, torch.full((4, 256), 7.0, device="cuda"), 0, have)
+        assert (left[[1, 3]] == 7).all() and (left[2] == 0).all() and left[0].isfinite().all() and (left[0] != 7).any()
+        cleared = _raw_attend(eng, cache, q, slots, lens, torch.full((4, 256), 7.0, device="cuda"), 1, have)
+        assert (cleared[1:] == 0).all() and torch.equal(cleared[0], left[0])
+    kept = torch.full((4, 256), 7.0, device="cuda")
+    put = lambda x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    assert torch.equal(eng.qcache_attention(q, cache, put(slots), put(lens), out=kept)[[1, 2, 3]], torch.tensor([7.0, 0.0, 7.0], device="cuda")[:, None].expand(3, 256))
+    assert (eng.qcache_attention(q, cache, put(slots), put(lens))[1:] == 0).all()
     eng.device_status()
