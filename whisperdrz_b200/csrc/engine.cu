@@ -1909,12 +1909,20 @@ int qcache_view(wdz_engine* e, const char* who, const wdz_qcache* c, QcView* v) 
 // How a launch of qcache_attend_kernel is cut: warps to a CTA, CTAs to a cluster, lone CTAs (parts) to an item.
 struct QcAttendPlan { int warps, cluster, parts; };
 
+int qcache_attend_step(int pairs) { return 2 * pairs * (QC_HD + 2); }   // floats of a partial result
+// Its dynamic shared memory: the warps' rings, their partial results, and in a cluster those of its CTAs.
+int qcache_attend_smem(int warps, int cluster, int pairs) {
+  return warps * QC_RING + (int)sizeof(float) * qcache_attend_step(pairs) * (warps + (cluster > 1 ? cluster : 0));
+}
+
 // The cut with the shortest estimated time, in microseconds.  What it weighs: CTAs come to an SM whole, so 640 items of
 // 1500 tokens are 4 or 5 to an SM and take 23 us with three warps each (five such CTAs fit), 27 with four (four fit: a second
 // wave) and 26 with two (ten warps do not draw an SM's share of the bandwidth); rows of a few tiles are over before a CTA of
 // four warps has started (7680 items of 128 tokens: 26 us with one warp, 32 with two, 50 with four); few items need
-// clusters (20 items of 1500 tokens: 4.5 us in clusters, 6.5 without).  The constants are fitted to 19 shapes from
-// 80 to 7680 items of 2 to 24 tiles, where the cut it takes is 1 % slower than the best of 4 x 4 on average.
+// clusters (20 items of 1500 tokens: 4.5 us in clusters, 6.5 without).  What an SM holds is worked out from the launch; the other
+// constants are fitted to 19 shapes from 80 to 7680 items of 2 to 24 tiles, where the cut it takes is 1.5 % slower than the best
+// of 4 x 4 on average.  A tile's time does not know the query heads that share it: with eight the cut is up to half slower than
+// the best (6000 items of 1024 tokens: 381 us, 254 with one warp).
 QcAttendPlan qcache_attend_plan(const wdz_engine* e, int64_t items, int tiles, int pairs) {
   const double start = 3.0, per_tile = 1.2;              // a CTA's way to its first tile; a warp's time for a tile
   const double kb = 8.2e-3, warp_rate = 4.0e-3, sm_rate = 52.0e-3, full_rate = 50.0e-3;   // MB a tile; MB a microsecond
@@ -1930,16 +1938,16 @@ QcAttendPlan qcache_attend_plan(const wdz_engine* e, int64_t items, int tiles, i
   }
   // Rows of a few tiles in more than a wave of single-warp CTAs: such caches fill up token by token, so most rows are short
   // (lengths spread over 448 tokens: 40 us against 43 with two warps; all of 512 tokens: 79 against 76).
-  if (tiles <= 8 && pairs == 1 && items > 17 * sms) return QcAttendPlan{1, 1, 1};
+  if (tiles <= 8 && pairs == 1 && items > 16 * sms) return QcAttendPlan{1, 1, 1};
   QcAttendPlan best{4, 1, 1};
   double least = 1e30;
   const int even = tiles / 6 < 1 ? 1 : tiles / 6 > 4 ? 4 : tiles / 6;   // where the estimates agree: about six tiles a warp
   for (int warps = 1; warps <= 4; ++warps) {
-    static const int by_memory[5] = {0, 17, 8, 5, 4};                  // CTAs of an SM by their rings
-    const int by_registers = (pairs == 1 ? 20 : pairs == 2 ? 16 : 11) / warps;
-    const int fit = by_memory[warps] < by_registers ? by_memory[warps] : by_registers;
+    const int by_registers = (pairs == 1 ? 20 : pairs == 2 ? 16 : 8) / warps;   // 96, 126 and 176 a lane, and a quarter of the warps to each scheduler
     for (int cluster = 1; cluster <= 8; cluster *= 2) {
       if (cluster > 1 && (cluster - 1) * warps >= tiles) break;       // the last CTA would have no tile
+      const int by_memory = 228 * 1024 / (qcache_attend_smem(warps, cluster, pairs) + 1024);   // of an SM; 1 KB a CTA is the system's
+      const int fit = by_memory < by_registers ? by_memory : by_registers;
       const int each = (tiles + cluster - 1) / cluster;
       const double latency = start + (each + warps - 1) / warps * per_tile;
       auto wave = [&](double n, double top) {   // n CTAs of each SM at once
@@ -1966,7 +1974,7 @@ int64_t wdz_qcache_attention_scratch(const wdz_engine* e, const wdz_qcache* cach
   const int group = n_q_heads / cache->n_heads, pairs = group <= 2 ? 1 : group <= 4 ? 2 : 4;
   const int64_t items = (int64_t)n_rows * cache->n_heads;
   const QcAttendPlan plan = qcache_attend_plan(e, items, cache->n_blocks, pairs);
-  return plan.parts > 1 ? (int64_t)sizeof(float) * items * plan.parts * 2 * pairs * (QC_HD + 2) : 0;
+  return plan.parts > 1 ? (int64_t)sizeof(float) * items * plan.parts * qcache_attend_step(pairs) : 0;
 }
 
 int wdz_qcache_store(wdz_engine* e, const wdz_qcache* cache, const void* k_dev, int64_t ldk, const void* v_dev, int64_t ldv,
@@ -2039,7 +2047,7 @@ int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_d
   if ((rc = check_ready(e))) return rc;
   DeviceScope on(e->device);
   const int64_t items = (int64_t)n_rows * p.c.n_heads;
-  const int pairs = p.group <= 2 ? 1 : p.group <= 4 ? 2 : 4, step = 2 * pairs * (QC_HD + 2);
+  const int pairs = p.group <= 2 ? 1 : p.group <= 4 ? 2 : 4, step = qcache_attend_step(pairs);
   QcAttendPlan plan = qcache_attend_plan(e, items, p.c.n_blocks, pairs);
   if (plan.parts > 1) {
     const size_t need = sizeof(float) * (size_t)items * plan.parts * step;
@@ -2050,7 +2058,7 @@ int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_d
     return e->fail(WDZ_ECAPACITY, "wdz_qcache_attention: %d rows of %d heads", n_rows, p.c.n_heads);
   auto go = [&](auto kern) -> int {
     cudaLaunchConfig_t cfg{};
-    cfg.dynamicSmemBytes = (size_t)plan.warps * QC_RING + sizeof(float) * step * (plan.warps + (plan.cluster > 1 ? plan.cluster : 0));
+    cfg.dynamicSmemBytes = qcache_attend_smem(plan.warps, plan.cluster, pairs);
     cfg.gridDim = dim3((unsigned)(items * plan.cluster * plan.parts)); cfg.blockDim = dim3(plan.warps * 32); cfg.stream = (cudaStream_t)s;
     cudaLaunchAttribute attr[2];
     int n = 0;
