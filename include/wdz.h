@@ -343,10 +343,11 @@ int wdz_qcache_store(wdz_engine* e, const wdz_qcache* cache, const void* k_dev, 
                      const int32_t* positions_dev, int n_runs, int max_run, wdz_stream s);
 /* Row r's n_q_heads queries (q_dtype [n_rows][n_q_heads * 64]) attend to the first lens_dev[r] tokens of slot
  * slot_ids_dev[r]: out = softmax(scale * q k^T) v, query head h over key head h / (n_q_heads / n_heads), at most 8
- * query heads to a key head.  Queries and softmax weights are held to 2^-31 of the largest of their head or row,
- * everything else in fp32; out: out_dtype [n_rows][n_q_heads * 64], which may be q itself (its rows and type) and overlaps it in no other way.  Lengths are clamped to
- * the slot; a row of length 0 gives zeros; a row whose slot is outside [0, n_slots) is left as it was, or zeroed
- * when clear_skipped != 0. */
+ * query heads to a key head.  A query's values are rounded as fp32 is and then to steps of 2^-31 of their head's largest,
+ * softmax weights to 2^-21 of themselves and then to steps of 2^-32 of the largest so far (the sum that divides them has the
+ * weights before that step); everything else is fp32.  out: out_dtype [n_rows][n_q_heads * 64], which may be q itself (its rows
+ * and type) and overlaps it in no other way.  Lengths are clamped to the slot; a row of length 0 gives zeros; a row whose slot
+ * is outside [0, n_slots) is left as it was, or zeroed when clear_skipped != 0. */
 int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_dev, int64_t ldq, int q_dtype, int n_q_heads,
                          const int32_t* slot_ids_dev, const int32_t* lens_dev, int n_rows, float scale, void* out_dev,
                          int64_t ldo, int out_dtype, int clear_skipped, void* scratch_dev, size_t scratch_bytes, wdz_stream s);
@@ -354,12 +355,13 @@ int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_d
  * above takes a few long rows apart over all SMs; 0 where it wants none.  Without it those rows are slower. */
 int64_t wdz_qcache_attention_scratch(const wdz_engine* e, const wdz_qcache* cache, int n_q_heads, int n_rows);
 /* wdz_linear_rows with 4-bit weights: y f32 [M][N] = x[M][K] W^T (+ bias, x_dtype [N]) (+ residual f32 [M][N], which
- * may be y; y overlaps x and the residual in no other way), W[n][k] = (u - 8) * scale[n][k / group], group 32, 64 or 128.  w_dev: K is padded to Kp, a multiple of
- * 128, with u = 8; row n is Kp / 8 32-bit words; of every 128 weights word 4 t + i (t, i < 4) holds elements
+ * may be y; y overlaps x and the residual in no other way), W[n][k] = (u - 8) * scale[n][k / group], group 32, 64 or
+ * 128.  w_dev: K is padded to Kp, a multiple of 128, with u = 8; row n is Kp / 8 32-bit words; of every 128 weights word 4 t + i (t, i < 4) holds elements
  * 32 i + 8 t + 0..7, element 2 j in its bits 4 j, element 2 j + 1 in its bits 4 (j + 4).  scale_dev: bf16
- * [N][Kp / group].  w_dev starts on 16 bytes, scale_dev on 8; x rows may have any alignment.  Products are exact and
- * their sums fp32; bf16 rows are held exactly down to 2^-38 of their largest value, to 2^-46 of it below.  Of f32 rows and
- * of three bf16 rows or more, a group's sum before its scale has to fit fp32.  Scales of padding have to be finite.  Infinities and NaN in x give what the formula gives, in their row. */
+ * [N][Kp / group], finite in the padding too.  w_dev starts on 16 bytes, scale_dev on 8; x rows may have any alignment.
+ * Products are exact and their sums fp32.  One or two bf16 rows are held exactly down to 2^-38 of their largest value, to
+ * 2^-46 of it below; f32 rows exactly from 2^-110 on, smaller values down to 2^-133.  Of f32 rows and of three bf16 rows or
+ * more, a group's sum before its scale has to fit fp32.  Infinities and NaN in x give what the formula gives, in their row. */
 int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_dtype, int M, int K, const void* w_dev,
                            const void* scale_dev, int group, const void* bias_dev, const float* residual_dev, int N,
                            float* y_dev, wdz_stream s);

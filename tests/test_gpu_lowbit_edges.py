@@ -108,6 +108,20 @@ def test_linear_of_groups_with_far_scales(eng, m, group):
     assert (np.abs(got - x64 @ w.T) <= tol).all()
 
 
+@pytest.mark.parametrize("m", [1, 3, 9])
+@pytest.mark.parametrize("size", [1e-32, 1e-34, 1e-36, 1e-38, 1e-41])
+def test_linear_of_tiny_f32_rows(eng, size, m):
+    """Three bf16 pieces reach down to 2^-133: what a value holds below that is cut off."""
+    packed, w = _scaled(40, 300, 64, seed=m, scale=0.02)
+    x = torch.randn(m, 300, generator=torch.Generator().manual_seed(5)) * size
+    x64 = x.double().numpy()
+    want, total = x64 @ w.T, np.abs(x64) @ np.abs(w).T
+    got = eng.linear_rows_packed(x.cuda(), packed).double().cpu().numpy()
+    tol = 308 * U * total + 2.0 ** -133 * np.abs(w).sum(1) + 308 * 2.0 ** -150
+    err = np.abs(got - want)
+    assert (err <= tol).all(), float((err / tol).max())
+
+
 # ------------------------------------------------------------------ attention
 @pytest.mark.parametrize("group", [1, 2, 4])
 @pytest.mark.parametrize("size", [1e-35, 1e-32, 1e-28, 1e-24, 1e30, 1e34])
