@@ -128,6 +128,16 @@ def test_operands_keep_the_tensors_that_their_addresses_belong_to():
     assert (w.at, w.scale_at) == (w.weight.data_ptr(), w.scale.data_ptr())
 
 
+def test_a_bias_stays_the_one_that_was_checked():
+    """Its length, type and device are looked at when the operand is made."""
+    w = pack_linear(torch.zeros(4, 128), bias=torch.zeros(4))
+    for bad in (torch.zeros(3), torch.zeros(4, device="meta"), None):
+        with pytest.raises(AttributeError):
+            w.bias = bad
+    w.bias.fill_(2.0)
+    assert (w.bias == 2).all()
+
+
 def test_store_refuses_keys_and_values_in_one_place(host):  # noqa: F811
     """Rows of both would be rounded into the same bytes, in no order; attending over such a cache is all right."""
     rows = torch.zeros(2, 128)

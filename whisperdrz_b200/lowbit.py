@@ -32,7 +32,7 @@ def rows_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _fixed(name: str) -> property:
-    """A tensor whose address the operand has handed on: it may be written into, not replaced."""
+    """A tensor that was checked, and whose address may have been handed on: it may be written into, not replaced."""
     return property(lambda self: self.__dict__["_" + name])
 
 
@@ -89,7 +89,7 @@ class PackedLinear:
     (wdz_linear_rows_packed), ``scale`` bf16 [N, Kp / group], optional ``bias`` [N]; Kp is ``in_features`` rounded up
     to a multiple of 128."""
 
-    weight, scale = map(_fixed, ("weight", "scale"))
+    weight, scale, bias = map(_fixed, ("weight", "scale", "bias"))
 
     def __init__(self, weight: torch.Tensor, scale: torch.Tensor, in_features: int, group: int, bias: torch.Tensor | None = None):
         if group not in (32, 64, 128):
@@ -107,7 +107,7 @@ class PackedLinear:
             raise ValueError("PackedLinear: contiguous tensors, the weights on 16 bytes and the scales on 8")
         self._weight, self._scale, self.in_features, self.group = weight, scale, int(in_features), int(group)
         self.out_features, self.device, self.ordinal = weight.shape[0], weight.device, weight.get_device()
-        self.bias = None if bias is None else bias.contiguous()
+        self._bias = None if bias is None else bias.contiguous()
         self.at, self.scale_at = weight.data_ptr(), scale.data_ptr()
 
 
