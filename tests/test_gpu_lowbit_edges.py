@@ -122,6 +122,21 @@ def test_linear_of_tiny_f32_rows(eng, size, m):
     assert (err <= tol).all(), float((err / tol).max())
 
 
+@pytest.mark.parametrize("m", [1, 2, 5])
+def test_linear_of_a_bias_that_is_not_rounded(eng, m):
+    """bf16 rows round a bias to their own type; as the residual it is added in f32."""
+    packed, w = _scaled(200, 512, 64, seed=m, scale=0.02)
+    b = torch.randn(200, generator=torch.Generator().manual_seed(1))
+    x = torch.randn(m, 512, generator=torch.Generator().manual_seed(2)).bfloat16()
+    x64 = x.double().numpy()
+    got = eng.linear_rows_packed(x.cuda(), packed, residual=b.expand(m, 200).contiguous().cuda()).double().cpu().numpy()
+    tol = 520 * U * (np.abs(x64) @ np.abs(w).T + np.abs(b.double().numpy())) + 2.0 ** -46 * np.abs(x64).max(1, keepdims=True) * np.abs(w).sum(1)
+    assert (np.abs(got - (x64 @ w.T + b.double().numpy())) <= tol).all()
+    own = PackedLinear(packed.weight, packed.scale, 512, 64, b.cuda())
+    rounded = PackedLinear(packed.weight, packed.scale, 512, 64, b.bfloat16().cuda())
+    assert torch.equal(eng.linear_rows_packed(x.cuda(), own), eng.linear_rows_packed(x.cuda(), rounded))
+
+
 # ------------------------------------------------------------------ attention
 @pytest.mark.parametrize("group", [1, 2, 4])
 @pytest.mark.parametrize("size", [1e-35, 1e-32, 1e-28, 1e-24, 1e30, 1e34])

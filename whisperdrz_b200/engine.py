@@ -596,7 +596,11 @@ class Engine:
     def linear_rows_packed(self, x: torch.Tensor, w: PackedLinear, residual: torch.Tensor | None = None,
                            out: torch.Tensor | None = None) -> torch.Tensor:
         """``linear_rows`` with 4-bit weights (``lowbit.pack_linear``): x f32 or bf16 [M, K] @ W[N, K].T (+ bias)
-        (+ residual f32 [M, N]) -> f32 [M, N].  ``residual`` and ``out`` may be the same tensor; ``out`` may not lie over x."""
+        (+ residual f32 [M, N]) -> f32 [M, N].  ``residual`` and ``out`` may be the same tensor; ``out`` may not lie over x.
+
+        As in ``linear_rows`` the bias has the rows' type: one of the other type is converted in every call, which rounds an
+        f32 bias to bf16 under bf16 rows and costs a launch.  An f32 bias that must not be rounded goes in with ``residual``,
+        which is added in f32."""
         code, ordinal = _TORCH_DTYPE.get(x.dtype), self._ordinal
         if code is None or x.dim() != 2:
             raise ValueError(f"x must be [rows, {w.in_features}] in float32 or bfloat16, got {x.dtype} {tuple(x.shape)}")
@@ -621,7 +625,7 @@ class Engine:
                 raise ValueError("out may be residual itself, but not lie over x or a part of residual")
         b = w.bias
         if b is not None and b.dtype is not x.dtype:
-            b = b.to(x.dtype)
+            b = b.to(x.dtype)   # not kept: the caller may write into the bias
         rc = self.lib.wdz_linear_rows_packed(
             self.h, x.data_ptr(), step, code, M, K, w.at, w.scale_at, w.group, None if b is None else b.data_ptr(), add, N,
             out.data_ptr(), torch._C._cuda_getCurrentRawStream(ordinal))

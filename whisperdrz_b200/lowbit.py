@@ -86,8 +86,8 @@ class QCache:
 
 class PackedLinear:
     """A linear layer's weights in 4 bits: ``weight`` uint8 [N, Kp / 2] in the order of include/wdz.h
-    (wdz_linear_rows_packed), ``scale`` bf16 [N, Kp / group], optional ``bias`` [N]; Kp is ``in_features`` rounded up
-    to a multiple of 128."""
+    (wdz_linear_rows_packed), ``scale`` bf16 [N, Kp / group], optional ``bias`` [N], best in the type of the rows to
+    come (one of the other type is converted in every call); Kp is ``in_features`` rounded up to a multiple of 128."""
 
     weight, scale, bias = map(_fixed, ("weight", "scale", "bias"))
 
