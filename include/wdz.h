@@ -361,7 +361,9 @@ int64_t wdz_qcache_attention_scratch(const wdz_engine* e, const wdz_qcache* cach
  * [N][Kp / group], finite in the padding too.  w_dev starts on 16 bytes, scale_dev on 8; x rows may have any alignment.
  * Products are exact and their sums fp32.  One or two bf16 rows are held exactly down to 2^-38 of their largest value, to
  * 2^-46 of it below; f32 rows exactly from 2^-110 on, smaller values down to 2^-133.  Of f32 rows and of three bf16 rows or
- * more, a group's sum before its scale has to fit fp32.  Infinities and NaN in x give what the formula gives, in their row. */
+ * more, a group's sum before its scale has to fit fp32.  Infinities and NaN in x give what the formula gives, in their row.
+ * Made for few rows: every 16 bf16 (8 f32) rows take the weights apart anew.  From about 48 bf16 rows on (1280 -> 3840; 128 for
+ * 1280 -> 1280 and 5120 -> 1280) wdz_linear_rows on bf16 weights takes less time, at 384 rows a sixth. */
 int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_dtype, int M, int K, const void* w_dev,
                            const void* scale_dev, int group, const void* bias_dev, const float* residual_dev, int N,
                            float* y_dev, wdz_stream s);

@@ -2155,7 +2155,8 @@ int wdz_linear_rows_packed(wdz_engine* e, const void* x_dev, int64_t ldx, int x_
   using three = std::integral_constant<int, 3>;
   using four = std::integral_constant<int, 4>;
   // Two rows and fewer in bf16 leave six of a tile's columns empty: there bytes are cheaper (51866 features: one row 9.1 us,
-  // two 11.1, on bf16 operands 11.7 for either).
+  // two 11.3, on bf16 operands 11.7 for either).  Not so where x is taken apart for few features: two rows, 1280 -> 3840, 5.0 us,
+  // four on bf16 operands 3.1.
   if (x_dtype == WDZ_F32)
     by_group([&](auto gs) {
       if (M <= 2) mma(0.0f, one(), gs);

@@ -598,6 +598,7 @@ class Engine:
         """``linear_rows`` with 4-bit weights (``lowbit.pack_linear``): x f32 or bf16 [M, K] @ W[N, K].T (+ bias)
         (+ residual f32 [M, N]) -> f32 [M, N].  ``residual`` and ``out`` may be the same tensor; ``out`` may not lie over x.
 
+        Made for few rows: from about 48 bf16 rows on ``linear_rows`` on bf16 weights takes less time (include/wdz.h).
         As in ``linear_rows`` the bias has the rows' type: one of the other type is converted in every call, which rounds an
         f32 bias to bf16 under bf16 rows and costs a launch.  An f32 bias that must not be rounded goes in with ``residual``,
         which is added in f32."""
