@@ -576,8 +576,9 @@ class Engine:
                 raise ValueError(f"out must be [{n}, {width}] rows in float32 or bfloat16 that start on 16 bytes")
             self._here("out", out.get_device())
             out_step = out.stride(0)
-            same = out.data_ptr() == at and to == code and (n == 1 or out_step == step)
-            if not same and rows_overlap(q, out):
+            to_at, q_size, out_size = out.data_ptr(), 2 if code else 4, 2 if to else 4
+            same = to_at == at and to == code and (n == 1 or out_step == step)
+            if not same and rows_overlap(n, at, step * q_size, width * q_size, to_at, out_step * out_size, width * out_size):
                 raise ValueError("out may be q itself, but not lie over a part of it")
         slots, lens = self._index("slots", slots, n), self._index("lens", lens, n)
         if n == 0:
@@ -622,7 +623,9 @@ class Engine:
             out = x.new_empty((M, N), dtype=torch.float32)
         else:
             self._f32_rows("out", out, M, N)
-            if rows_overlap(x, out) or (residual is not None and add != out.data_ptr() and rows_overlap(residual, out)):
+            size, to_at = 2 if code else 4, out.data_ptr()
+            if (rows_overlap(M, x.data_ptr(), step * size, K * size, to_at, 4 * N, 4 * N)
+                    or (add is not None and add != to_at and abs(add - to_at) < 4 * M * N)):
                 raise ValueError("out may be residual itself, but not lie over x or a part of residual")
         b = w.bias
         if b is not None and b.dtype is not x.dtype:

@@ -15,33 +15,37 @@ HEAD_DIM = 64
 SEGMENT = 128   # weights of a row that are packed together
 
 
-def rows_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether a byte of one's rows is a byte of the other's.  Rows [n, width] with unit stride, none over another of its own."""
-    n = a.shape[0]
-    if n == 0:
+def rows_overlap(n: int, a: int, a_step: int, a_width: int, b: int, b_step: int, b_width: int) -> bool:
+    """Whether a byte of one's ``n`` rows is a byte of the other's: first row's address, bytes from row to row and of a row (the
+    step counts for nothing where n is 1, and no row lies over another of its own)."""
+    if n < 2:
+        return n == 1 and a < b + b_width and b < a + a_width
+    if a + (n - 1) * a_step + a_width <= b or b + (n - 1) * b_step + b_width <= a:
         return False
-    pa, pb = a.data_ptr(), b.data_ptr()
-    wa, wb = a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
-    sa = a.stride(0) * a.element_size() if n > 1 else wa
-    sb = b.stride(0) * b.element_size() if n > 1 else wb
-    if pa + (n - 1) * sa + wa <= pb or pb + (n - 1) * sb + wb <= pa:
+    if a_step == b_step and a_width <= (b - a) % a_step <= a_step - b_width:     # columns of one product
         return False
-    if sa == sb and wa <= (pb - pa) % sa <= sa - wb:     # columns of one product
-        return False
-    return any(max(0, (lo - wa - pa) // sa + 1) <= min(n - 1, (lo + wb - 1 - pa) // sa) for lo in range(pb, pb + n * sb, sb))
+    return any(max(0, (lo - a_width - a) // a_step + 1) <= min(n - 1, (lo + b_width - 1 - a) // a_step)
+               for lo in range(b, b + n * b_step, b_step))
 
 
-def _fixed(name: str) -> property:
-    """A tensor that was checked, and whose address may have been handed on: it may be written into, not replaced."""
-    return property(lambda self: self.__dict__["_" + name])
+class _Operand:
+    """Holds tensors that were checked and whose addresses have been handed on: they may be written into, not replaced.  A hook
+    on writes, so that reading one costs no more than any attribute."""
+    _fixed: tuple = ()
+    _made = False
+
+    def __setattr__(self, name, value):
+        if self._made and name in self._fixed:
+            raise AttributeError(f"{type(self).__name__}: {name} cannot be replaced")
+        super().__setattr__(name, value)
 
 
-class QCache:
+class QCache(_Operand):
     """An 8-bit cache by its tensors: ``k`` / ``v`` int8 [n_slots, n_heads, 64 * n_blocks, 64], ``k_scale`` / ``v_scale``
     f32 [n_slots, n_heads, n_blocks].  A token's values are its int8 times the scale of its block of 64 tokens.  Slots may
     lie further apart than their size (a layer of a larger allocation); K and V alike."""
 
-    k, v, k_scale, v_scale = map(_fixed, ("k", "v", "k_scale", "v_scale"))
+    _fixed = ("k", "v", "k_scale", "v_scale")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.dim() != 4 or k.shape[3] != HEAD_DIM or k.shape[2] == 0 or k.shape[2] % BLOCK or k.shape != v.shape:
@@ -67,13 +71,16 @@ class QCache:
             raise ValueError("QCache: the slots overlap")
         if step % 16 or k.data_ptr() % 16 or v.data_ptr() % 16:
             raise ValueError("QCache: values must start on 16 bytes")
-        self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_slots, self.n_heads, self.n_tokens, self.device, self.ordinal = n_slots, n_heads, n_tokens, k.device, k.get_device()
         self.desc = capi.QCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), step, scale_step,
                                     n_slots, n_heads, n_tokens // BLOCK)
         self.ref = C.byref(self.desc)
-        self.apart = not (rows_overlap(k.flatten(1), v.flatten(1)) or rows_overlap(k_scale.flatten(1), v_scale.flatten(1)))
+        size = n_heads * n_tokens * HEAD_DIM
+        self.apart = not (rows_overlap(n_slots, self.desc.k, step, size, self.desc.v, step, size)
+                          or rows_overlap(n_slots, self.desc.k_scale, 4 * scale_step, size // 1024, self.desc.v_scale, 4 * scale_step, size // 1024))
         self.scratch: dict = {}   # bytes of scratch by call shape, as the library told them
+        self._made = True
 
     @classmethod
     def empty(cls, n_slots: int, n_tokens: int, n_heads: int, device) -> "QCache":
@@ -84,12 +91,12 @@ class QCache:
                    torch.zeros(shape[:2] + (blocks,), device=device), torch.zeros(shape[:2] + (blocks,), device=device))
 
 
-class PackedLinear:
+class PackedLinear(_Operand):
     """A linear layer's weights in 4 bits: ``weight`` uint8 [N, Kp / 2] in the order of include/wdz.h
     (wdz_linear_rows_packed), ``scale`` bf16 [N, Kp / group], optional ``bias`` [N], best in the type of the rows to
     come (one of the other type is converted in every call); Kp is ``in_features`` rounded up to a multiple of 128."""
 
-    weight, scale, bias = map(_fixed, ("weight", "scale", "bias"))
+    _fixed = ("weight", "scale", "bias")
 
     def __init__(self, weight: torch.Tensor, scale: torch.Tensor, in_features: int, group: int, bias: torch.Tensor | None = None):
         if group not in (32, 64, 128):
@@ -105,10 +112,11 @@ class PackedLinear:
             raise ValueError("PackedLinear: the tensors lie on different devices")
         if not weight.is_contiguous() or not scale.is_contiguous() or weight.data_ptr() % 16 or scale.data_ptr() % 8:
             raise ValueError("PackedLinear: contiguous tensors, the weights on 16 bytes and the scales on 8")
-        self._weight, self._scale, self.in_features, self.group = weight, scale, int(in_features), int(group)
+        self.weight, self.scale, self.in_features, self.group = weight, scale, int(in_features), int(group)
         self.out_features, self.device, self.ordinal = weight.shape[0], weight.device, weight.get_device()
-        self._bias = None if bias is None else bias.contiguous()
+        self.bias = None if bias is None else bias.contiguous()
         self.at, self.scale_at = weight.data_ptr(), scale.data_ptr()
+        self._made = True
 
 
 def pack_linear(weight: torch.Tensor, group: int = 64, bias: torch.Tensor | None = None) -> PackedLinear:
