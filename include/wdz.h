@@ -318,7 +318,7 @@ int wdz_dtw(wdz_engine* e, const float* matrix_dev, int64_t chunk_stride, int64_
  * The cache: value(slot, head, token, c) = int8 * scale of the token's block of WDZ_QCACHE_BLOCK tokens.
  *   k_dev / v_dev              int8 [n_slots][n_heads][n_blocks * 64][64], slot_stride values from slot to slot
  *   k_scale_dev / v_scale_dev  f32  [n_slots][n_heads][n_blocks], scale_slot_stride scales from slot to slot
- * with n_heads <= 4096 and n_blocks <= 2^24. */
+ * with n_heads <= 4096 and n_blocks <= 2^24; what is stored to has K and V in memory of their own. */
 #define WDZ_QCACHE_BLOCK 64
 typedef struct wdz_qcache {
   void *k_dev, *v_dev;
@@ -345,7 +345,7 @@ int wdz_qcache_store(wdz_engine* e, const wdz_qcache* cache, const void* k_dev, 
  * slot_ids_dev[r]: out = softmax(scale * q k^T) v, query head h over key head h / (n_q_heads / n_heads), at most 8
  * query heads to a key head.  A query's values are rounded as fp32 is and then to steps of 2^-31 of their head's largest,
  * softmax weights to 2^-21 of themselves and then to steps of 2^-32 of the largest so far (the sum that divides them has the
- * weights before that step); everything else is fp32.  out: out_dtype [n_rows][n_q_heads * 64], which may be q itself (its rows
+ * weights before that step); everything else is fp32, in whose range scale * |q| * 2^-31 has to lie too.  out: out_dtype [n_rows][n_q_heads * 64], which may be q itself (its rows
  * and type) and overlaps it in no other way.  Lengths are clamped to the slot; a row of length 0 gives zeros; a row whose slot
  * is outside [0, n_slots) is left as it was, or zeroed when clear_skipped != 0. */
 int wdz_qcache_attention(wdz_engine* e, const wdz_qcache* cache, const void* q_dev, int64_t ldq, int q_dtype, int n_q_heads,

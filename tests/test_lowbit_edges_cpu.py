@@ -73,7 +73,7 @@ def test_index_tensors_keep_what_they_say(host):  # noqa: F811
     for t in (torch.uint8, torch.int16, torch.int32, torch.int64):
         x = host._index("lens", torch.tensor([3, 0], dtype=t), 2)
         assert x.dtype == torch.int32 and x.tolist() == [3, 0]
-    for bad in (torch.tensor([1.5, 2.0]), torch.tensor([True, False]), [1.5, 2.0], torch.tensor([1, 2, 3]), [1]):
+    for bad in (torch.tensor([1.5, 2.0]), torch.tensor([True, False]), torch.tensor([1, 2], dtype=torch.uint32), [1.5, 2.0], torch.tensor([1, 2, 3]), [1]):
         with pytest.raises(ValueError):
             host._index("slots", bad, 2)
     assert host._index("slots", [1, 2], 2).tolist() == [1, 2]

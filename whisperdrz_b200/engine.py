@@ -13,6 +13,7 @@ from . import capi, frontend
 from .dims import ModelDimensions
 from .lowbit import HEAD_DIM, PackedLinear, QCache, rows_overlap
 
+_INDEX_DTYPES = (torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64)
 _TORCH_DTYPE = {torch.float32: capi.WDZ_F32, torch.bfloat16: capi.WDZ_BF16}
 
 
@@ -470,8 +471,8 @@ class Engine:
         lo, hi = -2 ** 31, 2 ** 31 - 1
         if not isinstance(x, torch.Tensor):
             x = [min(max(v, lo), hi) for v in self._whole(name, x)]
-        elif x.dtype is torch.bool or x.is_floating_point() or x.is_complex():
-            raise ValueError(f"{name} must be whole numbers, got {x.dtype}")
+        elif x.dtype not in _INDEX_DTYPES:
+            raise ValueError(f"{name} must be whole numbers of a signed type or uint8, got {x.dtype}")
         elif x.dtype is torch.int64:
             x = x.clamp(lo, hi)
         x = self._i32(x)
